@@ -77,10 +77,23 @@ typedef enum lt_dtype {
  *               max|x| / 127, q = round(x / d) half away from zero, saturating
  *               to int8 (q = 0 when d = 0); d is kept as f16 (round to
  *               nearest even) and a value reads back as q * d.  0.53 of the
- *               f16 bytes per cached token. */
+ *               f16 bytes per cached token.
+ *   LT_KV_Q4_0  32-value groups of 4-bit codes with one f16 scale d; a value
+ *               reads back as (code - 8) * d, as a GGUF Q4_0 block's does
+ *               (quant.rs:254-275).  A group x is quantised as a = min(2720,
+ *               max|x| / 8 rounded to 8 significant bits, nearest even), kept
+ *               as f16; d = -a if the largest magnitude is a positive value
+ *               (also if both signs reach it), else a; code = clamp(floor(x / d
+ *               + 1/2) + 8, 0, 15), decided exactly; 8 when d = 0 or x is NaN
+ *               (NaN does not count in max|x|).  Magnitudes above 8 * 2720
+ *               saturate.  Every value (code - 8) * d is an f16.  0.28 of the
+ *               f16 bytes per cached token.  Calls that write or read such a
+ *               cache are refused inside a stream capture, and a write that
+ *               names a cell twice is refused. */
 typedef enum lt_kv_format {
     LT_KV_F16 = 0,
-    LT_KV_Q8_0 = 1
+    LT_KV_Q8_0 = 1,
+    LT_KV_Q4_0 = 2
 } lt_kv_format;
 
 typedef struct lt_kv lt_kv;
@@ -114,7 +127,7 @@ const char* lt_kv_last_error(const lt_kv* kv);
 /* The accessors below return 0 for a null handle. */
 /* KvCache::capacity (kv.rs:50-52): n_blocks * 16 tokens. Backend::n_ctx. */
 uint32_t lt_kv_capacity(const lt_kv* kv);
-/* KvCache::bytes (kv.rs:54-56): K + V pool bytes (LT_KV_Q8_0: values and
+/* KvCache::bytes (kv.rs:54-56): K + V pool bytes (quantised: values and
  * scales). */
 uint64_t lt_kv_bytes(const lt_kv* kv);
 /* KvCache::len (kv.rs:58-60): 0 for an unknown sequence. */
@@ -138,8 +151,8 @@ lt_status lt_kv_append(lt_kv* kv, const uint32_t* seq_host, const uint32_t* pos_
  * loop of Model::forward does (model.rs:414-429).  k and v are device arrays
  * [n][n_kv_heads * head_dim] of `dtype`.  LT_KV_F16: f32 is rounded to f16
  * with round-to-nearest-even (bit-identical to half::f16::from_f32), f16 is
- * stored unchanged.  LT_KV_Q8_0: each 32-value group of the given values
- * (f16 widened exactly) is quantised as lt_kv_format describes. */
+ * stored unchanged.  LT_KV_Q8_0, LT_KV_Q4_0: each 32-value group of the given
+ * values (f16 widened exactly) is quantised as lt_kv_format describes. */
 lt_status lt_kv_write(lt_kv* kv, uint32_t layer, const int32_t* block_host, const int32_t* slot_host,
                       uint32_t n, const void* k, const void* v, lt_dtype dtype, void* stream);
 
@@ -152,6 +165,32 @@ lt_status lt_kv_write(lt_kv* kv, uint32_t layer, const int32_t* block_host, cons
 lt_status lt_kv_attend(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype,
                        const uint32_t* seq_host, const uint32_t* pos_host, uint32_t n, void* out,
                        lt_dtype out_dtype, float scale, void* stream);
+
+/* Shape of the scores of an attention call.  No counterpart in the reference,
+ * whose closure is causal and plain.  For token i at position p = pos[i] and a
+ * cached position j, with s = scale * (q . k_j):
+ *   s = softcap * tanh(s / softcap)      if softcap > 0;
+ *   s = s - slopes[head] * |p - j|       if slopes (device f32 [n_heads]);
+ * and j takes part when max(first[i], p + 1 - window) <= j < end[i]:
+ * first_host NULL counts as 0, end_host NULL as p + 1 (causal), window 0 as no
+ * window.  end[i] may lie past p + 1 (a bidirectional prefix) but not past the
+ * sequence; a token whose interval is empty answers zero.  Blocks outside the
+ * interval are not read, and nothing that a masked cell holds (Inf, NaN)
+ * reaches an output. */
+typedef struct lt_kv_score {
+    float softcap;              /* finite, >= 0; 0: no cap                       */
+    uint32_t window;            /* positions before and with the token's own;    0: all */
+    const float* slopes;        /* device [n_heads], or NULL                     */
+    const uint32_t* first_host; /* [n] first position attended, or NULL          */
+    const uint32_t* end_host;   /* [n] one past the last, <= length, or NULL     */
+} lt_kv_score;
+
+/* lt_kv_attend with shaped scores, over a cache of any format; the same
+ * arguments, types and arithmetic otherwise.  Refused inside a stream capture. */
+lt_status lt_kv_attend_shaped(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype,
+                              const uint32_t* seq_host, const uint32_t* pos_host, uint32_t n,
+                              const lt_kv_score* score, void* out, lt_dtype out_dtype, float scale,
+                              void* stream);
 
 /* write + attend in one kernel launch (the K/V rows of each token are
  * written by the attention work item that covers them, then attended to).
@@ -189,9 +228,17 @@ lt_status lt_kv_flush(lt_kv* kv, void* stream);
 /* KvCache::rows (kv.rs:135-150): gather rows [0, n) of seq in `layer` into
  * device arrays k_out / v_out [n][n_kv_heads * head_dim] (f16, reference
  * row layout).  LT_KV_Q8_0: each value is q * d rounded to f16 (nearest
- * even). */
+ * even).  LT_KV_Q4_0: (code - 8) * d, exactly. */
 lt_status lt_kv_rows(lt_kv* kv, uint32_t layer, uint32_t seq, uint32_t n, void* k_out, void* v_out,
                      void* stream);
+
+/* The inverse of lt_kv_write: values of n cells of one layer into device
+ * arrays k_out / v_out [n][n_kv_heads * head_dim] of `dtype`, 16-byte aligned.
+ * A cell may be named more than once.  f32 holds every format's values exactly;
+ * f16 rounds LT_KV_Q8_0's q * d (nearest even) and nothing else.  New: the
+ * reference reads its cells in place.  Refused inside a stream capture. */
+lt_status lt_kv_read(lt_kv* kv, uint32_t layer, const int32_t* block_host, const int32_t* slot_host, uint32_t n,
+                     void* k_out, void* v_out, lt_dtype dtype, void* stream);
 
 /* Reads (and clears) the device error flag set by bounded waits in the
  * kernels; synchronises `stream`.  LT_OK or LT_E_TIMEOUT / LT_E_CUDA, or
@@ -249,6 +296,15 @@ uint32_t lt_kv_n_blocks(const lt_kv* kv);
  *   [32D, 33D)  K scales, f16 [D/32 groups][16]: group c of slot s at
  *               element 16*c + pos(s);
  *   [33D, 34D)  V scales, the same.
+ * LT_KV_Q4_0: [layer][block][kv_head] tiles of 18*head_dim bytes:
+ *   [0, 8D)     K codes, [8D, 16D) V codes, in 512-byte runs (64 values of 16
+ *               slots each); with w(i, g, t) = 512*(i/4) + 16*(4*g + t) + 4*(i%4),
+ *               the code of value e of slot s is in byte
+ *               K: w(e/16, s%8, (e%8)/2) + 2*(e%2) + s/8,
+ *               V: w(e/16, e%8, (s%8)/2) + 2*(s%2) + s/8,
+ *               its low nibble when e%16 < 8, else its high one;
+ *   [16D, 17D)  K scales, f16 [s%8][s/8][D/32 groups];
+ *   [17D, 18D)  V scales, f16 [(s%8)/2][D/32 groups][2*(s/8) + s%2].
  * Returns the device base address. */
 void* lt_kv_device_pool(const lt_kv* kv);
 /* Device block tables: int32 [max_seqs][max_blocks_per_seq]. */
@@ -296,7 +352,8 @@ lt_status lt_kv_set_min_tiles_per_warp(lt_kv* kv, uint32_t tiles);
  * the decode launch then covers only each token's own blocks and folds the
  * prefix result in (online-softmax merge, f32).  Default 8; 0 turns it off.
  * Calls of more than 1024 tokens (or max_batch) never use it, nor does an
- * LT_KV_Q8_0 cache (its tiles are not tensor-core f16 operands). */
+ * LT_KV_Q8_0 or LT_KV_Q4_0 cache (their tiles are not tensor-core f16
+ * operands) or a shaped call. */
 lt_status lt_kv_set_cascade(lt_kv* kv, uint32_t min_group_tokens);
 
 /* Prefix-pass launches issued by this handle since creation. */
@@ -371,8 +428,8 @@ lt_status lt_kv_write_attend_gather(lt_kv* kv, uint32_t layer, const int32_t* bl
  *   - pool_layer: the K/V tiles of one layer in the lt_kv_device_pool layout
  *     (lt_kv_device_pool(kv) + layer * n_blocks * n_kv_heads * 2 * 16 *
  *     head_dim halves), 16-byte aligned, holding n_blocks blocks;
- *     kv_format states its format and must be LT_KV_F16 (LT_KV_Q8_0 pools
- *     are refused with LT_E_UNSUPPORTED);
+ *     kv_format states its format and must be LT_KV_F16 (LT_KV_Q8_0 and
+ *     LT_KV_Q4_0 pools are refused with LT_E_UNSUPPORTED);
  *   - tables: device block tables, int32 [n_table_rows][max_blocks_per_seq],
  *     4-byte aligned;
  *   - host seq/pos arrays, device q and out (16-byte aligned).

@@ -21,13 +21,13 @@ LT_IPC_HANDLE_BYTES = 64
 LT_NOALLOC_SCRATCH_BYTES = 8 << 20
 LT_NOALLOC_MAX_TOKENS = 1024
 LT_F32, LT_F16 = 0, 1
-LT_KV_F16, LT_KV_Q8_0 = 0, 1
+LT_KV_F16, LT_KV_Q8_0, LT_KV_Q4_0 = 0, 1, 2
 BLOCK = 16
 
 # Every function include/lt_kv.h declares (tests check the export table).
 EXPORTS = (
     "lt_kv_create", "lt_kv_destroy", "lt_kv_last_error", "lt_kv_capacity", "lt_kv_bytes", "lt_kv_len",
-    "lt_kv_free_blocks", "lt_kv_append", "lt_kv_write", "lt_kv_attend", "lt_kv_write_attend",
+    "lt_kv_free_blocks", "lt_kv_append", "lt_kv_write", "lt_kv_attend", "lt_kv_attend_shaped", "lt_kv_write_attend", "lt_kv_read",
     "lt_kv_truncate", "lt_kv_share", "lt_kv_compact", "lt_kv_flush", "lt_kv_rows", "lt_kv_check",
     "lt_kv_seq_blocks", "lt_kv_refs", "lt_kv_free_list", "lt_kv_n_blocks", "lt_kv_device_pool",
     "lt_kv_device_tables", "lt_kv_read_pool", "lt_kv_launch_count", "lt_kv_profile", "lt_kv_profile_read", "lt_kv_profile_read_plan",
@@ -58,6 +58,16 @@ class lt_kv_config(C.Structure):
         ("max_blocks_per_seq", C.c_uint32),
         ("device", C.c_int32),
         ("kv_format", C.c_uint32),
+    ]
+
+
+class lt_kv_score(C.Structure):
+    _fields_ = [
+        ("softcap", C.c_float),
+        ("window", C.c_uint32),
+        ("slopes", C.c_void_p),
+        ("first_host", C.c_void_p),
+        ("end_host", C.c_void_p),
     ]
 
 
@@ -118,6 +128,8 @@ def _declare(L):
         "lt_kv_append": (st, [p, p, p, u32, p, p, C.POINTER(u32), p]),
         "lt_kv_write": (st, [p, u32, p, p, u32, p, p, C.c_int, p]),
         "lt_kv_attend": (st, [p, u32, p, C.c_int, p, p, u32, p, C.c_int, C.c_float, p]),
+        "lt_kv_attend_shaped": (st, [p, u32, p, C.c_int, p, p, u32, p, p, C.c_int, C.c_float, p]),
+        "lt_kv_read": (st, [p, u32, p, p, u32, p, p, C.c_int, p]),
         "lt_kv_write_attend": (st, [p, u32, p, p, p, p, C.c_int, p, C.c_int, p, p, u32, p, C.c_int,
                                     C.c_float, p]),
         "lt_kv_truncate": (None, [p, u32, u32]),

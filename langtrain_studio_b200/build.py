@@ -35,9 +35,9 @@ VARIANTS = {
               "-lasan", "-lubsan"]),
 }
 
-SOURCES = [CSRC / "lt_kv_kernels.cu", CSRC / "lt_kv.cpp", CSRC / "lt_kv_nccl.cpp", CSRC / "lt_kv_noalloc.cu",
+SOURCES = [CSRC / "lt_kv_kernels.cu", CSRC / "lt_kv_q4.cu", CSRC / "lt_kv.cpp", CSRC / "lt_kv_nccl.cpp", CSRC / "lt_kv_noalloc.cu",
            CSRC / "lt_llama.cu", CSRC / "lt_llama_decode.cu", CSRC / "lt_sched.cpp", CSRC / "lt_prefix.cpp"]
-HEADERS = [CSRC / "lt_kv_internal.h", CSRC / "lt_kv_layout.cuh", CSRC / "lt_q8_device.cuh", CSRC / "lt_llama_decode.h",
+HEADERS = [CSRC / "lt_kv_internal.h", CSRC / "lt_kv_layout.cuh", CSRC / "lt_kv_device.cuh", CSRC / "lt_q8_device.cuh", CSRC / "lt_llama_decode.h",
            INCLUDE / "lt_kv.h", INCLUDE / "lt_llama.h", INCLUDE / "lt_sched.h", INCLUDE / "lt_prefix.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

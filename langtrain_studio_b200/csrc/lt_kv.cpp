@@ -114,7 +114,7 @@ struct lt_kv {
     int casc_splits = 1;
     size_t casc_ntok = 0;  // tokens in the upload image's token list
     uint32_t n_blocks = 0, kv_dim = 0, group = 0, max_blocks = 0;
-    bool q8 = false;          // LT_KV_Q8_0 pool
+    int fmt = LT_KV_F16;      // lt_kv_format of the pool
     size_t block_elems = 0;   // 16-bit units of one block in one layer (all heads, K and V)
     size_t layer_elems = 0;   // 16-bit units of one layer of the pool
 
@@ -166,12 +166,17 @@ struct lt_kv {
     uint64_t plan_blocks = 0, plan_entries = 0;  // block copies and table entries of the timed plan launches
     uint64_t write_rows = 0, write_in_bytes = 0;  // rows and input bytes of the timed write launches
 
-    UploadCache cells_cache, items_cache, casc_cache;
+    UploadCache cells_cache, items_cache, casc_cache, shapes_cache;
     std::vector<ltkv::TokenDesc> toks_tmp;
     std::vector<std::pair<size_t, int32_t>> fold_tmp;  // (table index, previous shadow value)
     std::vector<uint32_t> fold_mark, fold_pos;         // per sequence, for one call
     uint32_t fold_epoch = 0;
-    ltkv::AttnParams params{};                         // large (inline descriptors): kept here
+    ltkv::AttnShapedParams params{};                   // large (inline descriptors): kept here
+    std::vector<uint32_t> apos_tmp;                    // shaped calls: last position each token attends
+    std::vector<ltkv::ShapeDesc> shapes_tmp;
+    // LT_KV_Q4_0 writes: slots of a block already named by the call (epoch << 16 | slot mask)
+    std::vector<uint64_t> cell_mark;
+    uint64_t cell_epoch = 0;
     std::vector<int2> cells_tmp;
     uint64_t launches = 0;
 };
@@ -451,6 +456,32 @@ lt_status check_cells(lt_kv* kv, const int32_t* block, const int32_t* slot, uint
     return LT_OK;
 }
 
+// Two rows of one call for the same cell would race on its bytes; a 4-bit cell
+// (codes and scale of one row) must not mix two.  LT_KV_Q4_0 only: the other
+// formats' writes keep the order they had.
+lt_status check_distinct_cells(lt_kv* kv, const int32_t* block, const int32_t* slot, uint32_t n) {
+    if (kv->fmt != LT_KV_Q4_0 || n < 2) return LT_OK;
+    if (kv->cell_mark.empty()) kv->cell_mark.assign(kv->n_blocks, 0);
+    const uint64_t ep = ++kv->cell_epoch << 16;
+    for (uint32_t i = 0; i < n; ++i) {
+        uint64_t& m = kv->cell_mark[block[i]];
+        if ((m & ~0xFFFFull) != ep) m = ep;
+        if (m >> slot[i] & 1) return fail(kv, LT_E_ARG, "cell %u (block %d, slot %d) is named twice", i, block[i], slot[i]);
+        m |= 1ull << slot[i];
+    }
+    return LT_OK;
+}
+
+// The launches of a call read staging slots and flags tagged for that call,
+// which a replayed graph would not refresh.
+lt_status refuse_capture(lt_kv* kv, cudaStream_t st, const char* what) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    LT_CUDA(kv, cudaStreamIsCapturing(st, &cs));
+    if (cs != cudaStreamCaptureStatusNone)
+        return fail(kv, LT_E_ARG, "%s cannot be captured into a graph: each call stages its own cells and flags", what);
+    return LT_OK;
+}
+
 constexpr size_t kProfPairs = 512;
 
 // Fold the oldest `n` recorded (start, end) pairs of a ring into its totals.
@@ -581,7 +612,8 @@ int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n
 
 lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype, const uint32_t* seq,
                       const uint32_t* pos, uint32_t n, void* out, lt_dtype out_dtype, float scale, const void* k,
-                      const void* v, lt_dtype kv_dtype, bool fused, cudaStream_t st, bool gather = false) {
+                      const void* v, lt_dtype kv_dtype, bool fused, cudaStream_t st, bool gather = false,
+                      const lt_kv_score* score = nullptr) {
     if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) ||
         (k && (reinterpret_cast<uintptr_t>(k) & 15)) || (v && (reinterpret_cast<uintptr_t>(v) & 15)))
         return fail(kv, LT_E_ARG, "q, out, k and v must be 16-byte aligned device pointers");
@@ -592,20 +624,40 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
                         kv->peer.max_tokens);
     }
     if (n == 0) return flush(kv, st);
+    if (score || kv->fmt == LT_KV_Q4_0)
+        if (lt_status crc = refuse_capture(kv, st, score ? "lt_kv_attend_shaped" : "attention over a 4-bit cache"))
+            return crc;
     // Per-token descriptors; the kernel derives its stream-K partition from them.
     const int q_f32 = q_dtype == LT_F32;
-    const int max_warps = ltkv::attend_warps(kv->cfg.device, (int)kv->group, (int)kv->cfg.head_dim, q_f32, kv->q8);
+    const int max_warps = ltkv::attend_warps(kv->cfg.device, (int)kv->group, (int)kv->cfg.head_dim, q_f32, kv->fmt,
+                                             score != nullptr);
     if (max_warps <= 0) return fail(kv, LT_E_CUDA, "could not size the attention launch on device %d", kv->cfg.device);
     kv->toks_tmp.resize(n);
+    // Shaped: the tiles of a token are the blocks of its interval alone; from
+    // here on `pos` is the last position it attends.
+    if (score) {
+        kv->apos_tmp.resize(n);
+        kv->shapes_tmp.resize(n);
+        for (uint32_t i = 0; i < n; ++i) {
+            uint32_t lo = score->first_host ? score->first_host[i] : 0;
+            const uint32_t end = score->end_host ? score->end_host[i] : pos[i] + 1;
+            if (score->window && pos[i] >= score->window) lo = std::max(lo, pos[i] + 1 - score->window);
+            const bool empty = lo >= end;
+            kv->shapes_tmp[i] = {(int32_t)(empty ? 1 : lo), (int32_t)pos[i]};
+            kv->apos_tmp[i] = empty ? 0 : end - 1;
+        }
+        pos = kv->apos_tmp.data();
+    }
     for (uint32_t i = 0; i < n; ++i) {
         ltkv::TokenDesc& t = kv->toks_tmp[i];
         t.seq = (int32_t)seq[i];
         t.pos = (int32_t)pos[i];
         t.last_block = kv->blocks[seq[i]][pos[i] / kBlock];
-        t.skip = 0;
+        t.skip = score && kv->shapes_tmp[i].lo <= t.pos ? kv->shapes_tmp[i].lo / kBlock : 0;
     }
-    // sets skip of the tokens it covers; Q8_0 tiles are not f16 tensor-core operands
-    const int n_items = kv->q8 ? 0 : plan_cascade(kv, seq, pos, n);
+    // sets skip of the tokens it covers; the quantised tiles are not f16
+    // tensor-core operands, and the pass does not shape scores
+    const int n_items = kv->fmt != LT_KV_F16 || score ? 0 : plan_cascade(kv, seq, pos, n);
     long long tiles = 0;
     for (uint32_t i = 0; i < n; ++i) {
         ltkv::TokenDesc& t = kv->toks_tmp[i];
@@ -645,7 +697,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         rollback();
         return rc;
     }
-    ltkv::AttnParams& p = kv->params;
+    ltkv::AttnShapedParams& p = kv->params;
     p.pool_layer = kv->d_pool + (size_t)layer * kv->layer_elems;
     p.pool_layer_w = kv->d_pool + (size_t)layer * kv->layer_elems;
     p.tables = kv->d_tables;
@@ -705,10 +757,32 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         }
         p.toks = static_cast<const ltkv::TokenDesc*>(d_toks);
     }
+    int s_shape = -1;
+    if (score) {
+        const float cap = score->softcap;
+        p.shape.capped = cap > 0.f;
+        p.shape.scale_cap = cap > 0.f ? scale / cap : 0.f;
+        p.shape.cap_log2 = cap * 1.4426950408889634f;
+        p.shape.scale_log2 = p.scale_log2;
+        p.shape.slopes = score->slopes;
+        p.shapes = nullptr;
+        if (n <= (uint32_t)ltkv::kInlineTokens) {
+            std::memcpy(p.inl_shapes, kv->shapes_tmp.data(), n * sizeof(ltkv::ShapeDesc));
+        } else {
+            const void* d_shapes = nullptr;
+            rc = upload(kv, kv->shapes_cache, kv->shapes_tmp.data(), n * sizeof(ltkv::ShapeDesc), st, &d_shapes,
+                        &s_shape);
+            if (rc) {
+                rollback();
+                return rc;
+            }
+            p.shapes = static_cast<const ltkv::ShapeDesc*>(d_shapes);
+        }
+    }
     p.pre_o = kv->d_pre_o;
     p.pre_ml = kv->d_pre_ml;
     p.pre_splits = n_items > 0 ? kv->casc_splits : 0;
-    p.q8 = kv->q8;
+    p.fmt = kv->fmt;
     p.pre_split_rows = (int64_t)kv->pre_cap * kv->cfg.n_heads;
     p.n_peers = 0;
     uint32_t g_epoch = 0;
@@ -763,7 +837,8 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         kv->launches++;
         kv->cascade_launches++;
     }
-    const cudaError_t le = ltkv::launch_attend(p, (int)kv->cfg.head_dim, st);
+    const cudaError_t le = score ? ltkv::launch_attend_shaped(p, (int)kv->cfg.head_dim, st)
+                                 : ltkv::launch_attend(p, (int)kv->cfg.head_dim, st);
     if (le != cudaSuccess) {
         rollback();
         return fail(kv, LT_E_CUDA, "attention launch: %s", cudaGetErrorString(le));
@@ -779,6 +854,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
                                                   srcs, out, n, slice, kv->d_err, st));
         kv->launches++;
     }
+    if (s_shape >= 0 && (rc = mark_slot_use(kv, s_shape, st)) != LT_OK) return rc;
     if (s_casc >= 0 && (rc = mark_slot_use(kv, s_casc, st)) != LT_OK) return rc;
     return s_plan >= 0 ? mark_slot_use(kv, s_plan, st) : LT_OK;
 }
@@ -809,7 +885,7 @@ lt_status lt_kv_create(const lt_kv_config* cfg, lt_kv** out) {
     if (c.n_heads % c.n_kv_heads != 0) return LT_E_ARG;
     if (c.head_dim != 64 && c.head_dim != 128) return LT_E_UNSUPPORTED;
     if (c.n_heads / c.n_kv_heads > (uint32_t)ltkv::kMaxGroup) return LT_E_UNSUPPORTED;
-    if (c.kv_format != LT_KV_F16 && c.kv_format != LT_KV_Q8_0) return LT_E_ARG;
+    if (c.kv_format != LT_KV_F16 && c.kv_format != LT_KV_Q8_0 && c.kv_format != LT_KV_Q4_0) return LT_E_ARG;
     lt_kv* kv = new (std::nothrow) lt_kv();
     if (!kv) return LT_E_ARG;
     kv->cfg = c;
@@ -823,9 +899,10 @@ lt_status lt_kv_create(const lt_kv_config* cfg, lt_kv** out) {
         return LT_E_ARG;
     }
     // 16-bit units of one block (all heads, K and V): f16 tiles of 2*16*D
-    // values, or Q8_0 tiles of 34*D bytes.
-    kv->q8 = c.kv_format == LT_KV_Q8_0;
-    kv->block_elems = (size_t)c.n_kv_heads * (kv->q8 ? 17 : 2 * kBlock) * c.head_dim;
+    // values, or Q8_0 (Q4_0) tiles of 34*D (18*D) bytes.
+    kv->fmt = (int)c.kv_format;
+    kv->block_elems = (size_t)c.n_kv_heads * c.head_dim *
+                      (kv->fmt == LT_KV_Q4_0 ? 9 : kv->fmt == LT_KV_Q8_0 ? 17 : 2 * kBlock);
     kv->layer_elems = (size_t)kv->n_blocks * kv->block_elems;
     kv->blocks.resize(c.max_seqs);
     kv->lens.assign(c.max_seqs, 0);
@@ -853,8 +930,11 @@ lt_status lt_kv_create(const lt_kv_config* cfg, lt_kv** out) {
         if (!g.ok) ck(cudaErrorInvalidDevice, "cudaSetDevice");
         const size_t pool_bytes = (size_t)c.n_layers * kv->layer_elems * 2;
         // Partial slots: a warp's first piece may be part of a split sequence.
-        const int max_warps = std::max(ltkv::attend_warps(c.device, (int)kv->group, (int)c.head_dim, 1, kv->q8),
-                                       ltkv::attend_warps(c.device, (int)kv->group, (int)c.head_dim, 0, kv->q8));
+        int max_warps = 0;
+        for (int shaped = 0; shaped < 2; ++shaped)
+            for (int q_f32 = 0; q_f32 < 2; ++q_f32)
+                max_warps = std::max(max_warps, ltkv::attend_warps(c.device, (int)kv->group, (int)c.head_dim, q_f32,
+                                                                   kv->fmt, shaped != 0));
         if (max_warps <= 0) ck(cudaErrorInvalidDevice, "attend_warps");
         kv->ws_slots = (size_t)std::max(max_warps, 0);  // one partial slot per warp
         const size_t gd = (size_t)kv->group * c.head_dim;
@@ -940,8 +1020,14 @@ lt_status lt_kv_write(lt_kv* kv, uint32_t layer, const int32_t* block, const int
     if (rc || (rc = require_device(kv))) return rc;
     if (layer >= kv->cfg.n_layers) return fail(kv, LT_E_ARG, "layer %u out of range", layer);
     if ((rc = check_cells(kv, block, slot, n))) return rc;
+    if ((rc = check_distinct_cells(kv, block, slot, n))) return rc;
     DeviceGuard g(kv->cfg.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (kv->fmt == LT_KV_Q4_0) {
+        if ((reinterpret_cast<uintptr_t>(k) & 15) || (reinterpret_cast<uintptr_t>(v) & 15))
+            return fail(kv, LT_E_ARG, "k and v must be 16-byte aligned device pointers");
+        if ((rc = refuse_capture(kv, st, "lt_kv_write to a 4-bit cache"))) return rc;
+    }
     if ((rc = flush(kv, st))) return rc;
     if (n == 0) return LT_OK;
     kv->cells_tmp.resize(n);
@@ -956,7 +1042,7 @@ lt_status lt_kv_write(lt_kv* kv, uint32_t layer, const int32_t* block, const int
         kv->write_in_bytes += (uint64_t)n * 2 * kv->cfg.n_kv_heads * kv->cfg.head_dim * (dtype == LT_F32 ? 4 : 2);
     }
     LT_CUDA(kv, ltkv::launch_write(kv->d_pool + (size_t)layer * kv->layer_elems, static_cast<const int2*>(d_cells),
-                                   (int)n, (int)kv->cfg.n_kv_heads, (int)kv->cfg.head_dim, k, v, dtype == LT_F32, kv->q8,
+                                   (int)n, (int)kv->cfg.n_kv_heads, (int)kv->cfg.head_dim, k, v, dtype == LT_F32, kv->fmt,
                                    st));
     if (ev_end) LT_CUDA(kv, cudaEventRecord(ev_end, st));
     kv->launches++;
@@ -1025,6 +1111,28 @@ lt_status lt_kv_attend(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtyp
     if (!kv) return LT_E_ARG;
     if (lt_status rc = check_dtypes(kv, {&q_dtype, &out_dtype})) return rc;
     return attend_entry(kv, layer, q, q_dtype, seq, pos, n, out, out_dtype, scale, stream, false);
+}
+
+lt_status lt_kv_attend_shaped(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype, const uint32_t* seq,
+                              const uint32_t* pos, uint32_t n, const lt_kv_score* score, void* out,
+                              lt_dtype out_dtype, float scale, void* stream) {
+    ltkv::NvtxRange nv("lt_kv_attend_shaped");
+    if (!kv) return LT_E_ARG;
+    lt_status rc = check_dtypes(kv, {&q_dtype, &out_dtype});
+    if (rc || (rc = require_device(kv))) return rc;
+    if (!score) return fail(kv, LT_E_ARG, "attend_shaped without a score");
+    if (layer >= kv->cfg.n_layers) return fail(kv, LT_E_ARG, "layer %u out of range", layer);
+    if ((rc = check_tokens(kv, seq, pos, n))) return rc;
+    if (!(score->softcap >= 0.f) || std::isinf(score->softcap))
+        return fail(kv, LT_E_ARG, "softcap %g is not a finite number >= 0", (double)score->softcap);
+    if (reinterpret_cast<uintptr_t>(score->slopes) & 3) return fail(kv, LT_E_ARG, "slopes must be 4-byte aligned");
+    for (uint32_t i = 0; i < n && score->end_host; ++i)
+        if (score->end_host[i] > kv->lens[seq[i]])
+            return fail(kv, LT_E_ARG, "token %u: end %u is past its sequence (length %u)", i, score->end_host[i],
+                        kv->lens[seq[i]]);
+    DeviceGuard g(kv->cfg.device);
+    return attend_impl(kv, layer, q, q_dtype, seq, pos, n, out, out_dtype, scale, nullptr, nullptr, LT_F32, false,
+                       static_cast<cudaStream_t>(stream), false, score);
 }
 
 lt_status lt_kv_write_attend(lt_kv* kv, uint32_t layer, const int32_t* block, const int32_t* slot, const void* k,
@@ -1252,9 +1360,36 @@ lt_status lt_kv_rows(lt_kv* kv, uint32_t layer, uint32_t seq, uint32_t n, void* 
     LT_CUDA(kv, ltkv::launch_rows(kv->d_pool + (size_t)layer * kv->layer_elems,
                                   kv->d_tables + (size_t)seq * kv->max_blocks, (int)n, (int)kv->cfg.n_kv_heads,
                                   (int)kv->cfg.head_dim, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out),
-                                  kv->q8, (int)kv->n_blocks, kv->d_err, st));
+                                  kv->fmt, (int)kv->n_blocks, kv->d_err, st));
     kv->launches++;
     return LT_OK;
+}
+
+lt_status lt_kv_read(lt_kv* kv, uint32_t layer, const int32_t* block, const int32_t* slot, uint32_t n, void* k_out,
+                     void* v_out, lt_dtype dtype, void* stream) {
+    ltkv::NvtxRange nv("lt_kv_read");
+    if (!kv) return LT_E_ARG;
+    lt_status rc = check_dtypes(kv, {&dtype});
+    if (rc || (rc = require_device(kv))) return rc;
+    if (layer >= kv->cfg.n_layers) return fail(kv, LT_E_ARG, "layer %u out of range", layer);
+    if ((rc = check_cells(kv, block, slot, n))) return rc;
+    if ((reinterpret_cast<uintptr_t>(k_out) & 15) || (reinterpret_cast<uintptr_t>(v_out) & 15))
+        return fail(kv, LT_E_ARG, "k_out and v_out must be 16-byte aligned device pointers");
+    DeviceGuard g(kv->cfg.device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if ((rc = refuse_capture(kv, st, "lt_kv_read"))) return rc;
+    if ((rc = flush(kv, st))) return rc;
+    if (n == 0) return LT_OK;
+    kv->cells_tmp.resize(n);
+    for (uint32_t i = 0; i < n; ++i) kv->cells_tmp[i] = make_int2(block[i], slot[i]);
+    const void* d_cells = nullptr;
+    int s = -1;
+    if ((rc = upload(kv, kv->cells_cache, kv->cells_tmp.data(), n * sizeof(int2), st, &d_cells, &s))) return rc;
+    LT_CUDA(kv, ltkv::launch_read(kv->d_pool + (size_t)layer * kv->layer_elems, static_cast<const int2*>(d_cells),
+                                  (int)n, (int)kv->cfg.n_kv_heads, (int)kv->cfg.head_dim, k_out, v_out,
+                                  dtype == LT_F32, kv->fmt, st));
+    kv->launches++;
+    return mark_slot_use(kv, s, st);
 }
 
 lt_status lt_kv_check(lt_kv* kv, void* stream) {

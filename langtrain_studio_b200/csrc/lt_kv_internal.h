@@ -81,7 +81,7 @@ struct AttnParams {
     const float* pre_ml;         // [pre_splits][rows][2]: its (m, l); row = (token*n_kv_heads + h)*group + g
     int32_t pre_splits;          // partials per row (the prefix blocks split over that many CTAs)
     int64_t pre_split_rows;      // rows between split slabs
-    int32_t q8;                  // pool tiles are Q8_0 (lt_kv.h LT_KV_Q8_0); no prefix partials then
+    int32_t fmt;                 // lt_kv_format of the pool's tiles; prefix partials only for LT_KV_F16
     // Head-sharded gather over NVLink (lt_kv_attend_gather).  With n_peers > 0
     // every output row goes, instead of to `out`, to this rank's gather half
     // gather_out at row tok*(n_peers*n_heads) + peer_rank*n_heads + head, and
@@ -96,6 +96,42 @@ struct AttnParams {
     uint32_t* peer_flag[kMaxPeers];
     TokenDesc inl[kInlineTokens];
 };
+
+// Score terms of a shaped call (lt_kv_score), the same for all its tokens.
+// q.k becomes, in log2 units, cap_log2 * tanh(q.k * scale_cap) with a cap,
+// else q.k * scale_log2; then slope * |distance| is taken off.
+struct ShapeTerms {
+    int32_t capped;
+    float scale_cap;      // scale / cap
+    float cap_log2;       // cap * log2(e)
+    float scale_log2;     // scale * log2(e)
+    const float* slopes;  // [n_heads], natural units, or null
+};
+
+// Per-token part of a shaped call beside its TokenDesc, whose pos is the last
+// position attended and whose skip counts the blocks before position lo.
+// An empty interval is described by one block with lo past pos.
+struct ShapeDesc {
+    int32_t lo;    // first position attended
+    int32_t qpos;  // the token's own position (distances count from it)
+};
+
+struct AttnShapedParams : AttnParams {
+    ShapeTerms shape;
+    const ShapeDesc* shapes;  // n_tok entries in global memory, or null: use inl_shapes
+    ShapeDesc inl_shapes[kInlineTokens];
+};
+
+template <bool SH>
+struct AttnParamsSel {
+    using type = AttnParams;
+};
+template <>
+struct AttnParamsSel<true> {
+    using type = AttnShapedParams;
+};
+template <bool SH>
+using AttnParamsOf = typename AttnParamsSel<SH>::type;
 
 // Shared-prefix (cascade) pass: one CTA per item attends up to
 // prefix_tokens_per_cta(group) tokens of one prefix group (128 query rows on
@@ -134,8 +170,14 @@ inline int prefix_tokens_per_cta(int group) { return 128 / group; }
 cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, cudaStream_t s);
 
 // Warps of one attention launch on `device` (all resident at once), or 0.
-int attend_warps(int device, int group, int head_dim, int q_f32, int q8);
+// fmt: lt_kv_format of the pool; shaped: the launch is launch_attend_shaped.
+int attend_warps(int device, int group, int head_dim, int q_f32, int fmt, bool shaped = false);
 cudaError_t launch_attend(const AttnParams& p, int head_dim, cudaStream_t s);
+cudaError_t launch_attend_shaped(const AttnShapedParams& p, int head_dim, cudaStream_t s);
+// The same for LT_KV_Q4_0 pools, on the current device (called by the above).
+int attend_q4_warps(int device, int group, int head_dim, int q_f32, bool shaped);
+cudaError_t launch_attend_q4(const AttnParams& p, int head_dim, cudaStream_t s);
+cudaError_t launch_attend_q4_shaped(const AttnShapedParams& p, int head_dim, cudaStream_t s);
 // Kernel launches made by launch_attend(p).
 int attend_launches(const AttnParams& p);
 
@@ -145,7 +187,13 @@ cudaError_t launch_gather_permute(const void* gathered, void* out, int nranks, u
                                   cudaStream_t s);
 
 cudaError_t launch_write(uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim,
-                         const void* k, const void* v, int in_f32, int q8, cudaStream_t s);
+                         const void* k, const void* v, int in_f32, int fmt, cudaStream_t s);
+cudaError_t launch_write_q4(uint8_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, const void* k,
+                            const void* v, int in_f32, cudaStream_t s);
+
+// Values of n cells of a pool of any format -> k_out, v_out [n][n_kv_heads*head_dim], f32 or f16.
+cudaError_t launch_read(const uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, void* k_out,
+                        void* v_out, int out_f32, int fmt, cudaStream_t s);
 
 // Block copies (copy-on-write and compaction moves) and table scatter.
 // copies: (src, dst) pairs; tw: (flat table index, value) pairs.  n_blocks
@@ -156,8 +204,10 @@ cudaError_t launch_apply_plan(uint16_t* pool, size_t layer_stride_elems, size_t 
                               int n_blocks, long long n_entries, int32_t* err, cudaStream_t s);
 
 cudaError_t launch_rows(const uint16_t* pool_layer, const int32_t* table_row, int n, int n_kv_heads,
-                        int head_dim, uint16_t* k_out, uint16_t* v_out, int q8, int n_blocks, int32_t* err,
+                        int head_dim, uint16_t* k_out, uint16_t* v_out, int fmt, int n_blocks, int32_t* err,
                         cudaStream_t s);
+cudaError_t launch_rows_q4(const uint8_t* pool_layer, const int32_t* table_row, int n, int n_kv_heads, int head_dim,
+                           uint16_t* k_out, uint16_t* v_out, int n_blocks, int32_t* err, cudaStream_t s);
 
 // One warp waits, through the kernels' bounded flag wait with a limit of
 // limit_ns, for a device word that nothing sets, then raises kErrTimeout in

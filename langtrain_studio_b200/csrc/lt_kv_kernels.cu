@@ -24,6 +24,7 @@
 
 #include <algorithm>
 
+#include "lt_kv_device.cuh"
 #include "lt_kv_internal.h"
 #include "lt_kv_layout.cuh"
 
@@ -34,188 +35,8 @@ constexpr int kWarps = 4;                         // warps per attention CTA
 constexpr int kStages = 3;                        // bulk-copy stages per warp (f16 tiles)
 constexpr int kStagesQ8 = 5;                      // the same for Q8_0 tiles (about half the bytes;
                                                   // 5 keeps two group-8 CTAs per SM)
-constexpr uint64_t kWaitLimitNs = 2000000000ull;  // bounded mbarrier wait: 2 s
-constexpr unsigned kFull = 0xffffffffu;
-
-// ------------------------------------------------------------- helpers ----
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ uint64_t global_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void fence_mbar_init() {
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-}
-
-__device__ __forceinline__ void fence_proxy_async_smem() {
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// Wait for `parity` of an mbarrier, giving up after kWaitLimitNs.
-__device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    for (uint32_t it = 1;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 15u) == 0 && global_ns() - t0 > kWaitLimitNs) return false;
-    }
-}
-
-// Non-multicast 1-D bulk copy global -> this CTA's shared memory.
-__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-        "l"(src), "r"(bytes), "r"(bar)
-        : "memory");
-}
-
-__device__ __forceinline__ void st_release_gpu(uint32_t* p, uint32_t v) {
-    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
-
-__device__ __forceinline__ uint32_t ld_acquire_gpu(const uint32_t* p) {
-    uint32_t v;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
-
-// System scope (another GPU over NVLink reads or writes the word).
-__device__ __forceinline__ void fence_acq_rel_sys() { asm volatile("fence.acq_rel.sys;" ::: "memory"); }
-
-__device__ __forceinline__ void st_relaxed_sys(uint32_t* p, uint32_t v) {
-    asm volatile("st.relaxed.sys.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
-
-__device__ __forceinline__ uint32_t ld_acquire_sys(const uint32_t* p) {
-    uint32_t v;
-    asm volatile("ld.acquire.sys.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ uint32_t atom_add_acq_rel_gpu(uint32_t* p, uint32_t v) {
-    uint32_t old;
-    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
-    return old;
-}
-
-
-// Wait until *flag == epoch, giving up after limit_ns.
-__device__ __forceinline__ int wait_flag_bounded(const uint32_t* flag, uint32_t epoch,
-                                                 uint64_t limit_ns = kWaitLimitNs) {
-    if (ld_acquire_gpu(flag) == epoch) return 1;
-    const uint64_t t0 = global_ns();
-    for (;;) {
-        __nanosleep(64);
-        if (ld_acquire_gpu(flag) == epoch) return 1;
-        if (global_ns() - t0 > limit_ns) return 0;
-    }
-}
-
-// A block id read from a block table.  Builds with LT_BOUNDS_CHECK test it
-// against the pool (n_blocks > 0), and so does every build when `check` is
-// set (tables the caller owns): a bad id raises kErrBounds and block 0
-// stands in for it, so the access stays inside the pool and only the
-// output is wrong (and reported).  Otherwise the host bookkeeping that
-// wrote the table is trusted.
-__device__ __forceinline__ int checked_block(int b, int n_blocks, int32_t* err, bool check = false) {
-#ifdef LT_BOUNDS_CHECK
-    check = true;
-#endif
-    if (check && n_blocks > 0 && (unsigned)b >= (unsigned)n_blocks) {
-        atomicOr(err, kErrBounds);
-        return 0;
-    }
-    return b;
-}
-
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-                 : "r"(addr));
-}
-
-__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-                 : "r"(addr));
-}
-
-// D(16x8 f32) += A(16x16 f16, row) * B(16x8 f16, col)
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// 2^x on the SFU (hardware instruction; relative error ~2^-22).
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
-// Load 8 consecutive input values (f32 or f16) and return them as 8 f16.
-__device__ __forceinline__ uint4 load8_as_f16(const void* base, size_t idx, int in_f32) {
-    uint4 r;
-    if (in_f32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + idx);
-        const float4 a = __ldg(p), b = __ldg(p + 1);
-        r.x = f32_to_f16_ref(a.x) | (uint32_t(f32_to_f16_ref(a.y)) << 16);
-        r.y = f32_to_f16_ref(a.z) | (uint32_t(f32_to_f16_ref(a.w)) << 16);
-        r.z = f32_to_f16_ref(b.x) | (uint32_t(f32_to_f16_ref(b.y)) << 16);
-        r.w = f32_to_f16_ref(b.z) | (uint32_t(f32_to_f16_ref(b.w)) << 16);
-    } else {
-        r = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + idx));
-    }
-    return r;
-}
 
 // ---------------------------------------------------------- Q8_0 tile ----
-__host__ __device__ constexpr int q8_tile_bytes(int D) { return 34 * D; }
-
-// Position of entry i (0..15) inside a 16-byte run: the order
-// 0,1,8,9, 2,3,10,11, 4,5,12,13, 6,7,14,15, so bytes 4t..4t+3 of a run hold
-// entries 2t, 2t+1, 2t+8, 2t+9 -- one lane's part of an m16n8k16 B fragment.
-__device__ __forceinline__ int q8_pos(int i) { return ((i & 7) >> 1) * 4 + ((i >> 3) << 1) + (i & 1); }
-
-// Byte offset of the 16-byte run of K values 16k..16k+15 of slot s: run
-// L = s*D/16 + k of the row-major K part, 128-byte lines swizzled by line.
-template <int D>
-__device__ __forceinline__ int q8_krun(int s, int k) {
-    const int L = s * (D / 16) + k;
-    return ((L >> 3) << 7) + (((L & 7) ^ ((L >> 3) & 7)) << 4);
-}
-
 // Four int8 (one 32-bit word) -> two f16x2, exactly: each biased byte
 // b = x + 128 becomes the f16 1024 + b (exponent 10, b in the mantissa),
 // then 1152 is subtracted.
@@ -227,24 +48,6 @@ __device__ __forceinline__ void i8x4_to_f16x2(uint32_t w, uint32_t& lo, uint32_t
     const __half2 hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
     lo = h2_bits(ha);
     hi = h2_bits(hb);
-}
-
-// Load 8 consecutive input values (f32, or f16 widened exactly).
-__device__ __forceinline__ void load8_f32(const void* base, size_t idx, int in_f32, float (&x)[8]) {
-    if (in_f32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + idx);
-        const float4 a = __ldg(p), b = __ldg(p + 1);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const uint4 r = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + idx));
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-            x[2 * j] = f.x;
-            x[2 * j + 1] = f.y;
-        }
-    }
 }
 
 // One 32-value group held as 8 values by each of the lanes 4j..4j+3 (all 32
@@ -384,6 +187,7 @@ __global__ void __launch_bounds__(256) kv_write_q8_kernel(uint8_t* __restrict__ 
 // this warp merges it.
 struct PieceRegs {
     int tok, h, seq, pos, b0, b1, kind, last_block, skip;  // b0, b1 count from block `skip`
+    int lo, qpos;  // shaped calls: first position attended, the token's own position
     long long ps;  // first tile of the (token, head)
 };
 
@@ -446,42 +250,6 @@ __device__ __forceinline__ void store_out(const AttnParams& p, int tok, int h, i
     }
 }
 
-// Peer gather: a warp is done and stored the output rows of `items`
-// (token, head) items into this rank's gather half (local memory).  Only
-// such warps take part: after the warp barrier, lane 0 adds the items to
-// this launch's count with an acq_rel RMW on this GPU, so the warp that
-// completes the count (n_tok * n_kv_heads items) has every row ordered
-// before it, in this GPU's memory.  It publishes this launch's epoch into
-// every rank's flag for this rank: one system-scope fence, then relaxed
-// system-scope stores (fence + store is a release; a release store per rank
-// would pay the fence once per rank).  A rank that acquires the flag then
-// reads the rows from here over NVLink.
-__device__ __forceinline__ void peer_done(const AttnParams& p, int lane, int items) {
-    if (p.n_peers == 0 || items == 0) return;
-    __syncwarp();
-    const uint32_t total = (uint32_t)p.n_tok * (uint32_t)p.n_kv_heads;
-    if (lane == 0 && atom_add_acq_rel_gpu(p.done_count, (uint32_t)items) + (uint32_t)items == total) {
-        *p.done_count = 0u;  // ready for the next launch (which starts after this one ends)
-        fence_acq_rel_sys();
-        for (int r = 0; r < p.n_peers; ++r) st_relaxed_sys(p.peer_flag[r], p.peer_epoch);
-    }
-}
-
-// Wait (bounded) until flags[w] == epoch for w = first, first + stride, ...
-// <= last; lane j polls every 32nd of them, so the round trips overlap.
-// Warp-uniform result.
-__device__ __forceinline__ bool wait_flags(const uint32_t* flags, uint32_t epoch, int first, int last, int stride,
-                                           int lane) {
-    int ready = 1;
-    for (int w0 = first; w0 <= last && ready; w0 += 32 * stride) {
-        int ok = 1;
-        const int w = w0 + lane * stride;
-        if (w <= last) ok = wait_flag_bounded(flags + w, epoch);
-        ready = __all_sync(kFull, ok);
-    }
-    return ready != 0;
-}
-
 // Fold the (m, l, O) partials in slots first, first + stride, ... <= last of
 // (po, pml) into the running (M, L, acc) of row g (log2 units; acc is the
 // unnormalised sum at maximum M), in one pass: each batch of U partials is
@@ -533,10 +301,12 @@ __device__ __forceinline__ void merge_slots(const float* po, const float* pml, i
 }
 
 // S = Q K^T, online softmax and O += P V for one staged (block, head) tile.
-template <int D>
+// SH: `sh` shapes the scores (before the mask) and masks the slots before its
+// first one too.
+template <int D, bool SH>
 __device__ __forceinline__ void attend_tile(const uint8_t* tile, int valid, const uint32_t (&qa)[D / 16][4],
                                             float (&o)[D / 8][4], float& m_run, float& l_run, float scale_log2,
-                                            int lane) {
+                                            int lane, const TileShape& sh) {
     constexpr int ROW = D * 2;
     constexpr int KS = D / 16;
     constexpr int NT = D / 8;
@@ -555,13 +325,29 @@ __device__ __forceinline__ void attend_tile(const uint8_t* tile, int valid, cons
             mma16816(s1, qa[ks], b2, b3);
         }
     }
-    float sc[4] = {(s0[0] + s0[2]) * scale_log2, (s0[1] + s0[3]) * scale_log2, (s1[0] + s1[2]) * scale_log2,
-                   (s1[1] + s1[3]) * scale_log2};
+    float sc[4];
+    if constexpr (SH) {
+        sc[0] = sh.score(s0[0] + s0[2], 2 * t);
+        sc[1] = sh.score(s0[1] + s0[3], 2 * t + 1);
+        sc[2] = sh.score(s1[0] + s1[2], 2 * t + 8);
+        sc[3] = sh.score(s1[1] + s1[3], 2 * t + 9);
+    } else {
+        sc[0] = (s0[0] + s0[2]) * scale_log2;
+        sc[1] = (s0[1] + s0[3]) * scale_log2;
+        sc[2] = (s1[0] + s1[2]) * scale_log2;
+        sc[3] = (s1[1] + s1[3]) * scale_log2;
+    }
     if (valid < kBlock) {
         if (2 * t >= valid) sc[0] = -INFINITY;
         if (2 * t + 1 >= valid) sc[1] = -INFINITY;
         if (2 * t + 8 >= valid) sc[2] = -INFINITY;
         if (2 * t + 9 >= valid) sc[3] = -INFINITY;
+    }
+    if (SH && sh.lo > 0) {
+        if (2 * t < sh.lo) sc[0] = -INFINITY;
+        if (2 * t + 1 < sh.lo) sc[1] = -INFINITY;
+        if (2 * t + 8 < sh.lo) sc[2] = -INFINITY;
+        if (2 * t + 9 < sh.lo) sc[3] = -INFINITY;
     }
     float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
     mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
@@ -569,9 +355,12 @@ __device__ __forceinline__ void attend_tile(const uint8_t* tile, int valid, cons
     const bool grow = mx > m_run;
     const float m_new = grow ? mx : m_run;
     const float alpha = grow ? ex2(m_run - m_new) : 1.f;
+    // A row that has seen nothing yet (SH: an empty interval) keeps m = -inf:
+    // its weights are ex2(-inf) = 0, not ex2(-inf + inf).
+    const float m_ref = SH && m_new == -INFINITY ? 0.f : m_new;
     float pr[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pr[e] = ex2(sc[e] - m_new);
+    for (int e = 0; e < 4; ++e) pr[e] = ex2(sc[e] - m_ref);
     l_run = l_run * alpha + ((pr[0] + pr[1]) + (pr[2] + pr[3]));
     m_run = m_new;
     if (__any_sync(kFull, grow)) {
@@ -615,10 +404,10 @@ __device__ __forceinline__ void attend_tile(const uint8_t* tile, int valid, cons
 // the slots' V scales (in f32, then split into f16 value + residual), so the
 // V bytes (again exact f16) go to the MMA unscaled.  Slots past `valid`
 // are masked out of S and contribute nothing to O, whatever their bytes.
-template <int D>
+template <int D, bool SH>
 __device__ __forceinline__ void attend_tile_q8(const uint8_t* tile, int valid, const uint32_t (&qa)[D / 16][4],
                                                float (&o)[D / 8][4], float& m_run, float& l_run, float scale_log2,
-                                               int lane) {
+                                               int lane, const TileShape& sh) {
     constexpr int G32 = D / 32;
     const int t = lane & 3;
     const int mi = lane >> 3, r = lane & 7;
@@ -647,13 +436,26 @@ __device__ __forceinline__ void attend_tile_q8(const uint8_t* tile, int valid, c
         sc[2] += d23.x * (t1[0] + t1[2]);
         sc[3] += d23.y * (t1[1] + t1[3]);
     }
+    if constexpr (SH) {
+        sc[0] = sh.score(sc[0], 2 * t);
+        sc[1] = sh.score(sc[1], 2 * t + 1);
+        sc[2] = sh.score(sc[2], 2 * t + 8);
+        sc[3] = sh.score(sc[3], 2 * t + 9);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sc[e] *= scale_log2;
+        for (int e = 0; e < 4; ++e) sc[e] *= scale_log2;
+    }
     // Slots past `valid` (only in a sequence's last block) are masked out of
     // S and weigh exactly 0 in O, whatever their stale bytes and scales.
-    const bool part = valid < kBlock;  // warp-uniform
-    const bool ok0 = !part || 2 * t < valid, ok1 = !part || 2 * t + 1 < valid, ok2 = !part || 2 * t + 8 < valid,
-               ok3 = !part || 2 * t + 9 < valid;
+    const bool part = valid < kBlock || (SH && sh.lo > 0);  // warp-uniform
+    bool ok0 = !part || 2 * t < valid, ok1 = !part || 2 * t + 1 < valid, ok2 = !part || 2 * t + 8 < valid,
+         ok3 = !part || 2 * t + 9 < valid;
+    if constexpr (SH) {
+        ok0 = ok0 && 2 * t >= sh.lo;
+        ok1 = ok1 && 2 * t + 1 >= sh.lo;
+        ok2 = ok2 && 2 * t + 8 >= sh.lo;
+        ok3 = ok3 && 2 * t + 9 >= sh.lo;
+    }
     if (part) {
         if (!ok0) sc[0] = -INFINITY;
         if (!ok1) sc[1] = -INFINITY;
@@ -666,9 +468,12 @@ __device__ __forceinline__ void attend_tile_q8(const uint8_t* tile, int valid, c
     const bool grow = mx > m_run;
     const float m_new = grow ? mx : m_run;
     const float alpha = grow ? ex2(m_run - m_new) : 1.f;
+    // A row that has seen nothing yet (SH: an empty interval) keeps m = -inf:
+    // its weights are ex2(-inf) = 0, not ex2(-inf + inf).
+    const float m_ref = SH && m_new == -INFINITY ? 0.f : m_new;
     float pr[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pr[e] = ex2(sc[e] - m_new);
+    for (int e = 0; e < 4; ++e) pr[e] = ex2(sc[e] - m_ref);
     l_run = l_run * alpha + ((pr[0] + pr[1]) + (pr[2] + pr[3]));
     m_run = m_new;
     if (__any_sync(kFull, grow)) {
@@ -734,8 +539,11 @@ __host__ __device__ inline int attn_smem(int group, int head_dim, int q_f32, int
     return kWarps * warp_smem(group, head_dim, q_f32, q8) + kWarps * stage_count(q8) * 8;
 }
 
-template <int D, bool Q8>
-__global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid_constant__ AttnParams p) {
+// SH: shaped calls (lt_kv_attend_shaped).  The tokens' descriptors then cover
+// the blocks of their intervals alone: pos is the last position attended,
+// skip the blocks before the first one; p.shapes holds the rest.
+template <int D, bool Q8, bool SH>
+__global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid_constant__ AttnParamsOf<SH> p) {
     constexpr int TILE = Q8 ? q8_tile_bytes(D) : 2 * kBlock * D * 2;
     constexpr int ROW = D * 2;
     constexpr int KS = D / 16;
@@ -799,6 +607,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
         r.ps = (long long)td.prefix * Hkv + (long long)gh * nb;
         r.kind = r.ps < t0 ? 1 : (r.ps + nb > t1 ? 2 : 0);
         r.last_block = r.b1 == nb ? td.last_block : -1;
+        if constexpr (SH) {
+            const ShapeDesc sd = p.shapes ? p.shapes[gi] : p.inl_shapes[gi];
+            r.lo = sd.lo;
+            r.qpos = sd.qpos;
+        }
         gt += len;
         gb += len;
         if (gb == nb) {
@@ -903,6 +716,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;
+    float slope = 0.f;  // SH: row g's distance slope, log2 units
     bool ok = true;
     int items_out = 0;   // (token, head) outputs this warp stored
     for (;;) {
@@ -991,11 +805,26 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
             }
             touched = true;
         }
+        TileShape sh;
+        if constexpr (SH) {
+            if (ct == 0) slope = p.shape.slopes && g < G ? __ldg(p.shape.slopes + dc.h * G + g) * kLog2e : 0.f;
+            const int j0 = (dc.skip + b) * kBlock;
+            sh = {p.shape, slope, dc.qpos - j0, dc.lo - j0};
+            if (!Q8 && sh.lo > 0) {
+                // Rows before the first attended one hold values of their
+                // own, possibly Inf or NaN: zero V as above.
+                const int n = min(sh.lo, kBlock), per_half = n * 8;
+                for (int e = lane; e < per_half * (D / 64); e += 32)
+                    reinterpret_cast<uint4*>(tile + kBlock * ROW + (e / per_half) * (kBlock * 128))[e % per_half] =
+                        make_uint4(0, 0, 0, 0);
+                touched = true;
+            }
+        }
         __syncwarp();
         if constexpr (Q8)
-            attend_tile_q8<D>(tile, valid, qa, o, m_run, l_run, p.scale_log2, lane);
+            attend_tile_q8<D, SH>(tile, valid, qa, o, m_run, l_run, p.scale_log2, lane, sh);
         else
-            attend_tile<D>(tile, valid, qa, o, m_run, l_run, p.scale_log2, lane);
+            attend_tile<D, SH>(tile, valid, qa, o, m_run, l_run, p.scale_log2, lane, sh);
         ++consumed;
         if (++cstage == S) {
             cstage = 0;
@@ -1023,8 +852,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
                         acc[nt][0] = o[nt][0] + o[nt][2];
                         acc[nt][1] = o[nt][1] + o[nt][3];
                     }
-                    if (dc.skip > 0) fold_prefix<D>(p, dc.tok, dc.h, g, t4, m_run, l, acc);
-                    store_out<D>(p, dc.tok, dc.h, g, t4, acc, 1.f / l);
+                    if (!SH && dc.skip > 0) fold_prefix<D>(p, dc.tok, dc.h, g, t4, m_run, l, acc);
+                    store_out<D>(p, dc.tok, dc.h, g, t4, acc, SH && l == 0.f ? 0.f : 1.f / l);
                 } else {
                     const size_t sl = (size_t)gw;  // partial slot of this warp (its first piece)
 #pragma unroll
@@ -1126,7 +955,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
         }
         merge_slots<D>(grouped ? p.part2_o : p.part_o, grouped ? p.part2_ml : p.part_ml, G, g, t4, gw + 1, w_last,
                        stride, M, L, acc);
-        if (dc.skip > 0) fold_prefix<D>(p, dc.tok, dc.h, g, t4, M, L, acc);
+        if (!SH && dc.skip > 0) fold_prefix<D>(p, dc.tok, dc.h, g, t4, M, L, acc);
         store_out<D>(p, dc.tok, dc.h, g, t4, acc, 1.f / L);
     }
     peer_done(p, lane, items_out + 1);
@@ -1771,27 +1600,27 @@ int sm_count(int dev) {
     return sms[dev];
 }
 
-template <int D, bool Q8>
+template <int D, bool Q8, bool SH>
 cudaError_t ensure_attr(int dev) {
     // opt-in shared memory is a per-device attribute; size it for the largest
     // layout (f32 q, group 8)
     static bool set[64] = {};
     if (set[dev]) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<D, Q8, SH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                attn_smem(kMaxGroup, D, 1, Q8));
     if (e == cudaSuccess) set[dev] = true;
     return e;
 }
 
-template <int D, bool Q8>
+template <int D, bool Q8, bool SH>
 int warps_for(int dev, int group, int q_f32) {
     // resident CTAs per SM for this layout, cached per (device, group, dtype)
     static int cache[64][kMaxGroup + 1][2] = {};
     int& c = cache[dev][group][q_f32 ? 1 : 0];
     if (c == 0) {
-        if (ensure_attr<D, Q8>(dev) != cudaSuccess) return 0;
+        if (ensure_attr<D, Q8, SH>(dev) != cudaSuccess) return 0;
         int per_sm = 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<D, Q8>, kWarps * 32,
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<D, Q8, SH>, kWarps * 32,
                                                           attn_smem(group, D, q_f32, Q8)) != cudaSuccess)
             return 0;
         c = (per_sm < 1 ? 1 : per_sm) * sm_count(dev) * kWarps;
@@ -1799,19 +1628,19 @@ int warps_for(int dev, int group, int q_f32) {
     return c;
 }
 
-template <int D, bool Q8>
-cudaError_t launch_attend_d(const AttnParams& p, cudaStream_t s) {
+template <int D, bool Q8, bool SH>
+cudaError_t launch_attend_d(const AttnParamsOf<SH>& p, cudaStream_t s) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if ((e = ensure_attr<D, Q8>(dev)) != cudaSuccess) return e;
+    if ((e = ensure_attr<D, Q8, SH>(dev)) != cudaSuccess) return e;
     // Cooperative: merging warps wait for other CTAs' flags, so the whole
     // grid (sized to the resident capacity) must be co-resident.
     const dim3 grid((p.n_warps + kWarps - 1) / kWarps), block(kWarps * 32);
     if (p.pre_splits == 0) {
-        void* args[] = {const_cast<AttnParams*>(&p)};
-        return cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(&paged_attn_kernel<D, Q8>), grid, block,
+        void* args[] = {const_cast<AttnParamsOf<SH>*>(&p)};
+        return cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(&paged_attn_kernel<D, Q8, SH>), grid, block,
                                            args, attn_smem(p.group, D, p.q_f32, Q8), s);
     }
     // After a prefix pass: a programmatic dependent of it, so its first CTAs
@@ -1834,29 +1663,49 @@ cudaError_t launch_attend_d(const AttnParams& p, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_attn_kernel<D, Q8>, p);
+    return cudaLaunchKernelEx(&cfg, paged_attn_kernel<D, Q8, SH>, p);
 }
 
 }  // namespace
 
-int attend_warps(int device, int group, int head_dim, int q_f32, int q8) {
+int attend_warps(int device, int group, int head_dim, int q_f32, int fmt, bool shaped) {
     if (device < 0 || device >= 64 || group < 1 || group > kMaxGroup) return 0;
     int prev = -1;
     cudaGetDevice(&prev);
     if (prev != device) cudaSetDevice(device);
     int w;
-    if (q8)
-        w = head_dim == 64 ? warps_for<64, true>(device, group, q_f32) : warps_for<128, true>(device, group, q_f32);
+    if (fmt == LT_KV_Q4_0)
+        w = attend_q4_warps(device, group, head_dim, q_f32, shaped);
+    else if (shaped && fmt == LT_KV_Q8_0)
+        w = head_dim == 64 ? warps_for<64, true, true>(device, group, q_f32)
+                           : warps_for<128, true, true>(device, group, q_f32);
+    else if (shaped)
+        w = head_dim == 64 ? warps_for<64, false, true>(device, group, q_f32)
+                           : warps_for<128, false, true>(device, group, q_f32);
+    else if (fmt == LT_KV_Q8_0)
+        w = head_dim == 64 ? warps_for<64, true, false>(device, group, q_f32)
+                           : warps_for<128, true, false>(device, group, q_f32);
     else
-        w = head_dim == 64 ? warps_for<64, false>(device, group, q_f32) : warps_for<128, false>(device, group, q_f32);
+        w = head_dim == 64 ? warps_for<64, false, false>(device, group, q_f32)
+                           : warps_for<128, false, false>(device, group, q_f32);
     if (prev != device && prev >= 0) cudaSetDevice(prev);
     return w;
 }
 
 cudaError_t launch_attend(const AttnParams& p, int head_dim, cudaStream_t s) {
     if (p.n_warps == 0) return cudaSuccess;
-    if (p.q8) return head_dim == 64 ? launch_attend_d<64, true>(p, s) : launch_attend_d<128, true>(p, s);
-    return head_dim == 64 ? launch_attend_d<64, false>(p, s) : launch_attend_d<128, false>(p, s);
+    if (p.fmt == LT_KV_Q4_0) return launch_attend_q4(p, head_dim, s);
+    if (p.fmt == LT_KV_Q8_0)
+        return head_dim == 64 ? launch_attend_d<64, true, false>(p, s) : launch_attend_d<128, true, false>(p, s);
+    return head_dim == 64 ? launch_attend_d<64, false, false>(p, s) : launch_attend_d<128, false, false>(p, s);
+}
+
+cudaError_t launch_attend_shaped(const AttnShapedParams& p, int head_dim, cudaStream_t s) {
+    if (p.n_warps == 0) return cudaSuccess;
+    if (p.fmt == LT_KV_Q4_0) return launch_attend_q4_shaped(p, head_dim, s);
+    if (p.fmt == LT_KV_Q8_0)
+        return head_dim == 64 ? launch_attend_d<64, true, true>(p, s) : launch_attend_d<128, true, true>(p, s);
+    return head_dim == 64 ? launch_attend_d<64, false, true>(p, s) : launch_attend_d<128, false, true>(p, s);
 }
 
 int attend_launches(const AttnParams& p) { return p.n_warps == 0 ? 0 : 1; }
@@ -1896,8 +1745,11 @@ cudaError_t launch_gather_permute(const void* gathered, void* out, int nranks, u
 }
 
 cudaError_t launch_write(uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, const void* k,
-                         const void* v, int in_f32, int q8, cudaStream_t s) {
+                         const void* v, int in_f32, int fmt, cudaStream_t s) {
     if (n == 0) return cudaSuccess;
+    if (fmt == LT_KV_Q4_0)
+        return launch_write_q4(reinterpret_cast<uint8_t*>(pool_layer), cells, n, n_kv_heads, head_dim, k, v, in_f32, s);
+    const bool q8 = fmt == LT_KV_Q8_0;
     const int threads = n * n_kv_heads * 2 * (head_dim / 8);
     const int blocks = (threads + 255) / 256;
     uint8_t* pool_bytes = reinterpret_cast<uint8_t*>(pool_layer);
@@ -1926,8 +1778,12 @@ cudaError_t launch_apply_plan(uint16_t* pool, size_t layer_stride_elems, size_t 
 }
 
 cudaError_t launch_rows(const uint16_t* pool_layer, const int32_t* table_row, int n, int n_kv_heads, int head_dim,
-                        uint16_t* k_out, uint16_t* v_out, int q8, int n_blocks, int32_t* err, cudaStream_t s) {
+                        uint16_t* k_out, uint16_t* v_out, int fmt, int n_blocks, int32_t* err, cudaStream_t s) {
     if (n == 0) return cudaSuccess;
+    if (fmt == LT_KV_Q4_0)
+        return launch_rows_q4(reinterpret_cast<const uint8_t*>(pool_layer), table_row, n, n_kv_heads, head_dim, k_out,
+                              v_out, n_blocks, err, s);
+    const bool q8 = fmt == LT_KV_Q8_0;
     const int threads = n * n_kv_heads * 2 * (head_dim / 8);
     const int blocks = (threads + 255) / 256;
     const uint8_t* pool_bytes = reinterpret_cast<const uint8_t*>(pool_layer);

@@ -95,7 +95,8 @@ extern "C" lt_status lt_paged_attend_noalloc(const void* pool_layer, uint32_t kv
     // ---- every argument, before any device work ----
     if (!pool_layer || !tables || !q || !out || (n && (!seq || !pos))) return LT_E_ARG;
     if (!ltkv::dtype_valid(q_dtype) || !ltkv::dtype_valid(out_dtype)) return LT_E_ARG;
-    if (kv_format == LT_KV_Q8_0) return LT_E_UNSUPPORTED;  // the kernel below reads f16 tiles only
+    if (kv_format == LT_KV_Q8_0 || kv_format == LT_KV_Q4_0)
+        return LT_E_UNSUPPORTED;  // the kernel below reads f16 tiles only
     if (kv_format != LT_KV_F16) return LT_E_ARG;
     if (n_blocks == 0 || n_blocks > 0x7FFFFFFFu) return LT_E_ARG;
     if (n_table_rows == 0 || max_blocks_per_seq == 0 || max_blocks_per_seq > 0x7FFFFFFFu) return LT_E_ARG;
@@ -196,7 +197,7 @@ extern "C" lt_status lt_paged_attend_noalloc(const void* pool_layer, uint32_t kv
         p.pre_ml = nullptr;
         p.pre_splits = 0;
         p.pre_split_rows = 0;
-        p.q8 = 0;
+        p.fmt = LT_KV_F16;
         p.n_peers = 0;
         if (ltkv::launch_attend(p, (int)head_dim, st) != cudaSuccess) return LT_E_CUDA;
     }

@@ -83,7 +83,7 @@ def _i32(a) -> np.ndarray:
     return np.ascontiguousarray(np.asarray(a, dtype=np.int32))
 
 
-KV_FORMATS = {"f16": N.LT_KV_F16, "q8_0": N.LT_KV_Q8_0}
+KV_FORMATS = {"f16": N.LT_KV_F16, "q8_0": N.LT_KV_Q8_0, "q4_0": N.LT_KV_Q4_0}
 
 
 class KvCache:
@@ -92,8 +92,8 @@ class KvCache:
     ``KvCache(n_layers, n_kv_heads, head_dim, n_tokens)`` is the reference's
     ``KvCache::new(n_layers, n_kv_heads * head_dim, n_tokens)``.  ``device=-1``
     builds a bookkeeping-only handle (no GPU), for host-side tests.
-    ``kv_format="q8_0"`` stores rows as Q8_0 groups (include/lt_kv.h,
-    LT_KV_Q8_0) instead of f16.
+    ``kv_format="q8_0"`` / ``"q4_0"`` stores rows as 8-bit / 4-bit groups
+    (include/lt_kv.h, LT_KV_Q8_0, LT_KV_Q4_0) instead of f16.
     """
 
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, n_tokens: int, *, n_heads: int | None = None,
@@ -203,6 +203,55 @@ class KvCache:
                                            _dptr(out), _dtype_code(out), scale, _stream(stream)))
         return out
 
+    def attend_shaped(self, layer: int, q, seqs, positions, *, softcap: float = 0.0, window: int = 0, slopes=None,
+                      first=None, end=None, out=None, out_dtype=None, scale: float | None = None, stream=None):
+        """attend() with shaped scores (include/lt_kv.h, lt_kv_score): a tanh
+        cap, a sliding window, a distance bias (``slopes`` CUDA f32
+        [n_heads]) and per-token intervals [first, end) (host arrays [n])."""
+        import torch
+
+        seqs, positions = _u32(seqs), _u32(positions)
+        n = seqs.size
+        self._on_device("q", q, n * self.n_heads * self.head_dim)
+        if positions.size != n:
+            raise ValueError(f"{positions.size} positions for {n} tokens")
+        if window < 0 or window > 0xFFFFFFFF:
+            raise ValueError(f"window {window} is out of range")
+        score = N.lt_kv_score(softcap=softcap, window=window)
+        if slopes is not None:
+            self._on_device("slopes", slopes, self.n_heads)
+            if slopes.dtype != torch.float32:
+                raise TypeError(f"slopes must be float32, not {slopes.dtype}")
+            score.slopes = slopes.data_ptr()
+        for name, a in (("first", first), ("end", end)):
+            if a is None:
+                continue
+            a = np.asarray(a)
+            if a.size != n or (n and (a.min() < 0 or a.max() > 0xFFFFFFFF)):
+                raise ValueError(f"{name}: {n} positions expected, each in [0, 2**32)")
+            a = _u32(a.reshape(-1))
+            setattr(score, name + "_host", a.ctypes.data)
+            if name == "first":
+                first = a  # keeps the arrays alive for the call
+            else:
+                end = a
+        if out is None:
+            out = torch.empty((n, self.n_heads * self.head_dim), dtype=out_dtype or torch.float32, device=q.device)
+        self._on_device("out", out, n * self.n_heads * self.head_dim)
+        if scale is None:
+            scale = self.default_scale
+        self._check(self._lib.lt_kv_attend_shaped(self._h, layer, _dptr(q), _dtype_code(q), _ptr(seqs),
+                                                  _ptr(positions), n, C.byref(score), _dptr(out), _dtype_code(out),
+                                                  scale, _stream(stream)))
+        return out
+
+    def _on_device(self, name: str, t, numel: int):
+        """Refuse a tensor that is not a contiguous array of `numel` values on the cache's device."""
+        if not t.is_cuda or t.device.index != self.device:
+            raise ValueError(f"{name} is on {t.device}, the cache on cuda:{self.device}")
+        if not t.is_contiguous() or t.numel() != numel:
+            raise ValueError(f"{name}: a contiguous array of {numel} values expected, not {tuple(t.shape)}")
+
     def write_attend(self, layer: int, blocks, slots, k, v, q, seqs, positions, out=None, out_dtype=None,
                      scale: float | None = None, stream=None):
         """write() then attend() for the same tokens, in one kernel when legal."""
@@ -310,6 +359,27 @@ class KvCache:
         self._check(self._lib.lt_kv_rows(self._h, layer, seq, n, _dptr(k), _dptr(v), _stream(stream)))
         return k, v
 
+    def read(self, layer: int, blocks, slots, dtype=None, k=None, v=None, stream=None):
+        """Values of cells (the inverse of write): (k, v) CUDA [n, kv_dim] of
+        `dtype` (float16 by default; float32 holds every format exactly)."""
+        import torch
+
+        blocks, slots = _i32(blocks), _i32(slots)
+        n = blocks.size
+        if slots.size != n:
+            raise ValueError(f"{slots.size} slots for {n} blocks")
+        if k is None:
+            k = torch.empty((n, self.kv_dim), dtype=dtype or torch.float16, device=f"cuda:{self.device}")
+        if v is None:
+            v = torch.empty_like(k)
+        if k.dtype != v.dtype:
+            raise TypeError(f"k is {k.dtype}, v {v.dtype}")
+        self._on_device("k", k, n * self.kv_dim)
+        self._on_device("v", v, n * self.kv_dim)
+        self._check(self._lib.lt_kv_read(self._h, layer, _ptr(blocks), _ptr(slots), n, _dptr(k), _dptr(v),
+                                         _dtype_code(k), _stream(stream)))
+        return k, v
+
     # --------------------------------------------------------- introspection
     def seq_blocks(self, seq: int) -> np.ndarray:
         n = self._lib.lt_kv_seq_blocks(self._h, seq, None, 0)
@@ -372,11 +442,12 @@ class KvCache:
         """Raw device pool of blocks [block0, block0 + count) of one layer
         (default: all): f16 caches give uint16 [block][kv_head][2][16][head_dim]
         with the chunk swizzle of include/lt_kv.h still applied; Q8_0 caches
-        give the uint8 tiles [block][kv_head][34 * head_dim]."""
+        give the uint8 tiles [block][kv_head][34 * head_dim] (Q4_0: 18 * head_dim)."""
         if count is None:
             count = self.n_blocks - block0
-        if self.kv_format == "q8_0":
-            out = np.zeros((count, self.n_kv_heads, 34 * self.head_dim), np.uint8)
+        tile = {"q8_0": 34, "q4_0": 18}.get(self.kv_format)
+        if tile:
+            out = np.zeros((count, self.n_kv_heads, tile * self.head_dim), np.uint8)
         else:
             out = np.zeros((count, self.n_kv_heads, 2, BLOCK, self.head_dim), np.uint16)
         self._check(self._lib.lt_kv_read_pool(self._h, layer, block0, count, _ptr(out)))
@@ -386,9 +457,11 @@ class KvCache:
         """Blocks [block0, block0 + count) of this layer's pool as the
         reference lays it out (kv.rs:20): (K, V) uint16 [block][slot][kv_dim];
         for Q8_0 (Kq, Vq) int8 [block][slot][kv_dim] and (Kd, Vd) f16 bits
-        [block][slot][kv_dim/32]."""
+        [block][slot][kv_dim/32]; for Q4_0 the same with codes 0..15 in uint8."""
         if self.kv_format == "q8_0":
             return unswizzle_pool_q8(self.read_pool(layer, block0, count), self.head_dim)
+        if self.kv_format == "q4_0":
+            return unswizzle_pool_q4(self.read_pool(layer, block0, count), self.head_dim)
         return unswizzle_pool(self.read_pool(layer, block0, count))
 
 
@@ -492,3 +565,28 @@ def unswizzle_pool_q8(raw: np.ndarray, head_dim: int):
         return np.ascontiguousarray(a.transpose(0, 2, 1, 3).reshape(nb, BLOCK, -1))
     return rows(kq), rows(vq), rows(kd), rows(vd)
 
+
+
+def unswizzle_pool_q4(raw: np.ndarray, head_dim: int):
+    """Invert the Q4_0 tile layout of include/lt_kv.h -> codes (Kc, Vc) uint8
+    [block][16][kv_heads*D] and (Kd, Vd) f16 bits [block][16][kv_heads*D/32]."""
+    nb, hkv, tb = raw.shape
+    d = head_dim
+    assert tb == 18 * d
+    s, e, c = np.arange(BLOCK)[:, None], np.arange(d)[None, :], np.arange(d // 32)[None, :]
+
+    def word(i, g, t):
+        return 512 * (i // 4) + 16 * (4 * g + t) + 4 * (i % 4)
+
+    koff = word(e // 16, s % 8, (e % 8) // 2) + 2 * (e % 2) + s // 8  # [16, D]
+    voff = 8 * d + word(e // 16, e % 8, (s % 8) // 2) + 2 * (s % 2) + s // 8
+    shift = 4 * (e % 16 // 8)
+    kc, vc = ((raw[:, :, off] >> shift) & 15 for off in (koff, voff))
+    half = raw[:, :, 16 * d:].copy().view(np.uint16)  # K scales, then V scales
+    kd = half[:, :, ((s % 8) * 2 + s // 8) * (d // 32) + c]
+    vd = half[:, :, d // 2 + ((s % 8) // 2 * (d // 32) + c) * 4 + 2 * (s // 8) + s % 2]
+
+    def rows(a):
+        return np.ascontiguousarray(a.transpose(0, 2, 1, 3).reshape(nb, BLOCK, -1))
+
+    return rows(kc), rows(vc), rows(kd), rows(vd)

@@ -1,0 +1,367 @@
+"""GPU tests of the 4-bit cache (include/lt_kv.h, LT_KV_Q4_0) through the C ABI.
+
+Codes and scales are bit-exact against a 64-bit restatement of the format on
+every write path (f32, f16, fused append, copy-on-write, compaction); values
+read back exactly.  Attention is compared with softmax attention in 64 bits
+over the cached values.
+
+Tolerances.  Cached values are f16s exactly and q and the weights are carried
+as f16 value + residual (relative error 2^-22 each); 2^x on the SFU is within
+2^-22; scores and sums are f32.  A score of magnitude up to 16 with 128 f32
+additions moves by at most ~128 * 2^-24 * 16 * log2(e) / sqrt(128) (random
+signs) ~ 2e-5 in the exponent for single positions, which averages out over
+the sum; rtol 1e-4 and atol 2e-5 (the other formats' bar) cover it.  f16
+outputs add half a step, 2^-11 relative."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import _attn64 as A  # noqa: E402
+
+from langtrain_studio_b200.kv import BLOCK, KvCache, KvError  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_cuda():
+    if not torch.cuda.is_available():
+        pytest.fail("CUDA device required for -m gpu tests")
+
+
+class Twin:
+    """A Q4_0 KvCache and the values it must hold, per sequence."""
+
+    def __init__(self, hkv, hd, tokens, hq=None, layers=1, max_seqs=8, **kw):
+        self.kv = KvCache(layers, hkv, hd, tokens, n_heads=hq or hkv, max_seqs=max_seqs, kv_format="q4_0", **kw)
+        self.hkv, self.hd, self.hq, self.layers = hkv, hd, hq or hkv, layers
+        self.rows = {}  # (layer, seq) -> list of (kc, kd, vc, vd) rows
+
+    def add(self, layer, seq, k, v):
+        rows = self.rows.setdefault((layer, seq), [])
+        for a, b in zip(k.reshape(-1, self.hkv, self.hd), v.reshape(-1, self.hkv, self.hd)):
+            rows.append((*A.quant4(a), *A.quant4(b)))
+
+    def draw(self, n, rng, dtype=np.float32):
+        return tuple((rng.standard_normal((n, self.hkv * self.hd)) * g).astype(dtype) for g in (1.5, 1.0))
+
+    def fill(self, seq, upto, rng, dtype=np.float32):
+        n0 = self.kv.len(seq)
+        if upto <= n0:
+            return
+        pos = np.arange(n0, upto)
+        cells = self.kv.append_batch(np.full(pos.size, seq), pos)
+        for layer in range(self.layers):
+            k, v = self.draw(pos.size, rng, dtype)
+            self.kv.write(layer, *cells, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+            self.add(layer, seq, k, v)
+
+    def values(self, layer, seq):
+        """(K, V) [len, hkv, hd] f64."""
+        rows = self.rows[(layer, seq)][: self.kv.len(seq)]
+        return (np.stack([A.value4(r[0], r[1]) for r in rows]), np.stack([A.value4(r[2], r[3]) for r in rows]))
+
+    def check(self, layer, seq):
+        """Codes and scales in the pool, through the table, bit for bit."""
+        n = self.kv.len(seq)
+        kc, vc, kd, vd = self.kv.pool_reference_layout(layer)
+        blocks = self.kv.seq_blocks(seq)
+        for i, (rk, dk, rv, dv) in enumerate(self.rows[(layer, seq)][:n]):
+            b, s = blocks[i // BLOCK], i % BLOCK
+            assert np.array_equal(kc[b, s], rk.reshape(-1)), (seq, i)
+            assert np.array_equal(vc[b, s], rv.reshape(-1)), (seq, i)
+            assert np.array_equal(kd[b, s].view(np.float16).astype(np.float64), dk.reshape(-1)), (seq, i)
+            assert np.array_equal(vd[b, s].view(np.float16).astype(np.float64), dv.reshape(-1)), (seq, i)
+        kr, vr = self.kv.rows(layer, seq, n)
+        K, V = self.values(layer, seq)
+        assert np.array_equal(kr.cpu().numpy().astype(np.float64).reshape(K.shape), K)
+        assert np.array_equal(vr.cpu().numpy().astype(np.float64).reshape(V.shape), V)
+
+    def attend_ref(self, layer, seqs, pos, q):
+        out = np.zeros((len(seqs), self.hq * self.hd))
+        cache = {}
+        for i, (s, p) in enumerate(zip(seqs, pos)):
+            if s not in cache:
+                cache[s] = self.values(layer, s)
+            K, V = cache[s]
+            out[i] = A.attend(q[i].reshape(self.hq, self.hd), K, V, int(p), self.hq // self.hkv,
+                              self.kv.default_scale).reshape(-1)
+        return out
+
+
+def close(out, ref, out_dtype=torch.float32):
+    half = out_dtype == torch.float16
+    np.testing.assert_allclose(out.float().cpu().numpy(), ref, rtol=1e-4 + (2 ** -11 if half else 0),
+                               atol=2e-5 + (2 ** -24 if half else 0))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_write_is_bit_exact(hd, dtype):
+    rng = np.random.default_rng(hd)
+    t = Twin(4, hd, 16 * 20, layers=2, max_seqs=4)
+    for s, n in enumerate([1, 17, 40, 100]):
+        t.fill(s, n, rng, dtype)
+    for s in range(4):
+        for layer in range(2):
+            t.check(layer, s)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_write_borders_and_odd_values(dtype):
+    """Values on and next to the code borders, ties of the two extremes, zeros,
+    subnormals, saturation, Inf and NaN."""
+    rng = np.random.default_rng(1)
+    t = Twin(2, 64, 16 * 4, max_seqs=1)
+    rows = []
+    for sign in (1.0, -1.0):
+        for d in (0.375, 1.0, 0.0078125, 2.0 ** -24, 3 * 2.0 ** -20, 300.0):
+            steps = (np.arange(32) % 17 - 8.5)  # k + 1/2: exactly between two codes
+            x = steps * d
+            x[0] = -8 * d
+            with np.errstate(over="ignore"):
+                near = np.nextafter(x.astype(dtype), np.array(np.inf if sign > 0 else -np.inf, dtype))
+            rows.append(np.concatenate([sign * x, sign * near.astype(np.float64), sign * 0.99 * x, rng.standard_normal(32)]))
+    both = np.zeros(128)
+    both[[3, 40, 70, 100]], both[[9, 35, 90, 110]] = 5.0, -5.0  # both signs reach the largest magnitude
+    rows += [both, np.zeros(128), np.full(128, 1e-7), np.full(128, 30000.0), -np.linspace(1, 65000, 128)]
+    odd = rng.standard_normal(128)
+    odd[5], odd[37], odd[70], odd[71] = np.nan, np.inf, -np.inf, np.nan
+    rows += [odd, np.full(128, np.nan), np.full(128, np.inf)]
+    with np.errstate(over="ignore"):
+        k = np.stack(rows).astype(dtype)
+    v = k[::-1].copy()
+    cells = t.kv.append_batch(np.zeros(len(k)), np.arange(len(k)))
+    t.kv.write(0, *cells, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+    t.add(0, 0, k, v)
+    t.check(0, 0)
+    # values read back and written again keep their codes
+    kr, vr = t.kv.read(0, *cells)
+    t.kv.write(0, *cells, kr, vr)
+    K, V = t.values(0, 0)
+    k2, v2 = t.kv.read(0, *cells, dtype=torch.float32)
+    assert np.array_equal(k2.cpu().numpy().reshape(K.shape), K) and np.array_equal(v2.cpu().numpy().reshape(V.shape), V)
+
+
+def test_writes_of_one_block_keep_their_neighbours():
+    """Single rows in any slot order: each write changes its own slot alone."""
+    rng = np.random.default_rng(2)
+    t = Twin(3, 128, 64, max_seqs=1)
+    t.fill(0, 40, rng)
+    blocks = t.kv.seq_blocks(0)
+    for p in [39, 0, 8, 7, 15, 16, 24, 31, 3, 11]:
+        k, v = t.draw(1, rng)
+        t.kv.write(0, [blocks[p // 16]], [p % 16], torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+        new = (A.quant4(k.reshape(3, 128)), A.quant4(v.reshape(3, 128)))
+        t.rows[(0, 0)][p] = (*new[0], *new[1])
+    t.check(0, 0)
+
+
+ATT_CASES = [
+    # (head_dim, n_heads, n_kv_heads, lens)
+    (128, 32, 8, [1, 15, 16, 17, 200]),
+    (128, 64, 8, [513, 1100]),
+    (64, 32, 4, [31, 192, 64]),
+    (128, 8, 8, [2049, 3]),      # group 1
+    (64, 12, 4, [77, 300]),      # group 3
+    (128, 10, 2, [65, 700]),     # group 5
+    (64, 14, 2, [48, 333]),      # group 7
+]
+
+
+@pytest.mark.parametrize("hd,hq,hkv,lens", ATT_CASES)
+@pytest.mark.parametrize("q_dtype,out_dtype,min_tiles", [(torch.float32, torch.float32, 8),
+                                                         (torch.float16, torch.float16, 8),
+                                                         (torch.float16, torch.float32, 2),
+                                                         (torch.float32, torch.float32, 1)])
+def test_attention(hd, hq, hkv, lens, q_dtype, out_dtype, min_tiles):
+    rng = np.random.default_rng(hd + hq + len(lens))
+    t = Twin(hkv, hd, 16 * (sum((n + 15) // 16 for n in lens)), hq, max_seqs=len(lens), max_batch=2100)
+    t.kv.set_min_tiles_per_warp(min_tiles)
+    for s, n in enumerate(lens):
+        t.fill(s, n, rng)
+    seqs, pos = np.arange(len(lens)), np.array(lens) - 1
+    q = torch.from_numpy(rng.standard_normal((len(lens), hq * hd)).astype(np.float32)).cuda().to(q_dtype)
+    out = t.kv.attend(0, q, seqs, pos, out_dtype=out_dtype)
+    t.kv.check()
+    close(out, t.attend_ref(0, seqs, pos, q.float().cpu().numpy()), out_dtype)
+
+
+@pytest.mark.parametrize("gain", [1e-6, 30.0, 3e4])
+def test_attention_of_small_and_large_q(gain):
+    """q far below and above 1 keeps its 22 bits (rows are scaled by a power of
+    two); the scale argument brings the scores back to ordinary ones."""
+    rng = np.random.default_rng(5)
+    t = Twin(2, 128, 16 * 20, 8, max_seqs=1)
+    t.fill(0, 300, rng)
+    q = (rng.standard_normal((1, 8 * 128)) * gain).astype(np.float32)
+    out = t.kv.attend(0, torch.from_numpy(q).cuda(), [0], [299], scale=t.kv.default_scale / gain)
+    K, V = t.values(0, 0)
+    scale = float(np.float32(t.kv.default_scale / gain))
+    ref = A.attend(q.reshape(8, 128), K, V, 299, 4, scale).reshape(1, -1)
+    close(out, ref)
+
+
+def test_prefill_chunk_and_repeated_tokens():
+    """Several tokens of one sequence, the same token twice, lengths that end
+    inside a block, and more than 512 tokens in a call."""
+    rng = np.random.default_rng(8)
+    t = Twin(2, 64, 16 * 64, 8, max_seqs=3, max_batch=1024)
+    for s, n in enumerate([333, 40, 1]):
+        t.fill(s, n, rng)
+    seqs = np.concatenate([np.zeros(100), np.ones(40), [2, 2, 0, 0]]).astype(np.int64)
+    pos = np.concatenate([np.arange(233, 333), np.arange(40), [0, 0, 5, 5]]).astype(np.int64)
+    seqs, pos = np.concatenate([seqs, np.zeros(460, np.int64)]), np.concatenate([pos, rng.integers(0, 333, 460)])
+    q = rng.standard_normal((seqs.size, 8 * 64)).astype(np.float32)
+    out = t.kv.attend(0, torch.from_numpy(q).cuda(), seqs, pos)
+    t.kv.check()
+    close(out, t.attend_ref(0, seqs, pos, q))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kv_dtype", [np.float32, np.float16])
+def test_fused_append(hd, kv_dtype):
+    """Decode steps through write_attend keep the pool bit-exact, and equal
+    write followed by attend."""
+    rng = np.random.default_rng(hd)
+    hkv, hq = 4, 16
+    t = Twin(hkv, hd, 16 * 40, hq, max_seqs=4)
+    for s, n in enumerate([3, 30, 64, 100]):
+        t.fill(s, n, rng)
+    for _ in range(20):
+        seqs = np.arange(4)
+        pos = np.array([t.kv.len(s) for s in seqs])
+        b, sl = t.kv.append_batch(seqs, pos)
+        k, v = t.draw(4, rng, kv_dtype)
+        for s in seqs:
+            t.add(0, int(s), k[s], v[s])
+        q = rng.standard_normal((4, hq * hd)).astype(np.float32)
+        kd, vd, qd = (torch.from_numpy(x).cuda() for x in (k, v, q))
+        out = t.kv.write_attend(0, b, sl, kd, vd, qd, seqs, pos)
+        close(out, t.attend_ref(0, seqs, pos, q))
+    assert torch.equal(out, t.kv.attend(0, qd, seqs, pos))
+    for s in range(4):
+        t.check(0, s)
+    t.kv.check()
+
+
+def test_copy_on_write_compaction_and_stale_blocks():
+    rng = np.random.default_rng(7)
+    t = Twin(2, 64, 16 * 90, 8, layers=2, max_seqs=12)
+    t.fill(0, 200, rng)
+    for s in range(1, 10):
+        t.kv.share(0, s, 150 + s)
+        for layer in range(2):
+            t.rows[(layer, s)] = list(t.rows[(layer, 0)][: 150 + s])
+        t.fill(s, 170 + 3 * s, rng)
+    c0 = t.kv.cascade_launches()
+    t.kv.truncate(0, 0)
+    t.kv.truncate(4, 0)
+    assert t.kv.compact() > 0
+    t.fill(11, 21, rng)  # reuses freed blocks: stale codes past slot 5 of its last one
+    seqs = np.array([1, 2, 3, 5, 6, 7, 8, 9, 11])
+    pos = np.array([t.kv.len(int(s)) - 1 for s in seqs])
+    q = rng.standard_normal((9, 8 * 64)).astype(np.float32)
+    for layer in range(2):
+        for s in (1, 5, 9, 11):
+            t.check(layer, s)
+        close(t.kv.attend(layer, torch.from_numpy(q).cuda(), seqs, pos), t.attend_ref(layer, seqs, pos, q))
+    assert t.kv.cascade_launches() == c0
+    t.kv.check()
+
+
+def test_long_sequence_two_level_merge():
+    """One long sequence cut over many warps, each range a few tiles."""
+    rng = np.random.default_rng(11)
+    n = 16 * 700 + 5
+    t = Twin(1, 128, n + 16, 8, max_seqs=1, max_batch=n)
+    k, v = t.draw(n, rng)
+    cells = t.kv.append_batch(np.zeros(n), np.arange(n))
+    t.kv.write(0, *cells, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+    K, V = (A.value4(*A.quant4(x.reshape(n, 1, 128))) for x in (k, v))
+    q = rng.standard_normal((1, 8 * 128)).astype(np.float32)
+    ref = A.attend(q.reshape(8, 128), K, V, n - 1, 8, t.kv.default_scale).reshape(1, -1)
+    for tiles in (1, 8, 40):
+        t.kv.set_min_tiles_per_warp(tiles)
+        close(t.kv.attend(0, torch.from_numpy(q).cuda(), [0], [n - 1]), ref)
+    t.kv.check()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8_0", "q4_0"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_read_cells(fmt, hd):
+    """Cells in any order, one of them twice, against rows()."""
+    rng = np.random.default_rng(3)
+    kv = KvCache(2, 3, hd, 16 * 8, max_seqs=2, kv_format=fmt)
+    n = 50
+    cells = kv.append_batch(np.repeat([0, 1], [n, n]), np.tile(np.arange(n), 2))
+    x = torch.from_numpy(rng.standard_normal((2, 2 * n, 3 * hd)).astype(np.float32)).cuda()
+    kv.write(1, *cells, x[0], x[1])
+    order = np.concatenate([rng.permutation(2 * n), [7, 7]])
+    k, v = kv.read(1, cells[0][order], cells[1][order])
+    for s in range(2):
+        kr, vr = kv.rows(1, s, n)
+        at = np.flatnonzero(order // n == s)
+        assert torch.equal(k[at], kr[order[at] % n]) and torch.equal(v[at], vr[order[at] % n])
+    k32, _ = kv.read(1, cells[0][order], cells[1][order], dtype=torch.float32)
+    assert torch.equal(k32.half(), k)
+    k0, v0 = kv.read(1, [], [])
+    assert k0.shape == (0, 3 * hd)
+
+
+def test_other_stream_and_two_caches():
+    """Two caches on two streams at once, each with its own workspace."""
+    rng = np.random.default_rng(13)
+    ts, qs, outs = [], [], []
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(2):
+        t = Twin(2, 128, 16 * 140, 8, max_seqs=2, max_batch=2048)
+        with torch.cuda.stream(streams[i]):
+            t.fill(0, 2000, rng)
+            t.fill(1, 77 + i, rng)
+        ts.append(t)
+        qs.append(torch.from_numpy(rng.standard_normal((2, 8 * 128)).astype(np.float32)).cuda())
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for t, q, st in zip(ts, qs, streams):
+            outs.append(t.kv.attend(0, q, [0, 1], [1999, t.kv.len(1) - 1], stream=st))
+    torch.cuda.synchronize()
+    for i, (t, q) in enumerate(zip(ts, qs)):
+        ref = t.attend_ref(0, [0, 1], [1999, t.kv.len(1) - 1], q.cpu().numpy())
+        for o in outs[i::2]:
+            close(o, ref)
+
+
+def test_refused_on_the_device():
+    t = Twin(1, 64, 64, 4, max_seqs=2)
+    rng = np.random.default_rng(0)
+    t.fill(0, 20, rng)
+    b = t.kv.seq_blocks(0)
+    k, v = (torch.zeros((2, 64), device="cuda") for _ in range(2))
+    with pytest.raises(KvError, match="named twice"):
+        t.kv.write(0, [b[0], b[0]], [3, 3], k, v)
+    with pytest.raises(KvError, match="out of range"):
+        t.kv.read(0, [b[0], 99], [0, 0])
+    with pytest.raises(KvError, match="out of range"):
+        t.kv.read(3, [b[0]], [0])
+    with pytest.raises(ValueError):
+        t.kv.read(0, [b[0]], [0], k=torch.zeros((1, 64)), v=torch.zeros((1, 64)))
+    big = torch.zeros(130, device="cuda")
+    with pytest.raises(KvError, match="aligned"):
+        t.kv.write(0, [b[0], b[1]], [0, 0], big[1:129].view(2, 64), v)
+    t.check(0, 0)
+    # a captured call would replay the staging and flags of the first one
+    q = torch.zeros((1, 256), device="cuda")
+    st = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    out = torch.empty((1, 256), device="cuda")
+    with torch.cuda.graph(graph, stream=st):
+        for call in (lambda: t.kv.attend(0, q, [0], [19], out=out, stream=st),
+                     lambda: t.kv.write(0, b[:2], [0, 0], k, v, stream=st),
+                     lambda: t.kv.read(0, b[:1], [0], k=k[:1], v=v[:1], stream=st),
+                     lambda: t.kv.attend_shaped(0, q, [0], [19], window=4, out=out, stream=st)):
+            with pytest.raises(KvError, match="captured"):
+                call()
+    t.kv.attend(0, q, [0], [19], out=out)
+    t.kv.check()
