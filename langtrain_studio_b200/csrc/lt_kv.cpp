@@ -30,6 +30,7 @@ namespace {
 constexpr int kSlots = 8;  // staging ring depth (pinned host + device pairs)
 constexpr uint32_t kCascadeMaxTokens = 1024;  // tokens of one call the prefix pass serves
 constexpr int kCascadeMinBlocks = 4;          // shortest shared prefix worth a pass (64 positions)
+constexpr size_t kExpandBytes = 128u << 20;   // f16 workspace of a 4-bit cache's prefix pass
 constexpr uint32_t kClean = 0xFFFFFFFFu;
 
 struct Slot {
@@ -113,6 +114,12 @@ struct lt_kv {
     uint64_t cascade_launches = 0;
     int casc_splits = 1;
     size_t casc_ntok = 0;  // tokens in the upload image's token list
+    // LT_KV_Q4_0: the prefix pass reads f16 tiles, so its blocks are expanded
+    // into this workspace first (exp_cap blocks of one layer, all heads)
+    uint16_t* d_exp = nullptr;
+    int32_t* d_iota = nullptr;  // 0, 1, ..., exp_cap - 1: the workspace's block table
+    size_t exp_cap = 0;
+    std::vector<ltkv::ExpandGroup> exp_groups;
     uint32_t n_blocks = 0, kv_dim = 0, group = 0, max_blocks = 0;
     int fmt = LT_KV_F16;      // lt_kv_format of the pool
     size_t block_elems = 0;   // 16-bit units of one block in one layer (all heads, K and V)
@@ -220,6 +227,10 @@ void free_device(lt_kv* kv) {
     cudaFree(kv->d_pre_o);
     cudaFree(kv->d_pre_ml);
     kv->d_pre_o = kv->d_pre_ml = nullptr;
+    cudaFree(kv->d_exp);
+    cudaFree(kv->d_iota);
+    kv->d_exp = nullptr;
+    kv->d_iota = nullptr;
     cudaFree(kv->d_err);
     cudaFree(kv->d_flags);
     kv->d_flags = nullptr;
@@ -523,8 +534,13 @@ lt_status prof_begin(lt_kv* kv, ProfRing& r, cudaStream_t st, cudaEvent_t* end) 
 // stream-K launch only the token's own block.  The prefix pass items (KV
 // head x chunks of the group's tokens, each over [0, its tokens' largest
 // skip)), the token list and the tokens' skips go to casc_buf.  Returns the
-// number of items (0: no pass).
+// number of items (0: no pass).  LT_KV_Q4_0: only groups whose blocks fit the
+// workspace take part; exp_groups lists them, and an item's root is its
+// group's first workspace block.
 int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n) {
+    const bool expand = kv->fmt == LT_KV_Q4_0;
+    size_t exp_used = 0;
+    kv->exp_groups.clear();
     if (kv->cascade_min_tokens == 0 || n < kv->cascade_min_tokens || n > kv->pre_cap) return 0;
     auto& ord = kv->casc_order;
     ord.resize(n);
@@ -558,14 +574,18 @@ int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n
                     P = (size_t)(std::mismatch(rb.begin(), rb.begin() + lim, sb.begin()).first - rb.begin());
                 }
             }
-            if (P >= (size_t)kCascadeMinBlocks) {
-                bool one_seq = true;
-                for (uint32_t k = a; k < b && one_seq; ++k) one_seq = seq[ord[k]] == root;
-                groups.push_back({(int32_t)root, (int32_t)P, (int32_t)toks.size(), (int32_t)(b - a), one_seq});
+            bool one_seq = true;
+            for (uint32_t k = a; k < b && one_seq; ++k) one_seq = seq[ord[k]] == root;
+            size_t covered = P;  // blocks the group's tokens cover
+            for (uint32_t k = a; k < b && one_seq; ++k) covered = std::max<size_t>(covered, pos[ord[k]] / kBlock);
+            if (P >= (size_t)kCascadeMinBlocks && (!expand || exp_used + covered <= kv->exp_cap)) {
+                if (expand) kv->exp_groups.push_back({(int32_t)root, (int32_t)exp_used, (int32_t)covered});
+                groups.push_back({expand ? (int32_t)exp_used : (int32_t)root, (int32_t)P, (int32_t)toks.size(), (int32_t)(b - a), one_seq});
                 for (uint32_t k = a; k < b; ++k) {
                     toks.push_back((int32_t)ord[k]);
                     kv->toks_tmp[ord[k]].skip = one_seq ? (int32_t)(pos[ord[k]] / kBlock) : (int32_t)P;
                 }
+                exp_used += covered;
             }
         }
         a = b;
@@ -655,9 +675,9 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         t.last_block = kv->blocks[seq[i]][pos[i] / kBlock];
         t.skip = score && kv->shapes_tmp[i].lo <= t.pos ? kv->shapes_tmp[i].lo / kBlock : 0;
     }
-    // sets skip of the tokens it covers; the quantised tiles are not f16
-    // tensor-core operands, and the pass does not shape scores
-    const int n_items = kv->fmt != LT_KV_F16 || score ? 0 : plan_cascade(kv, seq, pos, n);
+    // sets skip of the tokens it covers; Q8_0 tiles are not f16 tensor-core
+    // operands (Q4_0 blocks are expanded for it), and the pass does not shape scores
+    const int n_items = kv->fmt == LT_KV_Q8_0 || score ? 0 : plan_cascade(kv, seq, pos, n);
     long long tiles = 0;
     for (uint32_t i = 0; i < n; ++i) {
         ltkv::TokenDesc& t = kv->toks_tmp[i];
@@ -829,6 +849,23 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         pp.pre_ml = kv->d_pre_ml;
         pp.split_rows = p.pre_split_rows;
         pp.err = kv->d_err;
+        if (kv->fmt == LT_KV_Q4_0) {
+            // One launch for all groups' blocks; the pass then reads the
+            // workspace through its identity table.
+            const cudaError_t xe =
+                ltkv::launch_expand_q4(reinterpret_cast<const uint8_t*>(p.pool_layer), kv->d_tables, (int)kv->max_blocks,
+                                       kv->exp_groups.data(), (int)kv->exp_groups.size(), (int)kv->cfg.n_kv_heads,
+                                       (int)kv->cfg.head_dim, kv->d_exp, (int)kv->n_blocks, kv->d_err, st);
+            if (xe != cudaSuccess) {
+                rollback();
+                return fail(kv, LT_E_CUDA, "expand launch: %s", cudaGetErrorString(xe));
+            }
+            kv->launches++;
+            pp.pool_layer = kv->d_exp;
+            pp.tables = kv->d_iota;
+            pp.max_blocks = 1;
+            pp.n_blocks = (int32_t)kv->exp_cap;
+        }
         const cudaError_t pe = ltkv::launch_prefix(pp, n_items, (int)kv->cfg.head_dim, st);
         if (pe != cudaSuccess) {
             rollback();
@@ -955,6 +992,18 @@ lt_status lt_kv_create(const lt_kv_config* cfg, lt_kv** out) {
                             "cudaDeviceGetAttribute");
         if (rc == LT_OK) ck(cudaMalloc(&kv->d_pre_o, pre_rows * c.head_dim * sizeof(float) + 16), "cudaMalloc(prefix)");
         if (rc == LT_OK) ck(cudaMalloc(&kv->d_pre_ml, pre_rows * 2 * sizeof(float) + 16), "cudaMalloc(prefix)");
+        if (kv->fmt == LT_KV_Q4_0) {
+            // Workspace of the prefix pass: one layer's blocks as f16 tiles, at
+            // most kExpandBytes of them (32 k tokens of 8 heads x 128).
+            const size_t blk = (size_t)c.n_kv_heads * 4 * kBlock * c.head_dim;
+            kv->exp_cap = std::min<size_t>(kv->n_blocks, kExpandBytes / blk);
+            std::vector<int32_t> iota(kv->exp_cap + 1);
+            for (size_t i = 0; i < iota.size(); ++i) iota[i] = (int32_t)i;
+            if (rc == LT_OK) ck(cudaMalloc(&kv->d_exp, kv->exp_cap * blk + 16), "cudaMalloc(expand)");
+            if (rc == LT_OK) ck(cudaMalloc(&kv->d_iota, iota.size() * 4), "cudaMalloc(expand)");
+            if (rc == LT_OK)
+                ck(cudaMemcpy(kv->d_iota, iota.data(), iota.size() * 4, cudaMemcpyHostToDevice), "cudaMemcpy(expand)");
+        }
         if (rc == LT_OK) ck(cudaMalloc(&kv->d_err, sizeof(int32_t)), "cudaMalloc(err)");
         if (rc == LT_OK) ck(cudaMemset(kv->d_err, 0, sizeof(int32_t)), "cudaMemset(err)");
         kv->slot_bytes = std::max<size_t>(1u << 20, sizeof(ltkv::TokenDesc) * (size_t)c.max_batch + 64);

@@ -191,6 +191,16 @@ cudaError_t launch_write(uint16_t* pool_layer, const int2* cells, int n, int n_k
 cudaError_t launch_write_q4(uint8_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, const void* k,
                             const void* v, int in_f32, cudaStream_t s);
 
+// Blocks [0, count) of sequence root's table, expanded to f16 tiles as blocks
+// base, base + 1, ... of a workspace.
+struct ExpandGroup {
+    int32_t root, base, count;
+};
+constexpr int kExpandGroups = 128;  // groups of one launch (kernel parameters)
+cudaError_t launch_expand_q4(const uint8_t* pool_layer, const int32_t* tables, int max_blocks, const ExpandGroup* groups,
+                             int n_groups, int n_kv_heads, int head_dim, uint16_t* out, int n_blocks, int32_t* err,
+                             cudaStream_t s);
+
 // Values of n cells of a pool of any format -> k_out, v_out [n][n_kv_heads*head_dim], f32 or f16.
 cudaError_t launch_read(const uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, void* k_out,
                         void* v_out, int out_f32, int fmt, cudaStream_t s);

@@ -223,18 +223,35 @@ cudaError_t launch_read_fmt(const uint8_t* pool, const int2* cells, const int32_
 // that the 4-bit tile is the A operand of mma.sync m16n8k16 (16 slots x 16
 // dims, or 16 dims x 16 slots), one 32-bit word of codes per lane and step, and
 // the query heads are the 8 columns of B:
-//   K: a code under a 4-bit mask is, read as f16, the subnormal code * 2^-24
-//      (or 2^-20 from the high nibble, whose dims meet q / 16): exact, for one
-//      logic operation per pair.  sum (code - 8) q = sum code q - 8 sum q, the
-//      second term being the accumulator's start value, formed once per q row;
-//      each group's partial scores are scaled by the slots' scales in f32.
-//   V: the codes become (code - 8) * d in f16, exactly (two f16 operations).
+//   K: the codes become code - 8 in f16 (one logic and one f16 operation a
+//      pair); each group's partial scores are scaled by the slots' scales in f32.
+//      (A masked code read as the subnormal f16 code * 2^-24 would save the f16
+//      operation, but the MMA aligns its products by their exponent fields:
+//      the scores then lose ~10 bits, 2.5e-6 of an output against 4e-7.)
+//   V: the codes become (code - 8) * d in f16, exactly (one operation more).
 // q and P are split into an f16 value and its f16 residual (~22 bits).  With a
 // group of at most 4 heads (PACK) the 8 columns hold both (columns 0-3 the
 // values, 4-7 the residuals), so one MMA carries them; larger groups take two.
 // P^T in B-operand form is the transpose of the scores' fragment: movmatrix.
+//
+// A warp takes two tiles a step: their score chains (MMA, scale, max, 2^x,
+// transpose, MMA) are independent and fill one another's latencies, and the
+// barriers, the maximum's vote and the issuer's bookkeeping are paid once.
 constexpr int kQ4Warps = 4;
 constexpr int kQ4Stages = 6;
+constexpr int kQ4Step = 2;  // tiles a step
+
+// D = A * B (f16, f32 accumulators from zero), D += A * B.
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma16816_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
     uint32_t y;
@@ -242,17 +259,26 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
     return y;
 }
 
-// D = A * B + C with separate C (the start value of a group's partial scores).
-__device__ __forceinline__ void mma16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
-                                              float c1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%10,%11,%10,%11};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
-}
-
 __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+
+// The low (high) nibbles of bytes 0 and 2 of w, minus 8, as two f16s: 1024 +
+// code (64 + code) is the f16 whose last bits are the nibble.  The exponent
+// patterns come in registers (`magic`), so that one three-input logic
+// operation does mask and exponent (it takes one immediate only).
+struct Q4Magic {
+    uint32_t low, high;
+};
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    return r;
+}
+__device__ __forceinline__ __half2 q4_low(uint32_t w, const Q4Magic& m) {
+    return __hsub2(as_h2(and_or(w, 0x000f000fu, m.low)), __floats2half2_rn(1032.f, 1032.f));
+}
+__device__ __forceinline__ __half2 q4_high(uint32_t w, const Q4Magic& m) {
+    return __hsub2(as_h2(and_or(w, 0x00f000f0u, m.high)), __floats2half2_rn(72.f, 72.f));
+}
 
 // A piece: tiles [b0, b1) (counted from block skip) of (token, head).
 // kind: 0 whole (token, head) -> output; 1 it started before this warp's range
@@ -260,17 +286,87 @@ __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<
 struct Q4Piece {
     int tok, h, seq, pos, b0, b1, kind, last_block, skip;
     int lo, qpos;
-    long long ps;
+    int ps;  // first tile of the (token, head)
 };
+constexpr int kQ4Pieces = 4;  // pieces a warp has in hand: consumed, issued, the next one (a power of two)
 
 __host__ __device__ inline int q4_qbuf_bytes(int group, int head_dim, int q_f32) {
     return (group * head_dim * (q_f32 ? 4 : 2) + 127) & ~127;
 }
+// Two q buffers, so that the issuer runs a piece ahead from the start; one
+// where two would cost the third resident CTA.
+__host__ __device__ inline int q4_qbufs(int group, int head_dim, int q_f32) {
+    return q4_qbuf_bytes(group, head_dim, q_f32) > 2048 ? 1 : 2;
+}
 __host__ __device__ inline int q4_warp_smem(int group, int head_dim, int q_f32) {
-    return kQ4Stages * q4_tile_bytes(head_dim) + q4_qbuf_bytes(group, head_dim, q_f32);
+    return kQ4Stages * q4_tile_bytes(head_dim) +
+           q4_qbufs(group, head_dim, q_f32) * q4_qbuf_bytes(group, head_dim, q_f32);
 }
 __host__ __device__ inline int q4_smem(int group, int head_dim, int q_f32) {
-    return kQ4Warps * (q4_warp_smem(group, head_dim, q_f32) + kQ4Stages * 8);
+    return kQ4Warps * (q4_warp_smem(group, head_dim, q_f32) + kQ4Pieces * (int)sizeof(Q4Piece) + kQ4Stages * 8);
+}
+
+// -------------------------------------------------------------- expand ----
+// 4-bit tiles -> f16 tiles (lt_kv_layout.cuh) for the shared-prefix pass, whose
+// tensor-core operands they are.  One warp per (block, head).  The words are
+// read and dequantised as the attention kernel's A fragments; V's are turned
+// over by movmatrix, so that every register is two neighbouring dims of a slot
+// and four lanes store one 16-byte chunk.  Reads 18*D bytes and writes 64*D.
+struct ExpandParams {
+    const uint8_t* pool;
+    const int32_t* tables;
+    uint16_t* out;
+    int32_t* err;
+    int max_blocks, n_kv_heads, n_blocks, n_groups, total;  // total: blocks of all groups
+    ExpandGroup groups[kExpandGroups];
+    int first[kExpandGroups];  // blocks before each group
+};
+
+template <int D>
+__global__ void __launch_bounds__(256) expand_q4_kernel(const __grid_constant__ ExpandParams p) {
+    constexpr int G32 = D / 32;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int item = (int)((blockIdx.x * 256u + threadIdx.x) >> 5);
+    if (item >= p.total * p.n_kv_heads) return;
+    const int h = item % p.n_kv_heads, b = item / p.n_kv_heads;
+    int lo = 0, hi = p.n_groups - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.first[mid] <= b) lo = mid; else hi = mid - 1;
+    }
+    const ExpandGroup gr = p.groups[lo];
+    const int i = b - p.first[lo];
+    const int src = checked_block(__ldg(p.tables + (size_t)gr.root * p.max_blocks + i), p.n_blocks, p.err);
+    const uint8_t* tile = p.pool + ((size_t)src * p.n_kv_heads + h) * q4_tile_bytes(D);
+    uint16_t* out = p.out + ((size_t)(gr.base + i) * p.n_kv_heads + h) * (2 * kBlock * D);
+    const Q4Magic magic{0x64006400u, 0x54005400u};
+    auto put = [&](int kvsel, int slot, int e, __half2 v) {  // dims e, e + 1 of a slot
+        *reinterpret_cast<__half2*>(out + kvsel * kBlock * D + chunk_off(e >> 3, slot) + (e & 7)) = v;
+    };
+#pragma unroll
+    for (int ch = 0; ch < D / 64; ++ch) {
+        const uint4 kw = __ldg(reinterpret_cast<const uint4*>(tile + ch * 512 + lane * 16));
+        const uint4 vw = __ldg(reinterpret_cast<const uint4*>(tile + 8 * D + ch * 512 + lane * 16));
+        const uint4 vd = __ldg(reinterpret_cast<const uint4*>(tile + 17 * D + (t * G32 + 2 * ch) * 8));
+        const __half* ks = reinterpret_cast<const __half*>(tile + 16 * D + g * (4 * G32));
+        const uint32_t kws[4] = {kw.x, kw.y, kw.z, kw.w}, vws[4] = {vw.x, vw.y, vw.z, vw.w};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int e = 16 * (4 * ch + s) + 2 * t, c = 2 * ch + (s >> 1);
+            const __half2 d0 = __half2half2(ks[c]), d1 = __half2half2(ks[G32 + c]);  // slots g, g + 8
+            const uint32_t w = kws[s], w8 = w >> 8;
+            put(0, g, e, __hmul2(q4_low(w, magic), d0));
+            put(0, g, e + 8, __hmul2(q4_high(w, magic), d0));
+            put(0, g + 8, e, __hmul2(q4_low(w8, magic), d1));
+            put(0, g + 8, e + 8, __hmul2(q4_high(w8, magic), d1));
+            const uint32_t x = vws[s], x8 = x >> 8;
+            const __half2 dA = as_h2(s < 2 ? vd.x : vd.z), dB = as_h2(s < 2 ? vd.y : vd.w);
+            put(1, g, e, as_h2(movmatrix_trans(h2_bits(__hmul2(q4_low(x, magic), dA)))));
+            put(1, g, e + 8, as_h2(movmatrix_trans(h2_bits(__hmul2(q4_high(x, magic), dA)))));
+            put(1, g + 8, e, as_h2(movmatrix_trans(h2_bits(__hmul2(q4_low(x8, magic), dB)))));
+            put(1, g + 8, e + 8, as_h2(movmatrix_trans(h2_bits(__hmul2(q4_high(x8, magic), dB)))));
+        }
+    }
 }
 
 // The values of a (token, head)'s result that one lane holds once the columns
@@ -331,52 +427,52 @@ __device__ __forceinline__ void q4_merge_slots(const float* po, const float* pml
     }
 }
 
-// Store a partial (slot w) or the output rows of (tok, h).
+// Fold the prefix pass's partials (lt_kv_kernels.cu) of the blocks before
+// `skip` into (M, L, acc); the same log2 units.
 template <int D, bool PACK>
-__device__ __forceinline__ void q4_store_partial(float* po, float* pml, int G, int g, int t, size_t w,
-                                                 const float (&M)[2], const float (&L)[2],
-                                                 const float (&acc)[D / 16][Own<PACK>::N]) {
+__device__ __forceinline__ void q4_fold_prefix(const AttnParams& p, int tok, int h, int g, int t, float (&M)[2],
+                                               float (&L)[2], float (&acc)[D / 16][Own<PACK>::N]) {
     using O = Own<PACK>;
-#pragma unroll
-    for (int v = 0; v < O::N; ++v) {
-        const int h = O::head(v, t);
-        if (h < G) {
-            float* dst = po + (w * G + h) * D + g + 8 * O::row(v, t);
-#pragma unroll
-            for (int m = 0; m < D / 16; ++m) dst[16 * m] = acc[m][v];
-        }
-    }
-    if (g == 0 && (!PACK || t < 2)) {
+    const size_t r0 = ((size_t)tok * p.n_kv_heads + h) * p.group;
+#pragma unroll 1
+    for (int sp = 0; sp < p.pre_splits; ++sp) {
+        const size_t rs = r0 + (size_t)sp * p.pre_split_rows;
+        float a[2], b[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const int h = O::head(c, t);
-            if (h < G) {
-                pml[(w * G + h) * 2] = M[c];
-                pml[(w * G + h) * 2 + 1] = L[c];
-            }
+            const size_t r = rs + min(O::head(c, t), p.group - 1);
+            const float mp = __ldcg(p.pre_ml + r * 2), lp = __ldcg(p.pre_ml + r * 2 + 1);
+            const float Mn = fmaxf(M[c], mp);
+            a[c] = M[c] == Mn ? 1.f : ex2(M[c] - Mn);
+            b[c] = mp == Mn ? 1.f : ex2(mp - Mn);
+            M[c] = Mn;
+            L[c] = L[c] * a[c] + lp * b[c];
+        }
+#pragma unroll
+        for (int v = 0; v < O::N; ++v) {
+            const float* src = p.pre_o + (rs + min(O::head(v, t), p.group - 1)) * D + g + 8 * O::row(v, t);
+#pragma unroll
+            for (int m = 0; m < D / 16; ++m) acc[m][v] = acc[m][v] * a[O::col(v)] + __ldcg(src + 16 * m) * b[O::col(v)];
         }
     }
 }
 
+// Store the heads' rows at `dst` ([group][D] f32 or f16), each times inv of its column.
 template <int D, bool PACK>
-__device__ __forceinline__ void q4_store_out(const AttnParams& p, int tok, int h, int g, int t, const float (&L)[2],
-                                             const float (&acc)[D / 16][Own<PACK>::N]) {
+__device__ __forceinline__ void q4_store_rows(void* dst, bool f16, int G, int g, int t, const float (&inv)[2],
+                                              const float (&acc)[D / 16][Own<PACK>::N]) {
     using O = Own<PACK>;
-    const int hl = p.n_kv_heads * p.group;
-    const size_t row0 = p.n_peers == 0 ? (size_t)tok * hl + (size_t)h * p.group
-                                       : (size_t)tok * p.n_peers * hl + (size_t)p.peer_rank * hl + (size_t)h * p.group;
-    void* out = p.n_peers == 0 ? p.out : p.gather_out;
 #pragma unroll
     for (int v = 0; v < O::N; ++v) {
-        const int hh = O::head(v, t);
-        if (hh >= p.group) continue;
-        const float l = L[O::col(v)];
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: an interval without positions
-        const size_t at = (row0 + hh) * D + g + 8 * O::row(v, t);
+        const int h = O::head(v, t);
+        if (h >= G) continue;
+        const int at = h * D + g + 8 * O::row(v, t);
+        const float s = inv[O::col(v)];
 #pragma unroll
         for (int m = 0; m < D / 16; ++m) {
-            if (p.out_f32) static_cast<float*>(out)[at + 16 * m] = acc[m][v] * inv;
-            else static_cast<__half*>(out)[at + 16 * m] = __float2half_rn(acc[m][v] * inv);
+            const float x = acc[m][v] * s;
+            if (f16) static_cast<__half*>(dst)[at + 16 * m] = __float2half_rn(x);
+            else static_cast<float*>(dst)[at + 16 * m] = x;
         }
     }
 }
@@ -386,7 +482,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
     constexpr int TILE = q4_tile_bytes(D);
     constexpr int KS = D / 16;   // 16-dim steps of K, and 16-dim row tiles of V
     constexpr int G32 = D / 32;  // scale groups
-    constexpr int S = kQ4Stages;
+    constexpr int S = kQ4Stages, NT = kQ4Step;
     using O = Own<PACK>;
     extern __shared__ __align__(1024) uint8_t smem[];
 
@@ -394,9 +490,13 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int gw = blockIdx.x * kQ4Warps + warp;
     const int Hkv = p.n_kv_heads, G = p.group;
-    uint8_t* stages = smem + (size_t)warp * q4_warp_smem(G, D, p.q_f32);
-    uint8_t* qbuf = stages + S * TILE;
-    const uint32_t bar0 = smem_u32(smem + (size_t)kQ4Warps * q4_warp_smem(G, D, p.q_f32)) + 8u * S * warp;
+    const int QBUF = q4_qbuf_bytes(G, D, p.q_f32), nqb = q4_qbufs(G, D, p.q_f32);
+    const int WSM = q4_warp_smem(G, D, p.q_f32);
+    uint8_t* stages = smem + (size_t)warp * WSM;
+    uint8_t* qbufs = stages + S * TILE;
+    Q4Piece* pieces = reinterpret_cast<Q4Piece*>(smem + (size_t)kQ4Warps * WSM) + warp * kQ4Pieces;
+    const uint32_t bar0 =
+        smem_u32(smem + (size_t)kQ4Warps * (WSM + kQ4Pieces * sizeof(Q4Piece))) + 8u * S * warp;
     if (lane < S) mbar_init(bar0 + 8u * lane, 1);
     fence_mbar_init();
     __syncwarp();
@@ -404,47 +504,54 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
 
     const TokenDesc* toks = p.toks ? p.toks : p.inl;
     const uint8_t* pool = reinterpret_cast<const uint8_t*>(p.pool_layer);
-    const long long T = (long long)p.tiles_per_head * Hkv;
-    const long long t0 = T * gw / p.n_warps, t1 = T * (gw + 1) / p.n_warps;
+    // Range [T * gw / n, T * (gw + 1) / n) of the T < 2^31 tiles, in 32 bits:
+    // with T = quo * n + rem, floor(T * w / n) = quo * w + floor(rem * w / n).
+    const uint32_t T = (uint32_t)p.tiles_per_head * Hkv;
+    const uint32_t NWu = (uint32_t)p.n_warps, quo = T / NWu, rem = T % NWu;
+    const int t0 = (int)(quo * gw + rem * gw / NWu), t1 = (int)(quo * (gw + 1) + rem * (gw + 1) / NWu);
     const int g = lane >> 2, t = lane & 3;
     const int qelem = p.q_f32 ? 4 : 2;
     const uint32_t qbytes = (uint32_t)(G * D * qelem);
 
-    // ---- piece generator over [t0, t1) ----
-    int gi, gh, gb;
-    long long gt = t0;
+    // ---- piece generator over [t0, t1): piece i goes to slot i % kQ4Pieces ----
+    int gi, gh, gb, gt = t0, gn = 0;
     {
-        int lo = 0, hi = p.n_tok - 1;
+        int lo = 0, hi = p.n_tok - 1;  // last token whose first tile is <= t0
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if ((long long)toks[mid].prefix * Hkv <= t0) lo = mid; else hi = mid - 1;
+            if (toks[mid].prefix * Hkv <= t0) lo = mid; else hi = mid - 1;
         }
         gi = lo;
         const TokenDesc td = toks[gi];
-        const int nb = td.pos / kBlock + 1 - td.skip;
-        const long long off = t0 - (long long)td.prefix * Hkv;
+        const uint32_t nb = (uint32_t)(td.pos / kBlock + 1 - td.skip), off = (uint32_t)(t0 - td.prefix * Hkv);
         gh = (int)(off / nb);
         gb = (int)(off % nb);
     }
-    auto gen_piece = [&](Q4Piece& r) {
+    auto gen_piece = [&]() {
         const TokenDesc td = toks[gi];
         const int nb = td.pos / kBlock + 1 - td.skip;
-        const int len = (int)min((long long)(nb - gb), t1 - gt);
-        r.tok = gi;
-        r.skip = td.skip;
-        r.h = gh;
-        r.seq = td.seq;
-        r.pos = td.pos;
-        r.b0 = gb;
-        r.b1 = gb + len;
-        r.ps = (long long)td.prefix * Hkv + (long long)gh * nb;
-        r.kind = r.ps < t0 ? 1 : (r.ps + nb > t1 ? 2 : 0);
-        r.last_block = r.b1 == nb ? td.last_block : -1;
-        if constexpr (SH) {
-            const ShapeDesc sd = p.shapes ? p.shapes[gi] : p.inl_shapes[gi];
-            r.lo = sd.lo;
-            r.qpos = sd.qpos;
+        const int len = min(nb - gb, t1 - gt);
+        if (lane == 0) {
+            Q4Piece r;
+            r.tok = gi;
+            r.skip = td.skip;
+            r.h = gh;
+            r.seq = td.seq;
+            r.pos = td.pos;
+            r.b0 = gb;
+            r.b1 = gb + len;
+            r.ps = td.prefix * Hkv + gh * nb;
+            r.kind = r.ps < t0 ? 1 : (r.ps + nb > t1 ? 2 : 0);
+            r.last_block = r.b1 == nb ? td.last_block : -1;
+            r.lo = r.qpos = 0;
+            if constexpr (SH) {
+                const ShapeDesc sd = p.shapes ? p.shapes[gi] : p.inl_shapes[gi];
+                r.lo = sd.lo;
+                r.qpos = sd.qpos;
+            }
+            pieces[gn & (kQ4Pieces - 1)] = r;
         }
+        ++gn;
         gt += len;
         gb += len;
         if (gb == nb) {
@@ -454,6 +561,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
                 ++gi;
             }
         }
+        __syncwarp();
     };
     // block ids [b, min(b + 32, b1)) of a piece, lane j holding b + j
     auto load_window = [&](const Q4Piece& r, int b) {
@@ -464,76 +572,91 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
                              p.check_ids != 0);
     };
 
-    // ---- issuer ----
-    Q4Piece di{}, dn{};
-    gen_piece(di);
-    const long long f_ps = di.ps;
-    const int f_nb = di.pos / kBlock + 1 - di.skip, f_kind = di.kind;
-    bool dn_valid = gt < t1;
-    if (dn_valid) gen_piece(dn);
-    int ii = 0, it = 0, wb = 0;
-    int win = load_window(di, di.b0), win_n = 0;
+    // ---- issuer: piece ii, its tiles [it, d_len) not yet issued ----
+    gen_piece();
+    const bool f_cut = pieces[0].kind == 1;  // the range's first piece continues a cut (token, head)
+    const int f_tok = pieces[0].tok;
+    bool dn_valid = true;  // piece ii + 1 is generated
+    int ii = -1, it = 0, wb = 0, d_len = 0, d_h = 0;
+    int win = 0, win_n = 0;  // block ids [wb, wb + 32) of piece ii, and the 32 that follow (of ii or ii + 1)
     auto prefetch_window = [&]() {
-        if (wb + 32 < di.b1 - di.b0) win_n = load_window(di, di.b0 + wb + 32);
-        else if (dn_valid) win_n = load_window(dn, dn.b0);
+        const bool same = wb + 32 < d_len;
+        if (!same && !dn_valid) return;
+        const Q4Piece& d = pieces[(same ? ii : ii + 1) & (kQ4Pieces - 1)];
+        win_n = load_window(d, same ? d.b0 + wb + 32 : d.b0);
     };
     prefetch_window();
-    auto table_write = [&](const Q4Piece& r) {
-        if (r.h == 0 && r.last_block >= 0 && lane == 0)
-            p.tables[(size_t)r.seq * p.max_blocks + r.skip + r.b1 - 1] = r.last_block;
-    };
-    table_write(di);
     int issued = 0, consumed = 0, istage = 0, cstage = 0, cphase = 0;
-    auto issue_one = [&]() {
-        if (it - wb >= 32) {
-            win = win_n;
-            wb += 32;
-            prefetch_window();
-        }
-        const int b = __shfl_sync(kFull, win, it - wb);
-        if (lane == 0) {
-            const uint32_t bar = bar0 + 8u * istage;
-            mbar_arrive_expect_tx(bar, TILE + (it == 0 ? qbytes : 0u));
-            bulk_g2s(smem_u32(stages + (size_t)istage * TILE), pool + ((size_t)b * Hkv + di.h) * TILE, TILE, bar);
-            if (it == 0)
-                bulk_g2s(smem_u32(qbuf),
-                         static_cast<const uint8_t*>(p.q) + ((size_t)di.tok * Hkv + di.h) * G * D * qelem, qbytes, bar);
-        }
-        ++it;
-        ++issued;
-        istage = istage + 1 == S ? 0 : istage + 1;
-    };
-    auto issuer_advance = [&]() {
-        ++ii;
-        di = dn;
-        dn_valid = gt < t1;
-        if (dn_valid) gen_piece(dn);
-        it = 0;
-        wb = 0;
-        win = win_n;
-        prefetch_window();
-        table_write(di);
-    };
-
-    // ---- consumer ----
-    int ci = 0, ct = 0;
-    Q4Piece dc = di;
-    // The issuer runs at most one piece ahead, and only once the consumer has
-    // taken its own piece's q rows out of the single q buffer (ct > 0).
+    int ci = 0, ct = 0;  // the consumer's piece, and its tiles consumed
+    // Fill the ring: lane u issues the u-th of the next n tiles.  The issuer
+    // runs at most one piece ahead of the consumer, and with a single q buffer
+    // only once the consumer has taken its own piece's q rows (ct > 0).
     auto try_issue = [&]() {
-        while (issued - consumed < S) {
-            if (it < di.b1 - di.b0) {
-                issue_one();
+        for (;;) {
+            const int room = S - (issued - consumed);
+            if (it < d_len) {
+                if (room == 0) break;
+                if (it - wb == 32) {
+                    win = win_n;
+                    wb += 32;
+                    prefetch_window();
+                }
+                const int n = min(min(d_len - it, room), 32 - (it - wb));
+                const int b = __shfl_sync(kFull, win, (it - wb + lane) & 31);
+                if (lane < n) {
+                    int st = istage + lane;
+                    st = st >= S ? st - S : st;
+                    const uint32_t bar = bar0 + 8u * st;
+                    const bool with_q = it + lane == 0;
+                    mbar_arrive_expect_tx(bar, TILE + (with_q ? qbytes : 0u));
+                    bulk_g2s(smem_u32(stages) + st * TILE, pool + ((size_t)b * Hkv + d_h) * TILE, TILE, bar);
+                    if (with_q)
+                        bulk_g2s(smem_u32(qbufs) + (nqb == 2 ? (ii & 1) * QBUF : 0),
+                                 static_cast<const uint8_t*>(p.q) +
+                                     ((size_t)pieces[ii & (kQ4Pieces - 1)].tok * Hkv + d_h) * G * D * qelem,
+                                 qbytes, bar);
+                }
+                it += n;
+                issued += n;
+                istage += n;
+                istage = istage >= S ? istage - S : istage;
                 continue;
             }
-            if (ii != ci || ct == 0 || !dn_valid) break;
-            issuer_advance();
+            if (!dn_valid || ii > ci || (nqb == 1 && ii == ci && ct == 0)) break;
+            // on to the next piece
+            ++ii;
+            const Q4Piece& d = pieces[ii & (kQ4Pieces - 1)];
+            d_len = d.b1 - d.b0;
+            d_h = d.h;
+            dn_valid = gt < t1;
+            if (dn_valid) gen_piece();
+            it = 0;
+            wb = 0;
+            win = win_n;
+            prefetch_window();
+            // the token's last block entry, written once per token (head 0)
+            if (d.h == 0 && d.last_block >= 0 && lane == 0)
+                p.tables[(size_t)d.seq * p.max_blocks + d.skip + d.b1 - 1] = d.last_block;
         }
     };
-    try_issue();
+
+    // ---- consumer: c_* count from the piece's first position ----
+    int c_len, c_end, c_lo, c_q;
+    auto take_piece = [&]() {
+        const Q4Piece& c = pieces[ci & (kQ4Pieces - 1)];
+        const int base = (c.skip + c.b0) * kBlock;
+        c_len = c.b1 - c.b0;
+        c_end = c.pos + 1 - base;
+        c_lo = c.lo - base;
+        c_q = c.qpos - base;
+        ct = 0;
+    };
+    take_piece();
+    // an opaque zero keeps the exponent patterns in registers (see Q4Magic)
+    const uint32_t zero = (uint32_t)p.n_warps >> 31;
+    const Q4Magic magic{0x64006400u + zero, 0x54005400u + zero};
 
     uint32_t qh[KS][2], ql[PACK ? 1 : KS][2];  // B fragments: values (PACK: residuals in columns 4-7), residuals
-    float corr[G32][2];                        // -8 * 2^-24 * (sum of q over the group), columns 2t, 2t + 1
     float cmul[2] = {0.f, 0.f};                // from the MMA's units to q.k (SH) or log2 units
     float slope[2] = {0.f, 0.f};
     float o[KS][4];
@@ -576,113 +699,100 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
         }
     };
 
-    for (;;) {
-        if (!mbar_wait_bounded(bar0 + 8u * cstage, (uint32_t)cphase)) {
-            ok = false;
-            break;
+    // ---- q rows of a piece -> B fragments ----
+    auto load_q = [&](const uint8_t* qbuf) {
+        const int qg = PACK ? g & 3 : g;
+        float x[KS][4];
+        float mx = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                float2 f = make_float2(0.f, 0.f);
+                if (qg < G) {
+                    const int e = qg * D + ks * 16 + hf * 8 + 2 * t;
+                    if (p.q_f32) f = *reinterpret_cast<const float2*>(qbuf + e * 4);
+                    else f = __half22float2(*reinterpret_cast<const __half2*>(qbuf + e * 2));
+                }
+                x[ks][2 * hf] = f.x;
+                x[ks][2 * hf + 1] = f.y;
+                mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
         }
-        uint8_t* tile = stages + (size_t)cstage * TILE;
-        if (ct == 0) {
-            // ---- q rows of this piece -> B fragments ----
-            const int qg = PACK ? g & 3 : g;
-            float x[KS][4];
-            float mx = 0.f;
+        // Scale each row by a power of two that brings its largest value near
+        // 2^12: value and residual are then normal f16s.
+        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
+        const int ex = (int)(__float_as_uint(mx) >> 23);  // 255: Inf, which no scale helps
+        const int fe = ex == 255 ? 127 : min(253, max(1, 266 - ex));
+        const float f = __uint_as_float((uint32_t)fe << 23), finv = __uint_as_float((uint32_t)(254 - fe) << 23);
+        const bool resid = PACK && g >= 4;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
+        for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    float2 f = make_float2(0.f, 0.f);
-                    if (qg < G) {
-                        const int e = qg * D + ks * 16 + hf * 8 + 2 * t;
-                        if (p.q_f32) f = *reinterpret_cast<const float2*>(qbuf + e * 4);
-                        else f = __half22float2(*reinterpret_cast<const __half2*>(qbuf + e * 2));
-                    }
-                    x[ks][2 * hf] = f.x;
-                    x[ks][2 * hf + 1] = f.y;
-                    mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-                }
-            }
-            // Scale each row by a power of two that brings its largest value
-            // near 2^12: value, residual and q / 16 are then normal f16s.
-            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
-            const int ex = (int)(__float_as_uint(mx) >> 23);  // 255: Inf, which no scale helps
-            const int fe = ex == 255 ? 127 : min(253, max(1, 266 - ex));
-            const float f = __uint_as_float((uint32_t)fe << 23), finv = __uint_as_float((uint32_t)(254 - fe) << 23);
-            const bool resid = PACK && g >= 4;
-            float csum[G32];
-#pragma unroll
-            for (int c = 0; c < G32; ++c) csum[c] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const float s = hf ? f * 0.0625f : f;  // high nibbles weigh 16 times as much
-                    const float y0 = x[ks][2 * hf] * s, y1 = x[ks][2 * hf + 1] * s;
-                    __half2 hi = __floats2half2_rn(y0, y1);
-                    float2 back = __half22float2(hi);
-                    const __half2 lo = __floats2half2_rn(y0 - back.x, y1 - back.y);
-                    const float2 lback = __half22float2(lo);
-                    if constexpr (PACK) {
-                        if (resid) {
-                            hi = lo;
-                            back = lback;
-                        }
-                        qh[ks][hf] = h2_bits(hi);
-                        csum[ks >> 1] += (back.x + back.y) * (hf ? 16.f : 1.f);
-                    } else {
-                        qh[ks][hf] = h2_bits(hi);
-                        ql[ks][hf] = h2_bits(lo);
-                        csum[ks >> 1] += ((back.x + back.y) + (lback.x + lback.y)) * (hf ? 16.f : 1.f);
-                    }
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < G32; ++c) {
-                float v = csum[c];
-                v += __shfl_xor_sync(kFull, v, 1);
-                v += __shfl_xor_sync(kFull, v, 2);
-                corr[c][0] = __shfl_sync(kFull, v, 8 * t) * -4.76837158203125e-7f;  // -8 * 2^-24
-                corr[c][1] = __shfl_sync(kFull, v, 8 * t + 4) * -4.76837158203125e-7f;
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                cmul[c] = __shfl_sync(kFull, finv, 8 * t + 4 * c) * 16777216.f;  // 2^24
-                if constexpr (SH) {
-                    const int hh = O::head(c, t);
-                    slope[c] = p.shape.slopes && hh < G ? __ldg(p.shape.slopes + dc.h * G + hh) * kLog2e : 0.f;
+            for (int hf = 0; hf < 2; ++hf) {
+                const float y0 = x[ks][2 * hf] * f, y1 = x[ks][2 * hf + 1] * f;
+                const __half2 hi = __floats2half2_rn(y0, y1);
+                const float2 back = __half22float2(hi);
+                const __half2 lo = __floats2half2_rn(y0 - back.x, y1 - back.y);
+                if constexpr (PACK) {
+                    qh[ks][hf] = h2_bits(resid ? lo : hi);
                 } else {
-                    cmul[c] *= p.scale_log2;
+                    qh[ks][hf] = h2_bits(hi);
+                    ql[ks][hf] = h2_bits(lo);
                 }
             }
         }
-        const int b = dc.b0 + ct;  // from block dc.skip
-        const int valid = min(kBlock, dc.pos + 1 - (dc.skip + b) * kBlock);
-        bool touched = false;
-        if (!SH && p.k_new && dc.last_block >= 0 && b == dc.b1 - 1) {
-            // Fused append: quantise this token's new K and V row of head h
-            // into its pool cell and into the staged tile.
-            constexpr int L = D / 4;  // lanes of one row
-            const int slot = dc.pos % kBlock;
-            uint8_t* cell_tile = reinterpret_cast<uint8_t*>(p.pool_layer_w) + ((size_t)dc.last_block * Hkv + dc.h) * TILE;
 #pragma unroll
-            for (int r = 0; r < 2 * L / 32; ++r) {
-                const int kvsel = (r * 32 + lane) / L, i = (lane % L) >> 2;
-                float x[4];
-                load4_f32(kvsel ? p.v_new : p.k_new, (size_t)dc.tok * Hkv * D + (size_t)dc.h * D + 16 * i + 2 * t,
-                          p.kv_f32, x);
-                uint32_t code[4];
-                const float d = q4_quant4(x, code);
-                q4_store4<D>(tile, kvsel, i, t, slot, code, d);
-                q4_store4<D>(cell_tile, kvsel, i, t, slot, code, d);
+        for (int c = 0; c < 2; ++c) {
+            cmul[c] = __shfl_sync(kFull, finv, 8 * t + 4 * c);
+            if constexpr (SH) {
+                const int hh = O::head(c, t);
+                slope[c] = p.shape.slopes && hh < G
+                               ? __ldg(p.shape.slopes + pieces[ci & (kQ4Pieces - 1)].h * G + hh) * kLog2e
+                               : 0.f;
+            } else {
+                cmul[c] *= p.scale_log2;
             }
-            touched = true;
-            __syncwarp();
         }
+    };
 
-        // ---- S^T = K Q^T ----
-        float sc[4] = {0.f, 0.f, 0.f, 0.f};  // (slot g | g+8) x (column 2t | 2t+1)
-        {
+    // Fused append: quantise this token's new K and V row of head h into its
+    // pool cell and into the staged tile.
+    auto append = [&](uint8_t* tile) {
+        constexpr int L = D / 4;  // lanes of one row
+        const Q4Piece dc = pieces[ci & (kQ4Pieces - 1)];
+        const int slot = dc.pos % kBlock;
+        uint8_t* cell_tile = reinterpret_cast<uint8_t*>(p.pool_layer_w) + ((size_t)dc.last_block * Hkv + dc.h) * TILE;
+#pragma unroll 1
+        for (int r = 0; r < 2 * L / 32; ++r) {
+            const int kvsel = (r * 32 + lane) / L, i = (lane % L) >> 2;
+            float x[4];
+            load4_f32(kvsel ? p.v_new : p.k_new, (size_t)dc.tok * Hkv * D + (size_t)dc.h * D + 16 * i + 2 * t, p.kv_f32,
+                      x);
+            uint32_t code[4];
+            const float d = q4_quant4(x, code);
+            q4_store4<D>(tile, kvsel, i, t, slot, code, d);
+            q4_store4<D>(cell_tile, kvsel, i, t, slot, code, d);
+        }
+        __syncwarp();
+    };
+
+    // ---- the next nt <= NT staged tiles, blocks ct .. of the piece ----
+    // A step short of a tile takes its first tile again with every score -inf
+    // (weights 0, finite values): one copy of the code serves both.
+    auto step = [&](int nt) {
+        const uint8_t* tiles[NT];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            const int st = cstage + (u < nt ? u : 0);
+            tiles[u] = stages + (size_t)(st >= S ? st - S : st) * TILE;
+        }
+        // S^T = K Q^T
+        float sc[NT][4];  // (slot g | g+8) x (column 2t | 2t+1)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            const uint8_t* tile = tiles[u];
             uint32_t kd[G32];  // scales of slot g (first half of the run) and g+8
             const uint8_t* ks_p = tile + 16 * D + g * (4 * G32);
             if constexpr (D == 128) {
@@ -700,51 +810,65 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
                 const float2 dg8 = __half22float2(as_h2(kd[G32 / 2 + ch]));  // slot g+8
 #pragma unroll
                 for (int cc = 0; cc < 2; ++cc) {
-                    const int c = 2 * ch + cc;
                     float tt[4];
 #pragma unroll
                     for (int q2 = 0; q2 < 2; ++q2) {
-                        const int ks = 2 * c + q2;
+                        const int ks = 4 * ch + 2 * cc + q2;
                         const uint32_t w0 = w[2 * cc + q2], w8 = w0 >> 8;
-                        const uint32_t a[4] = {w0 & 0x000f000fu, w8 & 0x000f000fu, w0 & 0x00f000f0u, w8 & 0x00f000f0u};
-                        if (q2 == 0) mma16816_from(tt, a, qh[ks][0], qh[ks][1], corr[c][0], corr[c][1]);
-                        else mma16816(tt, a, qh[ks][0], qh[ks][1]);
-                        if constexpr (!PACK) mma16816(tt, a, ql[ks][0], ql[ks][1]);
+                        const uint32_t a[4] = {h2_bits(q4_low(w0, magic)), h2_bits(q4_low(w8, magic)), h2_bits(q4_high(w0, magic)),
+                                               h2_bits(q4_high(w8, magic))};
+                        if (q2 == 0) mma16816_zero(tt, a, qh[ks][0], qh[ks][1]);
+                        else mma16816_add(tt, a, qh[ks][0], qh[ks][1]);
+                        if constexpr (!PACK) mma16816_add(tt, a, ql[ks][0], ql[ks][1]);
                     }
                     const float d0 = cc ? dg.y : dg.x, d1 = cc ? dg8.y : dg8.x;
-                    sc[0] += d0 * tt[0];
-                    sc[1] += d0 * tt[1];
-                    sc[2] += d1 * tt[2];
-                    sc[3] += d1 * tt[3];
+                    const bool first = ch == 0 && cc == 0;
+                    sc[u][0] = first ? d0 * tt[0] : sc[u][0] + d0 * tt[0];
+                    sc[u][1] = first ? d0 * tt[1] : sc[u][1] + d0 * tt[1];
+                    sc[u][2] = first ? d1 * tt[2] : sc[u][2] + d1 * tt[2];
+                    sc[u][3] = first ? d1 * tt[3] : sc[u][3] + d1 * tt[3];
                 }
             }
         }
-        if constexpr (PACK) {
+        const int j0 = ct * kBlock;  // first position of the step in the piece
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[e] += __shfl_xor_sync(kFull, sc[e], 2);
+        for (int u = 0; u < NT; ++u) {
+            if constexpr (PACK) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[u][e] += __shfl_xor_sync(kFull, sc[u][e], 2);
+            }
+            if constexpr (SH) {
+                const int ju = j0 + u * kBlock, lo = c_lo - ju;
+                const TileShape s0{p.shape, slope[0], c_q - ju, lo}, s1{p.shape, slope[1], c_q - ju, lo};
+                sc[u][0] = s0.score(sc[u][0] * cmul[0], g);
+                sc[u][1] = s1.score(sc[u][1] * cmul[1], g);
+                sc[u][2] = s0.score(sc[u][2] * cmul[0], g + 8);
+                sc[u][3] = s1.score(sc[u][3] * cmul[1], g + 8);
+                if (g < lo) sc[u][0] = sc[u][1] = -INFINITY;
+                if (g + 8 < lo) sc[u][2] = sc[u][3] = -INFINITY;
+            } else {
+                sc[u][0] *= cmul[0];
+                sc[u][1] *= cmul[1];
+                sc[u][2] *= cmul[0];
+                sc[u][3] *= cmul[1];
+            }
         }
-        if constexpr (SH) {
-            const int j0 = (dc.skip + b) * kBlock, lo = dc.lo - j0;
-            const TileShape s0{p.shape, slope[0], dc.qpos - j0, lo}, s1{p.shape, slope[1], dc.qpos - j0, lo};
-            sc[0] = s0.score(sc[0] * cmul[0], g);
-            sc[1] = s1.score(sc[1] * cmul[1], g);
-            sc[2] = s0.score(sc[2] * cmul[0], g + 8);
-            sc[3] = s1.score(sc[3] * cmul[1], g + 8);
-            if (g < lo) sc[0] = sc[1] = -INFINITY;
-            if (g + 8 < lo) sc[2] = sc[3] = -INFINITY;
-        } else {
-            sc[0] *= cmul[0];
-            sc[1] *= cmul[1];
-            sc[2] *= cmul[0];
-            sc[3] *= cmul[1];
-        }
-        if (valid < kBlock) {
-            if (g >= valid) sc[0] = sc[1] = -INFINITY;
-            if (g + 8 >= valid) sc[2] = sc[3] = -INFINITY;
+        const int filled = min(c_end, c_len * kBlock) - j0;  // positions from the step's first to the piece's end
+        if (filled < NT * kBlock) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                if (g + u * kBlock >= filled) sc[u][0] = sc[u][1] = -INFINITY;
+                if (g + 8 + u * kBlock >= filled) sc[u][2] = sc[u][3] = -INFINITY;
+            }
         }
 
-        // ---- softmax ----
-        float mx0 = fmaxf(sc[0], sc[2]), mx1 = fmaxf(sc[1], sc[3]);
+        // softmax
+        float mx0 = fmaxf(sc[0][0], sc[0][2]), mx1 = fmaxf(sc[0][1], sc[0][3]);
+#pragma unroll
+        for (int u = 1; u < NT; ++u) {
+            mx0 = fmaxf(mx0, fmaxf(sc[u][0], sc[u][2]));
+            mx1 = fmaxf(mx1, fmaxf(sc[u][1], sc[u][3]));
+        }
         if (__any_sync(kFull, mx0 > mb[0] + 15.f || mx1 > mb[1] + 15.f)) {
 #pragma unroll
             for (int m = 4; m < 32; m <<= 1) {
@@ -767,136 +891,198 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
         }
         // Nothing seen yet (an empty interval): weights ex2(-inf) = 0.
         const float r0 = SH && mb[0] == -INFINITY ? 0.f : mb[0], r1 = SH && mb[1] == -INFINITY ? 0.f : mb[1];
-        const float p0 = ex2(sc[0] - r0), p1 = ex2(sc[1] - r1), p2 = ex2(sc[2] - r0), p3 = ex2(sc[3] - r1);
-        l_run[0] += p0 + p2;
-        l_run[1] += p1 + p3;
         // P^T as B fragments: value = the leading 11 bits (an f16), residual = the rest.
         constexpr uint32_t kLead = 0xffffe000u;
-        uint32_t ph[2], pl[2];
-        if constexpr (PACK) {
-            // lanes t < 2: minus the value; t >= 2: the residual (join() puts the sign right)
-            const float own = t < 2 ? 0.f : 1.f;
-            auto part = [&](float v) { return fmaf(v, own, -__uint_as_float(__float_as_uint(v) & kLead)); };
-            ph[0] = movmatrix_trans(h2_bits(__floats2half2_rn(part(p0), part(p1))));
-            ph[1] = movmatrix_trans(h2_bits(__floats2half2_rn(part(p2), part(p3))));
-        } else {
-            const float v0 = __uint_as_float(__float_as_uint(p0) & kLead), v1 = __uint_as_float(__float_as_uint(p1) & kLead);
-            const float v2 = __uint_as_float(__float_as_uint(p2) & kLead), v3 = __uint_as_float(__float_as_uint(p3) & kLead);
-            ph[0] = movmatrix_trans(h2_bits(__floats2half2_rn(v0, v1)));
-            ph[1] = movmatrix_trans(h2_bits(__floats2half2_rn(v2, v3)));
-            pl[0] = movmatrix_trans(h2_bits(__floats2half2_rn(p0 - v0, p1 - v1)));
-            pl[1] = movmatrix_trans(h2_bits(__floats2half2_rn(p2 - v2, p3 - v3)));
-        }
-
-        // ---- O^T += V^T P^T ----
-        const __half2 k1032 = __floats2half2_rn(1032.f, 1032.f), k72 = __floats2half2_rn(72.f, 72.f);
+        uint32_t ph[NT][2];
+        [[maybe_unused]] uint32_t pl[PACK ? 1 : NT][2];
+        [[maybe_unused]] const float own = t < 2 ? 0.f : 1.f;
 #pragma unroll
-        for (int ch = 0; ch < D / 64; ++ch) {
-            const uint4 wv = *reinterpret_cast<const uint4*>(tile + 8 * D + ch * 512 + lane * 16);
-            const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w};
-            const uint4 vd = *reinterpret_cast<const uint4*>(tile + 17 * D + (t * G32 + 2 * ch) * 8);
-#pragma unroll
-            for (int mm = 0; mm < 4; ++mm) {
-                const int m = 4 * ch + mm;
-                const __half2 dA = as_h2(mm < 2 ? vd.x : vd.z), dB = as_h2(mm < 2 ? vd.y : vd.w);
-                const uint32_t w0 = w[mm], w8 = w0 >> 8;
-                // 1024 + code and 64 + code are f16s whose last bits are the nibble
-                const uint32_t a[4] = {
-                    h2_bits(__hmul2(__hsub2(as_h2((w0 & 0x000f000fu) | 0x64006400u), k1032), dA)),
-                    h2_bits(__hmul2(__hsub2(as_h2((w0 & 0x00f000f0u) | 0x54005400u), k72), dA)),
-                    h2_bits(__hmul2(__hsub2(as_h2((w8 & 0x000f000fu) | 0x64006400u), k1032), dB)),
-                    h2_bits(__hmul2(__hsub2(as_h2((w8 & 0x00f000f0u) | 0x54005400u), k72), dB))};
-                mma16816(o[m], a, ph[0], ph[1]);
-                if constexpr (!PACK) mma16816(o[m], a, pl[0], pl[1]);
+        for (int u = 0; u < NT; ++u) {
+            const float p0 = ex2(sc[u][0] - r0), p1 = ex2(sc[u][1] - r1), p2 = ex2(sc[u][2] - r0),
+                        p3 = ex2(sc[u][3] - r1);
+            l_run[0] += p0 + p2;
+            l_run[1] += p1 + p3;
+            auto lead = [&](float v) { return __uint_as_float(__float_as_uint(v) & kLead); };
+            if constexpr (PACK) {
+                // lanes t < 2: minus the value; t >= 2: the residual (join() puts the sign right)
+                ph[u][0] = movmatrix_trans(h2_bits(__floats2half2_rn(fmaf(p0, own, -lead(p0)), fmaf(p1, own, -lead(p1)))));
+                ph[u][1] = movmatrix_trans(h2_bits(__floats2half2_rn(fmaf(p2, own, -lead(p2)), fmaf(p3, own, -lead(p3)))));
+            } else {
+                const float v0 = lead(p0), v1 = lead(p1), v2 = lead(p2), v3 = lead(p3);
+                ph[u][0] = movmatrix_trans(h2_bits(__floats2half2_rn(v0, v1)));
+                ph[u][1] = movmatrix_trans(h2_bits(__floats2half2_rn(v2, v3)));
+                pl[u][0] = movmatrix_trans(h2_bits(__floats2half2_rn(p0 - v0, p1 - v1)));
+                pl[u][1] = movmatrix_trans(h2_bits(__floats2half2_rn(p2 - v2, p3 - v3)));
             }
         }
-        ++consumed;
-        if (++cstage == S) {
-            cstage = 0;
+
+        // O^T += V^T P^T
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+#pragma unroll
+            for (int ch = 0; ch < D / 64; ++ch) {
+                const uint4 wv = *reinterpret_cast<const uint4*>(tiles[u] + 8 * D + ch * 512 + lane * 16);
+                const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w};
+                const uint4 vd = *reinterpret_cast<const uint4*>(tiles[u] + 17 * D + (t * G32 + 2 * ch) * 8);
+#pragma unroll
+                for (int mm = 0; mm < 4; ++mm) {
+                    const int m = 4 * ch + mm;
+                    const __half2 dA = as_h2(mm < 2 ? vd.x : vd.z), dB = as_h2(mm < 2 ? vd.y : vd.w);
+                    const uint32_t w0 = w[mm], w8 = w0 >> 8;
+                    const uint32_t a[4] = {h2_bits(__hmul2(q4_low(w0, magic), dA)), h2_bits(__hmul2(q4_high(w0, magic), dA)),
+                                           h2_bits(__hmul2(q4_low(w8, magic), dB)), h2_bits(__hmul2(q4_high(w8, magic), dB))};
+                    mma16816_add(o[m], a, ph[u][0], ph[u][1]);
+                    if constexpr (!PACK) mma16816_add(o[m], a, pl[u][0], pl[u][1]);
+                }
+            }
+        }
+    };
+
+    // The warp that holds tile x: the last w with floor(T * w / n) <= x.
+    auto warp_of = [&](int x) { return (int)(((long long)(x + 1) * p.n_warps - 1) / (long long)T); };
+    for (;;) {
+        try_issue();
+        const int nt = min(c_len - ct, NT);
+        {
+            // lane u waits for the u-th tile of the step
+            const int st = cstage + lane;
+            const bool wrap = st >= S;
+            const bool here = lane >= nt || mbar_wait_bounded(bar0 + 8u * (wrap ? st - S : st), (uint32_t)(cphase ^ wrap));
+            if (!__all_sync(kFull, here)) {
+                ok = false;
+                break;
+            }
+            __syncwarp();  // the waiting lanes' view of the copied bytes reaches the others
+        }
+        if (ct == 0) load_q(qbufs + (nqb == 2 ? (ci & 1) * QBUF : 0));
+        const bool fill = !SH && p.k_new && ct + nt == c_len && pieces[ci & (kQ4Pieces - 1)].last_block >= 0;
+        if (fill) {
+            const int st = cstage + nt - 1;
+            append(stages + (size_t)(st >= S ? st - S : st) * TILE);
+        }
+        step(nt);
+        consumed += nt;
+        cstage += nt;
+        if (cstage >= S) {
+            cstage -= S;
             cphase ^= 1;
         }
-        ++ct;
-        if (touched) fence_proxy_async_smem();
+        ct += nt;
+        if (fill) fence_proxy_async_smem();
         __syncwarp();
+        if (ct < c_len) continue;
 
-        if (ct == dc.b1 - dc.b0) {
-            if (dc.kind == 2) break;  // merged after the loop
-            float M[2], L[2], acc[KS][O::N];
-            join(M, L, acc);
-            if (dc.kind == 0) {
-                ++items_out;
-                q4_store_out<D, PACK>(p, dc.tok, dc.h, g, t, L, acc);
-            } else {
-                q4_store_partial<D, PACK>(p.part_o, p.part_ml, G, g, t, (size_t)gw, M, L, acc);
-            }
-#pragma unroll
-            for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
-            mb[0] = mb[1] = -INFINITY;
-            l_run[0] = l_run[1] = 0.f;
-            if (ii == ci) {
-                if (!dn_valid) break;
-                issuer_advance();
-            }
-            ++ci;
-            dc = di;
-            ct = 0;
+        // ---- piece done ----
+        // what: 0 store the output, 1 the warp's partial, 2 merge the following
+        // warps' partials and store the output, 3 lead: combine the partials of
+        // this warp and its next neighbours into a group partial.
+        const Q4Piece dc = pieces[ci & (kQ4Pieces - 1)];
+        const bool last_piece = ii == ci && !dn_valid;
+        int lead_to = 0;  // last warp of the group this one leads, 0: none
+        if (last_piece && f_cut && p.part2_o) {
+            // Helpers of a cut (token, head) are the warps after the one with
+            // its first tile; with more than kMergeGroup of them, every
+            // kMergeGroup-th leads, so that the merging warp reads one partial a group.
+            const TokenDesc td = toks[f_tok];
+            const int nb = td.pos / kBlock + 1 - td.skip, first = td.prefix * Hkv;
+            const int ps = first + (t0 - first) / nb * nb, ws = warp_of(ps), we = warp_of(ps + nb - 1);
+            if (we - ws > kMergeGroup && (gw - ws - 1) % kMergeGroup == 0) lead_to = min(gw + kMergeGroup - 1, we);
         }
-        try_issue();
-    }
-    if (!ok) {
-        for (int jj = consumed + 1; jj < issued; ++jj) mbar_wait_bounded(bar0 + 8u * (jj % S), (jj / S) & 1);
-        if (lane == 0) atomicOr(p.err, kErrTimeout);
-    }
-    __syncwarp();
-    if (lane == 0) st_release_gpu(p.flags + gw, p.epoch);
-    const long long NW = p.n_warps;
-
-    // ---- two-level merge: lead a group of helpers of a long cut (token, head) ----
-    if (ok && f_kind == 1 && p.part2_o) {
-        const int ws = (int)(((f_ps + 1) * NW - 1) / T), we = (int)(((f_ps + f_nb) * NW - 1) / T);
-        if (we - ws > kMergeGroup && (gw - ws - 1) % kMergeGroup == 0) {
-            const int last = min(gw + kMergeGroup - 1, we);
-            const bool rd = wait_flags(p.flags, p.epoch, gw + 1, last, 1, lane);
+        int what = dc.kind;
+        if (last_piece && what == 2) {
+            // this warp's own partial is stored: its flag may go up before the merge's wait
             __syncwarp();
-            if (rd) {
-                float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f}, acc[KS][O::N];
+            if (lane == 0) st_release_gpu(p.flags + gw, p.epoch);
+            if (lead_to) what = 3;
+        }
+#pragma unroll 1
+        for (;;) {
+            float M[2], L[2], acc[KS][O::N], inv[2] = {1.f, 1.f};
+            if (what != 3) {
+                join(M, L, acc);
+            } else {
+                M[0] = M[1] = -INFINITY;
+                L[0] = L[1] = 0.f;
 #pragma unroll
                 for (int m = 0; m < KS; ++m)
 #pragma unroll
                     for (int v = 0; v < O::N; ++v) acc[m][v] = 0.f;
-                q4_merge_slots<D, PACK>(p.part_o, p.part_ml, G, g, t, gw, last, 1, M, L, acc);
-                q4_store_partial<D, PACK>(p.part2_o, p.part2_ml, G, g, t, (size_t)gw, M, L, acc);
             }
-            if (!rd && lane == 0) atomicOr(p.err, kErrTimeout);
+            bool rd = true;
+            if (what >= 2) {
+                int from = gw, to = lead_to, stride = 1;
+                bool groups = false;
+                if (what == 2) {
+                    const int nb = dc.pos / kBlock + 1 - dc.skip;
+                    from = gw + 1;
+                    to = warp_of(dc.ps + nb - 1);
+                    groups = p.part2_o && to - gw > kMergeGroup;
+                    stride = groups ? kMergeGroup : 1;
+                }
+                // (a leader's own flag is up: `from` may be itself)
+                rd = wait_flags(groups ? p.flags2 : p.flags, p.epoch, from, to, stride, lane);
+                __syncwarp();
+                if (rd)
+                    q4_merge_slots<D, PACK>(groups ? p.part2_o : p.part_o, groups ? p.part2_ml : p.part_ml, G, g, t,
+                                            from, to, stride, M, L, acc);
+                else if (lane == 0)
+                    atomicOr(p.err, kErrTimeout);
+            }
+            if (what & 1) {  // 1, 3: a partial of this warp
+                float* ml = (what == 1 ? p.part_ml : p.part2_ml) + (size_t)gw * G * 2;
+                q4_store_rows<D, PACK>((what == 1 ? p.part_o : p.part2_o) + (size_t)gw * G * D, false, G, g, t, inv, acc);
+                if (g == 0 && (!PACK || t < 2)) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int h = O::head(c, t);
+                        if (h < G) {
+                            ml[h * 2] = M[c];
+                            ml[h * 2 + 1] = L[c];
+                        }
+                    }
+                }
+            } else {
+                ++items_out;
+                if (!SH && p.pre_splits > 0 && dc.skip > 0) q4_fold_prefix<D, PACK>(p, dc.tok, dc.h, g, t, M, L, acc);
+                const size_t hl = (size_t)Hkv * G;
+                const size_t row = p.n_peers == 0 ? dc.tok * hl + (size_t)dc.h * G
+                                                  : dc.tok * (size_t)p.n_peers * hl + p.peer_rank * hl + (size_t)dc.h * G;
+                uint8_t* out = static_cast<uint8_t*>(p.n_peers == 0 ? p.out : p.gather_out);
+                inv[0] = L[0] == 0.f ? 0.f : 1.f / L[0];  // 0: an interval without positions
+                inv[1] = L[1] == 0.f ? 0.f : 1.f / L[1];
+                if (rd) q4_store_rows<D, PACK>(out + row * D * (p.out_f32 ? 4 : 2), !p.out_f32, G, g, t, inv, acc);
+            }
+            if (!last_piece) break;
+            // Publish: every partial of this warp is visible before its flag.
             __syncwarp();
-            if (lane == 0) st_release_gpu(p.flags2 + gw, p.epoch);
+            if (what == 3) {
+                if (lane == 0) st_release_gpu(p.flags2 + gw, p.epoch);  // either way: no second wait
+                if (dc.kind != 2) break;
+                what = 2;
+                continue;
+            }
+            if (what == 2) break;
+            if (lane == 0) st_release_gpu(p.flags + gw, p.epoch);
+            if (!lead_to) break;
+            what = 3;
         }
+        if (last_piece) break;
+#pragma unroll
+        for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
+        mb[0] = mb[1] = -INFINITY;
+        l_run[0] = l_run[1] = 0.f;
+        ++ci;
+        take_piece();
     }
-    if (!ok || dc.kind != 2 || ct != dc.b1 - dc.b0) {
-        peer_done(p, lane, items_out);
-        return;
-    }
-
-    // ---- merge the cut (token, head) this range ends with ----
-    const int nb = dc.pos / kBlock + 1 - dc.skip;
-    const int w_last = (int)(((dc.ps + nb) * NW - 1) / T);
-    const bool grouped = p.part2_o && w_last - gw > kMergeGroup;
-    const int stride = grouped ? kMergeGroup : 1;
-    const bool ready = wait_flags(grouped ? p.flags2 : p.flags, p.epoch, gw + 1, w_last, stride, lane);
-    __syncwarp();
-    if (!ready) {
+    if (!ok) {
+        // bounded drain of the copies still in flight, then report; the flag
+        // goes up all the same, so that no other warp waits its limit out
+        for (int jj = consumed; jj < issued; ++jj) mbar_wait_bounded(bar0 + 8u * (jj % S), (jj / S) & 1);
         if (lane == 0) atomicOr(p.err, kErrTimeout);
-        peer_done(p, lane, items_out + 1);
-        return;
+        __syncwarp();
+        if (lane == 0) st_release_gpu(p.flags + gw, p.epoch);
     }
-    {
-        float M[2], L[2], acc[KS][O::N];
-        join(M, L, acc);
-        q4_merge_slots<D, PACK>(grouped ? p.part2_o : p.part_o, grouped ? p.part2_ml : p.part_ml, G, g, t, gw + 1,
-                                w_last, stride, M, L, acc);
-        q4_store_out<D, PACK>(p, dc.tok, dc.h, g, t, L, acc);
-    }
-    peer_done(p, lane, items_out + 1);
+    peer_done(p, lane, items_out);
 }
 
 // ------------------------------------------------------------- launches ----
@@ -970,6 +1156,33 @@ cudaError_t launch_attend_q4(const AttnParams& p, int head_dim, cudaStream_t s) 
 
 cudaError_t launch_attend_q4_shaped(const AttnShapedParams& p, int head_dim, cudaStream_t s) {
     return launch_q4_any<true>(p, head_dim, s);
+}
+
+cudaError_t launch_expand_q4(const uint8_t* pool_layer, const int32_t* tables, int max_blocks, const ExpandGroup* groups,
+                             int n_groups, int n_kv_heads, int head_dim, uint16_t* out, int n_blocks, int32_t* err,
+                             cudaStream_t s) {
+    for (int g0 = 0; g0 < n_groups; g0 += kExpandGroups) {
+        ExpandParams p{};
+        p.pool = pool_layer;
+        p.tables = tables;
+        p.out = out;
+        p.err = err;
+        p.max_blocks = max_blocks;
+        p.n_kv_heads = n_kv_heads;
+        p.n_blocks = n_blocks;
+        p.n_groups = std::min(kExpandGroups, n_groups - g0);
+        for (int i = 0; i < p.n_groups; ++i) {
+            p.groups[i] = groups[g0 + i];
+            p.first[i] = p.total;
+            p.total += groups[g0 + i].count;
+        }
+        const unsigned blocks = (unsigned)(((long long)p.total * n_kv_heads + 7) / 8);
+        if (head_dim == 64) expand_q4_kernel<64><<<blocks, 256, 0, s>>>(p);
+        else expand_q4_kernel<128><<<blocks, 256, 0, s>>>(p);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 cudaError_t launch_write_q4(uint8_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, const void* k,

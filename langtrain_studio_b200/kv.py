@@ -51,13 +51,24 @@ def _dptr(t) -> C.c_void_p:
     return C.c_void_p(t.data_ptr())
 
 
-def _stream(stream) -> C.c_void_p:
+_raw_stream = None
+
+
+def _stream(stream, device: int | None = None) -> C.c_void_p:
+    """The stream argument of a call: the given one, or the current stream of
+    `device` (default: the current device).  The raw-handle lookup costs 0.1 us
+    where building a torch.cuda.Stream object costs 4."""
+    global _raw_stream
     if isinstance(stream, C.c_void_p):
         return stream
     if stream is None:
         import torch
 
-        stream = torch.cuda.current_stream()
+        if _raw_stream is None:
+            torch.cuda.current_stream()  # initialises CUDA
+            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+                lambda d: torch.cuda.current_stream(d).cuda_stream)
+        stream = _raw_stream(torch.cuda.current_device() if device is None else device)
     return C.c_void_p(getattr(stream, "cuda_stream", stream))
 
 
@@ -108,6 +119,7 @@ class KvCache:
             max_batch=max_batch, max_blocks_per_seq=max_blocks_per_seq, device=device,
             kv_format=KV_FORMATS[kv_format])
         self.kv_format = kv_format
+        self._torch_device = None
         h = C.c_void_p()
         rc = self._lib.lt_kv_create(C.byref(cfg), C.byref(h))
         if rc != N.LT_OK:
@@ -171,7 +183,7 @@ class KvCache:
         blocks = np.zeros(max(n, 1), np.int32)
         slots = np.zeros(max(n, 1), np.int32)
         done = C.c_uint32()
-        st = _stream(stream) if self.device >= 0 else C.c_void_p(0)
+        st = _stream(stream, self.device) if self.device >= 0 else C.c_void_p(0)
         rc = self._lib.lt_kv_append(self._h, _ptr(seqs), _ptr(positions), n, _ptr(blocks), _ptr(slots),
                                     C.byref(done), st)
         if rc != N.LT_OK:
@@ -185,7 +197,7 @@ class KvCache:
         assert k.is_cuda and k.is_contiguous() and v.is_contiguous() and k.dtype == v.dtype
         assert k.numel() == n * self.kv_dim and v.numel() == n * self.kv_dim
         self._check(self._lib.lt_kv_write(self._h, layer, _ptr(blocks), _ptr(slots), n, _dptr(k), _dptr(v),
-                                          _dtype_code(k), _stream(stream)))
+                                          _dtype_code(k), _stream(stream, self.device)))
 
     def attend(self, layer: int, q, seqs, positions, out=None, out_dtype=None, scale: float | None = None,
                stream=None):
@@ -200,7 +212,7 @@ class KvCache:
         if scale is None:
             scale = self.default_scale
         self._check(self._lib.lt_kv_attend(self._h, layer, _dptr(q), _dtype_code(q), _ptr(seqs), _ptr(positions), n,
-                                           _dptr(out), _dtype_code(out), scale, _stream(stream)))
+                                           _dptr(out), _dtype_code(out), scale, _stream(stream, self.device)))
         return out
 
     def attend_shaped(self, layer: int, q, seqs, positions, *, softcap: float = 0.0, window: int = 0, slopes=None,
@@ -237,13 +249,22 @@ class KvCache:
                 end = a
         if out is None:
             out = torch.empty((n, self.n_heads * self.head_dim), dtype=out_dtype or torch.float32, device=q.device)
-        self._on_device("out", out, n * self.n_heads * self.head_dim)
+        else:
+            self._on_device("out", out, n * self.n_heads * self.head_dim)
         if scale is None:
             scale = self.default_scale
         self._check(self._lib.lt_kv_attend_shaped(self._h, layer, _dptr(q), _dtype_code(q), _ptr(seqs),
                                                   _ptr(positions), n, C.byref(score), _dptr(out), _dtype_code(out),
-                                                  scale, _stream(stream)))
+                                                  scale, _stream(stream, self.device)))
         return out
+
+    def _cuda(self):
+        """This cache's torch device."""
+        if self._torch_device is None:
+            import torch
+
+            self._torch_device = torch.device("cuda", self.device)
+        return self._torch_device
 
     def _on_device(self, name: str, t, numel: int):
         """Refuse a tensor that is not a contiguous array of `numel` values on the cache's device."""
@@ -266,7 +287,7 @@ class KvCache:
             scale = self.default_scale
         self._check(self._lib.lt_kv_write_attend(
             self._h, layer, _ptr(blocks), _ptr(slots), _dptr(k), _dptr(v), _dtype_code(k), _dptr(q), _dtype_code(q),
-            _ptr(seqs), _ptr(positions), n, _dptr(out), _dtype_code(out), scale, _stream(stream)))
+            _ptr(seqs), _ptr(positions), n, _dptr(out), _dtype_code(out), scale, _stream(stream, self.device)))
         return out
 
     # ------------------------------------------- head-sharded peer gather
@@ -302,7 +323,7 @@ class KvCache:
             scale = self.default_scale
         self._check(self._lib.lt_kv_attend_gather(self._h, layer, _dptr(q), _dtype_code(q), _ptr(seqs),
                                                   _ptr(positions), n, _dptr(out), _dtype_code(out), scale,
-                                                  _stream(stream)))
+                                                  _stream(stream, self.device)))
         return out
 
     def write_attend_gather(self, layer: int, blocks, slots, k, v, q, seqs, positions, out=None, out_dtype=None,
@@ -320,7 +341,7 @@ class KvCache:
             scale = self.default_scale
         self._check(self._lib.lt_kv_write_attend_gather(
             self._h, layer, _ptr(blocks), _ptr(slots), _dptr(k), _dptr(v), _dtype_code(k), _dptr(q), _dtype_code(q),
-            _ptr(seqs), _ptr(positions), n, _dptr(out), _dtype_code(out), scale, _stream(stream)))
+            _ptr(seqs), _ptr(positions), n, _dptr(out), _dtype_code(out), scale, _stream(stream, self.device)))
         return out
 
     def truncate(self, seq: int, start: int):
@@ -333,22 +354,22 @@ class KvCache:
 
     def compact(self, stream=None) -> int:
         moved = C.c_uint32()
-        st = _stream(stream) if self.device >= 0 else C.c_void_p(0)
+        st = _stream(stream, self.device) if self.device >= 0 else C.c_void_p(0)
         self._check(self._lib.lt_kv_compact(self._h, C.byref(moved), st))
         return moved.value
 
     def flush(self, stream=None):
-        st = _stream(stream) if self.device >= 0 else C.c_void_p(0)
+        st = _stream(stream, self.device) if self.device >= 0 else C.c_void_p(0)
         self._check(self._lib.lt_kv_flush(self._h, st))
 
     def check(self, stream=None):
-        st = _stream(stream) if self.device >= 0 else C.c_void_p(0)
+        st = _stream(stream, self.device) if self.device >= 0 else C.c_void_p(0)
         self._check(self._lib.lt_kv_check(self._h, st))
 
     def selftest_wait(self, limit_us: int, stream=None):
         """Make one bounded device wait run out (a flag nothing sets, limit
         `limit_us`); the next check() raises KvError(LT_E_TIMEOUT)."""
-        self._check(self._lib.lt_kv_selftest_wait(self._h, int(limit_us), _stream(stream)))
+        self._check(self._lib.lt_kv_selftest_wait(self._h, int(limit_us), _stream(stream, self.device)))
 
     def rows(self, layer: int, seq: int, n: int, stream=None):
         """K and V rows 0..n of seq (kv.rs:135-150) as f16 CUDA [n, kv_dim]."""
@@ -356,7 +377,7 @@ class KvCache:
 
         k = torch.empty((n, self.kv_dim), dtype=torch.float16, device=f"cuda:{self.device}")
         v = torch.empty_like(k)
-        self._check(self._lib.lt_kv_rows(self._h, layer, seq, n, _dptr(k), _dptr(v), _stream(stream)))
+        self._check(self._lib.lt_kv_rows(self._h, layer, seq, n, _dptr(k), _dptr(v), _stream(stream, self.device)))
         return k, v
 
     def read(self, layer: int, blocks, slots, dtype=None, k=None, v=None, stream=None):
@@ -368,16 +389,15 @@ class KvCache:
         n = blocks.size
         if slots.size != n:
             raise ValueError(f"{slots.size} slots for {n} blocks")
-        if k is None:
-            k = torch.empty((n, self.kv_dim), dtype=dtype or torch.float16, device=f"cuda:{self.device}")
-        if v is None:
-            v = torch.empty_like(k)
-        if k.dtype != v.dtype:
-            raise TypeError(f"k is {k.dtype}, v {v.dtype}")
-        self._on_device("k", k, n * self.kv_dim)
-        self._on_device("v", v, n * self.kv_dim)
+        if k is None and v is None:
+            k, v = torch.empty((2, n, self.kv_dim), dtype=dtype or torch.float16, device=self._cuda()).unbind(0)
+        elif k is None or v is None or k.dtype != v.dtype or (dtype is not None and k.dtype != dtype):
+            raise TypeError("k and v go together, of one dtype")
+        else:
+            self._on_device("k", k, n * self.kv_dim)
+            self._on_device("v", v, n * self.kv_dim)
         self._check(self._lib.lt_kv_read(self._h, layer, _ptr(blocks), _ptr(slots), n, _dptr(k), _dptr(v),
-                                         _dtype_code(k), _stream(stream)))
+                                         _dtype_code(k), _stream(stream, self.device)))
         return k, v
 
     # --------------------------------------------------------- introspection

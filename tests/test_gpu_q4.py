@@ -255,7 +255,6 @@ def test_copy_on_write_compaction_and_stale_blocks():
         for layer in range(2):
             t.rows[(layer, s)] = list(t.rows[(layer, 0)][: 150 + s])
         t.fill(s, 170 + 3 * s, rng)
-    c0 = t.kv.cascade_launches()
     t.kv.truncate(0, 0)
     t.kv.truncate(4, 0)
     assert t.kv.compact() > 0
@@ -267,7 +266,35 @@ def test_copy_on_write_compaction_and_stale_blocks():
         for s in (1, 5, 9, 11):
             t.check(layer, s)
         close(t.kv.attend(layer, torch.from_numpy(q).cuda(), seqs, pos), t.attend_ref(layer, seqs, pos, q))
-    assert t.kv.cascade_launches() == c0
+    t.kv.check()
+
+
+@pytest.mark.parametrize("hd,hq,hkv", [(128, 32, 8), (64, 8, 2), (128, 16, 2), (64, 5, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_prefix_pass(hd, hq, hkv, dtype):
+    """Prefill chunks and sequences on a shared prefix: the shared blocks go
+    through the tensor-core pass over expanded tiles.  Its scores and sums are
+    f32 with q and the weights as value + residual, like the other path's."""
+    rng = np.random.default_rng(hd + hq)
+    t = Twin(hkv, hd, 16 * 200, hq, max_seqs=14, max_batch=1024)
+    t.fill(0, 333, rng)
+    t.fill(1, 70, rng)
+    for s in range(2, 13):
+        t.kv.share(1, s, 70)
+        t.rows[(0, s)] = list(t.rows[(0, 1)][:70])
+        t.fill(s, 71 + 5 * (s % 4), rng)
+    t.fill(13, 40, rng)
+    # a chunk of sequence 0, eleven members of the shared prefix, one other
+    seqs = np.concatenate([np.zeros(150), np.arange(2, 13), [13]]).astype(np.int64)
+    pos = np.concatenate([np.arange(183, 333), [t.kv.len(s) - 1 for s in range(2, 13)], [39]]).astype(np.int64)
+    q = torch.from_numpy(rng.standard_normal((seqs.size, hq * hd)).astype(np.float32)).cuda().to(dtype)
+    ref = t.attend_ref(0, seqs, pos, q.float().cpu().numpy())
+    c0 = t.kv.cascade_launches()
+    close(t.kv.attend(0, q, seqs, pos, out_dtype=dtype), ref, dtype)
+    assert t.kv.cascade_launches() == c0 + 1
+    t.kv.set_cascade(0)
+    close(t.kv.attend(0, q, seqs, pos, out_dtype=dtype), ref, dtype)
+    assert t.kv.cascade_launches() == c0 + 1
     t.kv.check()
 
 
