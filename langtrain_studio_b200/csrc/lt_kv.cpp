@@ -679,10 +679,11 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
     // operands (Q4_0 blocks are expanded for it), and the pass does not shape scores
     const int n_items = kv->fmt == LT_KV_Q8_0 || score ? 0 : plan_cascade(kv, seq, pos, n);
     long long tiles = 0;
+    const int piece_cost = kv->fmt == LT_KV_Q4_0 ? ltkv::kQ4PieceCost : 0;
     for (uint32_t i = 0; i < n; ++i) {
         ltkv::TokenDesc& t = kv->toks_tmp[i];
         t.prefix = (int32_t)tiles;
-        tiles += pos[i] / kBlock + 1 - t.skip;
+        tiles += pos[i] / kBlock + 1 - t.skip + piece_cost;
     }
     if (tiles > 0x7FFFFFFFll / kv->cfg.n_kv_heads) return fail(kv, LT_E_ARG, "attention call too large");
     // The kernel writes every token's last table entry itself.  For the
@@ -726,6 +727,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
     p.check_ids = 0;  // this handle's bookkeeping wrote the tables
     p.n_tok = (int32_t)n;
     p.tiles_per_head = (int32_t)tiles;
+    p.piece_cost = piece_cost;
     // At least min_tiles_per_warp tiles a warp: a small step (few tokens, short
     // contexts) runs on fewer warps with fewer split merges instead of
     // paying every warp's ramp for one tile.

@@ -53,6 +53,8 @@ struct AttnParams {
     const TokenDesc* toks;       // n_tok entries in global memory, or null: use inl
     int32_t n_tok;
     int32_t tiles_per_head;      // prefix of n_tok (total blocks over the tokens)
+    int32_t piece_cost;          // LT_KV_Q4_0: tiles a (token, head) weighs in the partition beside its
+                                 // blocks; TokenDesc.prefix and tiles_per_head count them
     int32_t n_warps;             // stream-K ranges; tile total = tiles_per_head * n_kv_heads
     int32_t n_kv_heads;
     int32_t group;
@@ -178,6 +180,7 @@ cudaError_t launch_attend_shaped(const AttnShapedParams& p, int head_dim, cudaSt
 int attend_q4_warps(int device, int group, int head_dim, int q_f32, bool shaped);
 cudaError_t launch_attend_q4(const AttnParams& p, int head_dim, cudaStream_t s);
 cudaError_t launch_attend_q4_shaped(const AttnShapedParams& p, int head_dim, cudaStream_t s);
+constexpr int kQ4PieceCost = 4;  // AttnParams.piece_cost
 // Kernel launches made by launch_attend(p).
 int attend_launches(const AttnParams& p);
 

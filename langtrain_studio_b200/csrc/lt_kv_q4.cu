@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "lt_kv_device.cuh"
 #include "lt_kv_internal.h"
@@ -213,11 +214,17 @@ cudaError_t launch_read_fmt(const uint8_t* pool, const int2* cells, const int32_
 }
 
 // ----------------------------------------------------------- attention ----
-// Stream-K decode attention over 4-bit tiles.  Partition, descriptors, flags
-// and merges are those of the f16/Q8_0 kernel (lt_kv_kernels.cu): the call's
-// (token, KV head, block) tiles are cut into one contiguous range per
-// resident warp, each warp streams its 18*D-byte tiles through its own ring of
-// bulk copies, and cut (token, head)s are merged over epoch flags.
+// Stream-K decode attention over 4-bit tiles.  Descriptors, flags and merges
+// are those of the f16/Q8_0 kernel (lt_kv_kernels.cu): the call's (token, KV
+// head, block) tiles are cut into one contiguous range per resident worker
+// warp, and cut (token, head)s are merged over epoch flags.  Each (token, head)
+// weighs p.piece_cost tiles more than it has: that many tiles' time go into its
+// q rows and its output, and ranges of equal weight then end together (ragged
+// batches of short sequences).
+//
+// One producer warp per CTA feeds the workers: kQ4Lanes of its lanes cut
+// a worker's range into pieces and keep its ring of 18*D-byte bulk copies
+// full, all workers at once.  The workers only compute.
 //
 // Per tile the mathematics is turned over: S^T = K Q^T and O^T += V^T P^T, so
 // that the 4-bit tile is the A operand of mma.sync m16n8k16 (16 slots x 16
@@ -227,26 +234,41 @@ cudaError_t launch_read_fmt(const uint8_t* pool, const int2* cells, const int32_
 //      pair); each group's partial scores are scaled by the slots' scales in f32.
 //      (A masked code read as the subnormal f16 code * 2^-24 would save the f16
 //      operation, but the MMA aligns its products by their exponent fields:
-//      the scores then lose ~10 bits, 2.5e-6 of an output against 4e-7.)
+//      the scores then lose ~10 bits, 2.5e-6 of an output against 4e-7.  Codes in
+//      bytes, read as e4m3 and converted, save a seventh of the instructions, but
+//      the conversion shares the logic operations' half-rate pipe: 64 us against
+//      57 for 64 sequences of 512 to 4096.)
 //   V: the codes become (code - 8) * d in f16, exactly (one operation more).
 // q and P are split into an f16 value and its f16 residual (~22 bits).  With a
 // group of at most 4 heads (PACK) the 8 columns hold both (columns 0-3 the
 // values, 4-7 the residuals), so one MMA carries them; larger groups take two.
 // P^T in B-operand form is the transpose of the scores' fragment: movmatrix.
 //
-// A warp takes two tiles a step: their score chains (MMA, scale, max, 2^x,
-// transpose, MMA) are independent and fill one another's latencies, and the
-// barriers, the maximum's vote and the issuer's bookkeeping are paid once.
-constexpr int kQ4Warps = 4;
-constexpr int kQ4Stages = 6;
-constexpr int kQ4Step = 2;  // tiles a step
+// What bounds it: instruction issue.  An mma.sync m16n8k16 keeps its scheduler
+// from issuing anything else for 8 cycles on this chip, so a tile (D = 128)
+// costs 16 x 8 cycles of MMA (32 x 8 for larger groups) beside ~290 other
+// instructions, against ~380 cycles that its 2304 bytes take from HBM.
+//
+// Q16 (f16 q): q has no residual, so PACK's columns 4-7 repeat the values and
+// the scores come out in both halves without an exchange; larger groups take
+// half the score MMAs.
+//
+// A worker takes two tiles a step: their score chains (MMA, scale, max, 2^x,
+// transpose, MMA) are independent and fill one another's latencies.
+constexpr int kQ4Workers = 4;   // worker warps of a CTA
+constexpr int kQ4Stages = 8;    // tiles in a worker's ring
+constexpr int kQ4Step = 2;      // tiles a step
+constexpr int kQ4Pieces = 16;   // piece descriptors in its ring (> tiles ahead + 2; a power of two)
+constexpr int kQ4Threads = (kQ4Workers + 1) * 32;
+constexpr int kQ4Lanes = kQ4Workers > 8 ? 2 : 4;  // producer lanes of a worker
 
-// D = A * B (f16, f32 accumulators from zero), D += A * B.
+// D = A * B (f16 operands, f32 accumulators from zero).
 __device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
+// D += A * B.
 __device__ __forceinline__ void mma16816_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -281,29 +303,47 @@ __device__ __forceinline__ __half2 q4_high(uint32_t w, const Q4Magic& m) {
 }
 
 // A piece: tiles [b0, b1) (counted from block skip) of (token, head).
-// kind: 0 whole (token, head) -> output; 1 it started before this warp's range
-// -> partial slot; 2 it starts here and runs past the range -> merged here.
+// kind: 0 whole (token, head) -> output; 1 it started before this worker's
+// range -> partial slot; 2 it starts here and runs past the range -> merged here.
 struct Q4Piece {
-    int tok, h, seq, pos, b0, b1, kind, last_block, skip;
+    int tok, h, pos, b0, b1, kind, last_block, skip;
     int lo, qpos;
-    int ps;  // first tile of the (token, head)
+    int first;  // first tile of the (token, head), in the partition's units
+    int last;   // last piece of the range
 };
-constexpr int kQ4Pieces = 4;  // pieces a warp has in hand: consumed, issued, the next one (a power of two)
+
+// What a worker and its producer lanes share.
+struct Q4Ring {
+    unsigned long long full[kQ4Stages];
+    uint32_t consumed, q_taken;  // by the worker: tiles done, pieces whose q rows it has read
+    uint32_t issued;             // by the producer
+    uint32_t none, stop, stopped;  // range without tiles; the worker gave up; the producer has seen it
+    Q4Piece pieces[kQ4Pieces];
+};
+
+__device__ __forceinline__ uint32_t ld_acquire_cta(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_release_cta(uint32_t* p, uint32_t v) {
+    asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
+}
 
 __host__ __device__ inline int q4_qbuf_bytes(int group, int head_dim, int q_f32) {
     return (group * head_dim * (q_f32 ? 4 : 2) + 127) & ~127;
 }
-// Two q buffers, so that the issuer runs a piece ahead from the start; one
-// where two would cost the third resident CTA.
+// q buffers of a worker: 4 KiB worth, at most 4.
 __host__ __device__ inline int q4_qbufs(int group, int head_dim, int q_f32) {
-    return q4_qbuf_bytes(group, head_dim, q_f32) > 2048 ? 1 : 2;
+    const int n = 4096 / q4_qbuf_bytes(group, head_dim, q_f32);
+    return n < 1 ? 1 : n > 4 ? 4 : n;
 }
-__host__ __device__ inline int q4_warp_smem(int group, int head_dim, int q_f32) {
+__host__ __device__ inline int q4_worker_smem(int group, int head_dim, int q_f32) {
     return kQ4Stages * q4_tile_bytes(head_dim) +
            q4_qbufs(group, head_dim, q_f32) * q4_qbuf_bytes(group, head_dim, q_f32);
 }
 __host__ __device__ inline int q4_smem(int group, int head_dim, int q_f32) {
-    return kQ4Warps * (q4_warp_smem(group, head_dim, q_f32) + kQ4Pieces * (int)sizeof(Q4Piece) + kQ4Stages * 8);
+    return kQ4Workers * (q4_worker_smem(group, head_dim, q_f32) + (int)sizeof(Q4Ring));
 }
 
 // -------------------------------------------------------------- expand ----
@@ -462,23 +502,185 @@ template <int D, bool PACK>
 __device__ __forceinline__ void q4_store_rows(void* dst, bool f16, int G, int g, int t, const float (&inv)[2],
                                               const float (&acc)[D / 16][Own<PACK>::N]) {
     using O = Own<PACK>;
+    if (f16) {
 #pragma unroll
-    for (int v = 0; v < O::N; ++v) {
-        const int h = O::head(v, t);
-        if (h >= G) continue;
-        const int at = h * D + g + 8 * O::row(v, t);
-        const float s = inv[O::col(v)];
+        for (int v = 0; v < O::N; ++v) {
+            const int h = O::head(v, t);
+            if (h >= G) continue;
+            __half* at = static_cast<__half*>(dst) + h * D + g + 8 * O::row(v, t);
 #pragma unroll
-        for (int m = 0; m < D / 16; ++m) {
-            const float x = acc[m][v] * s;
-            if (f16) static_cast<__half*>(dst)[at + 16 * m] = __float2half_rn(x);
-            else static_cast<float*>(dst)[at + 16 * m] = x;
+            for (int m = 0; m < D / 16; ++m) at[16 * m] = __float2half_rn(acc[m][v] * inv[O::col(v)]);
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < O::N; ++v) {
+            const int h = O::head(v, t);
+            if (h >= G) continue;
+            float* at = static_cast<float*>(dst) + h * D + g + 8 * O::row(v, t);
+#pragma unroll
+            for (int m = 0; m < D / 16; ++m) at[16 * m] = acc[m][v] * inv[O::col(v)];
         }
     }
 }
 
-template <int D, bool PACK, bool SH>
-__global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_constant__ AttnParamsOf<SH> p) {
+// The producer warp: kQ4Lanes lanes feed each worker.
+template <int D, bool SH>
+__device__ __forceinline__ void q4_produce(const AttnParamsOf<SH>& p, uint8_t* stages0, Q4Ring* rings, int lane) {
+    constexpr int TILE = q4_tile_bytes(D), S = kQ4Stages;
+    const int G = p.group, Hkv = p.n_kv_heads, C = p.piece_cost;
+    const int WSM = q4_worker_smem(G, D, p.q_f32), QBUF = q4_qbuf_bytes(G, D, p.q_f32), nqb = q4_qbufs(G, D, p.q_f32);
+    const uint32_t qbytes = (uint32_t)(G * D * (p.q_f32 ? 4 : 2));
+    constexpr int LN = kQ4Lanes;
+    const int c = min(lane / LN, kQ4Workers - 1), u = lane % LN;
+    const int gw = blockIdx.x * kQ4Workers + c;
+    Q4Ring* ring = rings + c;
+    const uint32_t stages = smem_u32(stages0) + c * WSM, qbufs = stages + S * TILE, bar0 = smem_u32(ring->full);
+    const TokenDesc* toks = p.toks ? p.toks : p.inl;
+    const uint8_t* pool = reinterpret_cast<const uint8_t*>(p.pool_layer);
+    const uint32_t T = (uint32_t)p.tiles_per_head * Hkv, NW = (uint32_t)p.n_warps, quo = T / NW, rem = T % NW;
+    bool live = lane / LN < kQ4Workers && gw < p.n_warps;
+
+    // The generator's place: (token, head, offset); offsets below C are the (token, head)'s cost.
+    int gi = 0, gh = 0, go = 0, gt = 0, t1 = 0;
+    if (live) {
+        // Range [T * gw / n, T * (gw + 1) / n) of T < 2^31, in 32 bits: with
+        // T = quo * n + rem, floor(T * w / n) = quo * w + floor(rem * w / n).
+        gt = (int)(quo * gw + rem * gw / NW);
+        t1 = (int)(quo * (gw + 1) + rem * (gw + 1) / NW);
+        int lo = 0, hi = p.n_tok - 1;  // last token whose first tile is <= gt
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (toks[mid].prefix * Hkv <= gt) lo = mid; else hi = mid - 1;
+        }
+        gi = lo;
+        const uint32_t nv = (uint32_t)(toks[gi].pos / kBlock + 1 - toks[gi].skip + C), off = (uint32_t)(gt - toks[gi].prefix * Hkv);
+        gh = (int)(off / nv);
+        go = (int)(off % nv);
+    }
+    int stage = 0, qslot = nqb - 1;  // of the next tile, of the piece being issued
+    int pi = -1, it = 0, len = 0, head = 0, tok = 0, b_last = -1;  // the piece being issued
+    const int32_t* trow = p.tables;
+    int id = 0;  // block of tile it + u
+    uint32_t issued = 0;
+    bool first = true;
+    uint32_t idle = 0;  // passes without progress, and when the first of them was
+    uint64_t t_idle = 0;
+    auto load_id = [&]() {
+        if (it + u < len)
+            id = it + u == len - 1 && b_last >= 0 ? b_last
+                                                  : checked_block(__ldg(trow + it + u), p.n_blocks, p.err, p.check_ids != 0);
+    };
+    for (;;) {
+        bool moved = false;
+        // One reading for a worker's lanes, which must decide alike.
+        const uint32_t done = __shfl_sync(kFull, ld_acquire_cta(&ring->consumed), lane & ~(LN - 1));
+        const uint32_t taken = __shfl_sync(kFull, ld_acquire_cta(&ring->q_taken), lane & ~(LN - 1));
+        const uint32_t stop = __shfl_sync(kFull, ld_acquire_cta(&ring->stop), lane & ~(LN - 1));
+        if (live) {
+            if (stop) {
+                if (u == 0) st_release_cta(&ring->stopped, 1);
+                live = false;
+            } else if (it < len) {
+                const int room = S - (int)(issued - done);
+                int n = min(min(LN, room), len - it);
+                if (it == 0 && pi - (int)taken >= nqb) n = 0;  // no q buffer free
+                if (n > 0) {
+                    if (u < n) {
+                        const int st = stage + u >= S ? stage + u - S : stage + u;
+                        const bool with_q = it + u == 0;
+                        mbar_arrive_expect_tx(bar0 + 8u * st, TILE + (with_q ? qbytes : 0u));
+                        bulk_g2s(stages + st * TILE, pool + ((size_t)id * Hkv + head) * TILE, TILE, bar0 + 8u * st);
+                        if (with_q)
+                            bulk_g2s(qbufs + qslot * QBUF,
+                                     static_cast<const uint8_t*>(p.q) + ((size_t)tok * Hkv + head) * qbytes, qbytes,
+                                     bar0 + 8u * st);
+                    }
+                    issued += n;
+                    it += n;
+                    stage = stage + n >= S ? stage + n - S : stage + n;
+                    if (u == 0) st_release_cta(&ring->issued, issued);
+                    load_id();
+                    moved = true;
+                }
+            } else {
+                // ---- next piece ----
+                const TokenDesc td = toks[min(gi, p.n_tok - 1)];
+                const int nb = td.pos / kBlock + 1 - td.skip, nv = nb + C;
+                if (go < C) {
+                    gt += C - go;
+                    go = C;
+                }
+                if (gt >= t1) {  // the range ends here
+                    live = false;
+                    if (first && u == 0) {  // ... and has no tile: wake the worker
+                        st_release_cta(&ring->none, 1);
+                        mbar_arrive(bar0);
+                    }
+                } else {
+                    first = false;
+                    ++pi;
+                    qslot = qslot + 1 == nqb ? 0 : qslot + 1;
+                    len = min(nv - go, t1 - gt);
+                    it = 0;
+                    head = gh;
+                    tok = gi;
+                    const int b0 = go - C;
+                    b_last = b0 + len == nb ? td.last_block : -1;
+                    trow = p.tables + (size_t)td.seq * p.max_blocks + td.skip + b0;
+                    load_id();
+                    if (u == 0) {
+                        Q4Piece r;
+                        r.tok = gi;
+                        r.h = gh;
+                        r.pos = td.pos;
+                        r.b0 = b0;
+                        r.b1 = b0 + len;
+                        r.kind = b0 > 0 ? 1 : b0 + len < nb ? 2 : 0;
+                        r.last_block = b_last;
+                        r.skip = td.skip;
+                        r.first = td.prefix * Hkv + gh * nv + C;
+                        r.lo = r.qpos = 0;
+                        if constexpr (SH) {
+                            const ShapeDesc sd = p.shapes ? p.shapes[gi] : p.inl_shapes[gi];
+                            r.lo = sd.lo;
+                            r.qpos = sd.qpos;
+                        }
+                        // the next piece, if any, starts after the next (token, head)'s cost
+                        r.last = gt + len + (go + len == nv ? C : 0) >= t1;
+                        ring->pieces[pi % kQ4Pieces] = r;
+                        // the token's last block entry, written once per token (head 0)
+                        if (gh == 0 && b_last >= 0) p.tables[(size_t)td.seq * p.max_blocks + td.skip + b0 + len - 1] = b_last;
+                    }
+                    gt += len;
+                    go += len;
+                    if (go == nv) {
+                        go = 0;
+                        if (++gh == Hkv) {
+                            gh = 0;
+                            ++gi;
+                        }
+                    }
+                    moved = true;
+                }
+            }
+        }
+        if (!__any_sync(kFull, live)) break;
+        if (__any_sync(kFull, moved)) {
+            idle = 0;
+        } else {
+            if (idle == 0) t_idle = global_ns();
+            __nanosleep(20);
+            // (the workers' own waits are shorter)
+            if ((++idle & 255u) == 0 && __any_sync(kFull, global_ns() - t_idle > 2 * kWaitLimitNs)) {
+                if (lane == 0) atomicOr(p.err, kErrTimeout);
+                break;
+            }
+        }
+    }
+}
+
+template <int D, bool PACK, bool SH, bool Q16>
+__global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_constant__ AttnParamsOf<SH> p) {
     constexpr int TILE = q4_tile_bytes(D);
     constexpr int KS = D / 16;   // 16-dim steps of K, and 16-dim row tiles of V
     constexpr int G32 = D / 32;  // scale groups
@@ -488,186 +690,50 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int gw = blockIdx.x * kQ4Warps + warp;
     const int Hkv = p.n_kv_heads, G = p.group;
-    const int QBUF = q4_qbuf_bytes(G, D, p.q_f32), nqb = q4_qbufs(G, D, p.q_f32);
-    const int WSM = q4_warp_smem(G, D, p.q_f32);
-    uint8_t* stages = smem + (size_t)warp * WSM;
-    uint8_t* qbufs = stages + S * TILE;
-    Q4Piece* pieces = reinterpret_cast<Q4Piece*>(smem + (size_t)kQ4Warps * WSM) + warp * kQ4Pieces;
-    const uint32_t bar0 =
-        smem_u32(smem + (size_t)kQ4Warps * (WSM + kQ4Pieces * sizeof(Q4Piece))) + 8u * S * warp;
-    if (lane < S) mbar_init(bar0 + 8u * lane, 1);
-    fence_mbar_init();
-    __syncwarp();
+    const int WSM = q4_worker_smem(G, D, p.q_f32);
+    Q4Ring* rings = reinterpret_cast<Q4Ring*>(smem + (size_t)kQ4Workers * WSM);
+    if (warp < kQ4Workers) {
+        Q4Ring* r = rings + warp;
+        if (lane < S) mbar_init(smem_u32(r->full) + 8u * lane, 1);
+        if (lane == S) r->consumed = r->q_taken = r->issued = r->none = r->stop = r->stopped = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    if (warp == kQ4Workers) {
+        q4_produce<D, SH>(p, smem, rings, lane);
+        return;
+    }
+    const int gw = blockIdx.x * kQ4Workers + warp;
     if (gw >= p.n_warps) return;
 
-    const TokenDesc* toks = p.toks ? p.toks : p.inl;
-    const uint8_t* pool = reinterpret_cast<const uint8_t*>(p.pool_layer);
-    // Range [T * gw / n, T * (gw + 1) / n) of the T < 2^31 tiles, in 32 bits:
-    // with T = quo * n + rem, floor(T * w / n) = quo * w + floor(rem * w / n).
+    Q4Ring* ring = rings + warp;
+    uint8_t* stages = smem + (size_t)warp * WSM;
+    uint8_t* qbufs = stages + S * TILE;
+    const int QBUF = q4_qbuf_bytes(G, D, p.q_f32), nqb = q4_qbufs(G, D, p.q_f32);
+    const uint32_t bar0 = smem_u32(ring->full);
     const uint32_t T = (uint32_t)p.tiles_per_head * Hkv;
-    const uint32_t NWu = (uint32_t)p.n_warps, quo = T / NWu, rem = T % NWu;
-    const int t0 = (int)(quo * gw + rem * gw / NWu), t1 = (int)(quo * (gw + 1) + rem * (gw + 1) / NWu);
     const int g = lane >> 2, t = lane & 3;
-    const int qelem = p.q_f32 ? 4 : 2;
-    const uint32_t qbytes = (uint32_t)(G * D * qelem);
-
-    // ---- piece generator over [t0, t1): piece i goes to slot i % kQ4Pieces ----
-    int gi, gh, gb, gt = t0, gn = 0;
-    {
-        int lo = 0, hi = p.n_tok - 1;  // last token whose first tile is <= t0
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (toks[mid].prefix * Hkv <= t0) lo = mid; else hi = mid - 1;
-        }
-        gi = lo;
-        const TokenDesc td = toks[gi];
-        const uint32_t nb = (uint32_t)(td.pos / kBlock + 1 - td.skip), off = (uint32_t)(t0 - td.prefix * Hkv);
-        gh = (int)(off / nb);
-        gb = (int)(off % nb);
-    }
-    auto gen_piece = [&]() {
-        const TokenDesc td = toks[gi];
-        const int nb = td.pos / kBlock + 1 - td.skip;
-        const int len = min(nb - gb, t1 - gt);
-        if (lane == 0) {
-            Q4Piece r;
-            r.tok = gi;
-            r.skip = td.skip;
-            r.h = gh;
-            r.seq = td.seq;
-            r.pos = td.pos;
-            r.b0 = gb;
-            r.b1 = gb + len;
-            r.ps = td.prefix * Hkv + gh * nb;
-            r.kind = r.ps < t0 ? 1 : (r.ps + nb > t1 ? 2 : 0);
-            r.last_block = r.b1 == nb ? td.last_block : -1;
-            r.lo = r.qpos = 0;
-            if constexpr (SH) {
-                const ShapeDesc sd = p.shapes ? p.shapes[gi] : p.inl_shapes[gi];
-                r.lo = sd.lo;
-                r.qpos = sd.qpos;
-            }
-            pieces[gn & (kQ4Pieces - 1)] = r;
-        }
-        ++gn;
-        gt += len;
-        gb += len;
-        if (gb == nb) {
-            gb = 0;
-            if (++gh == Hkv) {
-                gh = 0;
-                ++gi;
-            }
-        }
-        __syncwarp();
-    };
-    // block ids [b, min(b + 32, b1)) of a piece, lane j holding b + j
-    auto load_window = [&](const Q4Piece& r, int b) {
-        const int bb = b + lane;
-        if (bb >= r.b1) return 0;
-        if (bb == r.b1 - 1 && r.last_block >= 0) return r.last_block;
-        return checked_block(__ldg(p.tables + (size_t)r.seq * p.max_blocks + r.skip + bb), p.n_blocks, p.err,
-                             p.check_ids != 0);
-    };
-
-    // ---- issuer: piece ii, its tiles [it, d_len) not yet issued ----
-    gen_piece();
-    const bool f_cut = pieces[0].kind == 1;  // the range's first piece continues a cut (token, head)
-    const int f_tok = pieces[0].tok;
-    bool dn_valid = true;  // piece ii + 1 is generated
-    int ii = -1, it = 0, wb = 0, d_len = 0, d_h = 0;
-    int win = 0, win_n = 0;  // block ids [wb, wb + 32) of piece ii, and the 32 that follow (of ii or ii + 1)
-    auto prefetch_window = [&]() {
-        const bool same = wb + 32 < d_len;
-        if (!same && !dn_valid) return;
-        const Q4Piece& d = pieces[(same ? ii : ii + 1) & (kQ4Pieces - 1)];
-        win_n = load_window(d, same ? d.b0 + wb + 32 : d.b0);
-    };
-    prefetch_window();
-    int issued = 0, consumed = 0, istage = 0, cstage = 0, cphase = 0;
-    int ci = 0, ct = 0;  // the consumer's piece, and its tiles consumed
-    // Fill the ring: lane u issues the u-th of the next n tiles.  The issuer
-    // runs at most one piece ahead of the consumer, and with a single q buffer
-    // only once the consumer has taken its own piece's q rows (ct > 0).
-    auto try_issue = [&]() {
-        for (;;) {
-            const int room = S - (issued - consumed);
-            if (it < d_len) {
-                if (room == 0) break;
-                if (it - wb == 32) {
-                    win = win_n;
-                    wb += 32;
-                    prefetch_window();
-                }
-                const int n = min(min(d_len - it, room), 32 - (it - wb));
-                const int b = __shfl_sync(kFull, win, (it - wb + lane) & 31);
-                if (lane < n) {
-                    int st = istage + lane;
-                    st = st >= S ? st - S : st;
-                    const uint32_t bar = bar0 + 8u * st;
-                    const bool with_q = it + lane == 0;
-                    mbar_arrive_expect_tx(bar, TILE + (with_q ? qbytes : 0u));
-                    bulk_g2s(smem_u32(stages) + st * TILE, pool + ((size_t)b * Hkv + d_h) * TILE, TILE, bar);
-                    if (with_q)
-                        bulk_g2s(smem_u32(qbufs) + (nqb == 2 ? (ii & 1) * QBUF : 0),
-                                 static_cast<const uint8_t*>(p.q) +
-                                     ((size_t)pieces[ii & (kQ4Pieces - 1)].tok * Hkv + d_h) * G * D * qelem,
-                                 qbytes, bar);
-                }
-                it += n;
-                issued += n;
-                istage += n;
-                istage = istage >= S ? istage - S : istage;
-                continue;
-            }
-            if (!dn_valid || ii > ci || (nqb == 1 && ii == ci && ct == 0)) break;
-            // on to the next piece
-            ++ii;
-            const Q4Piece& d = pieces[ii & (kQ4Pieces - 1)];
-            d_len = d.b1 - d.b0;
-            d_h = d.h;
-            dn_valid = gt < t1;
-            if (dn_valid) gen_piece();
-            it = 0;
-            wb = 0;
-            win = win_n;
-            prefetch_window();
-            // the token's last block entry, written once per token (head 0)
-            if (d.h == 0 && d.last_block >= 0 && lane == 0)
-                p.tables[(size_t)d.seq * p.max_blocks + d.skip + d.b1 - 1] = d.last_block;
-        }
-    };
-
-    // ---- consumer: c_* count from the piece's first position ----
-    int c_len, c_end, c_lo, c_q;
-    auto take_piece = [&]() {
-        const Q4Piece& c = pieces[ci & (kQ4Pieces - 1)];
-        const int base = (c.skip + c.b0) * kBlock;
-        c_len = c.b1 - c.b0;
-        c_end = c.pos + 1 - base;
-        c_lo = c.lo - base;
-        c_q = c.qpos - base;
-        ct = 0;
-    };
-    take_piece();
+    int ci = 0, ct = 0;  // the piece in hand, and its tiles consumed
+    int consumed = 0, cstage = 0, cphase = 0;
+    int qslot = 0;  // q buffer of the next piece
+    int c_len = 0, c_end = 0, c_lo = 0, c_q = 0;  // its length; its end, first position and own position from its start
     // an opaque zero keeps the exponent patterns in registers (see Q4Magic)
     const uint32_t zero = (uint32_t)p.n_warps >> 31;
     const Q4Magic magic{0x64006400u + zero, 0x54005400u + zero};
 
-    uint32_t qh[KS][2], ql[PACK ? 1 : KS][2];  // B fragments: values (PACK: residuals in columns 4-7), residuals
+    // B fragments: values (PACK: residuals in columns 4-7), residuals
+    uint32_t qh[KS][2], ql[PACK || Q16 ? 1 : KS][2];
     float cmul[2] = {0.f, 0.f};                // from the MMA's units to q.k (SH) or log2 units
     float slope[2] = {0.f, 0.f};
     float o[KS][4];
-#pragma unroll
-    for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
     // Weights are 2^(score - mb): mb trails the running maximum by 7, and moves
     // only when a score passes it by 15, so they stay within (0, 2^15] (an f16
     // and its residual keep 22 bits of all but the smallest) and o is rescaled rarely.
-    float mb[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    float mb[2], l_run[2];
     bool ok = true;
     int items_out = 0;
+    int lead_to = 0;  // last worker of the group of partials this one combines, 0: none
 
     // Join lanes and columns of the running piece: M, L of columns 0 and 1, acc.
     auto join = [&](float (&M)[2], float (&L)[2], float (&acc)[KS][O::N]) {
@@ -702,45 +768,37 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
     // ---- q rows of a piece -> B fragments ----
     auto load_q = [&](const uint8_t* qbuf) {
         const int qg = PACK ? g & 3 : g;
-        float x[KS][4];
-        float mx = 0.f;
+        const int at = min(qg, G - 1) * D + 2 * t;
+        float2 x[2 * KS];  // q values 16 ks + 8 hf + 2t, + 1 at 2 ks + hf
+        if constexpr (!Q16) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
+            for (int i = 0; i < 2 * KS; ++i) x[i] = *reinterpret_cast<const float2*>(qbuf + (at + 8 * i) * 4);
+        } else {
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                float2 f = make_float2(0.f, 0.f);
-                if (qg < G) {
-                    const int e = qg * D + ks * 16 + hf * 8 + 2 * t;
-                    if (p.q_f32) f = *reinterpret_cast<const float2*>(qbuf + e * 4);
-                    else f = __half22float2(*reinterpret_cast<const __half2*>(qbuf + e * 2));
-                }
-                x[ks][2 * hf] = f.x;
-                x[ks][2 * hf + 1] = f.y;
-                mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
+            for (int i = 0; i < 2 * KS; ++i)
+                x[i] = __half22float2(*reinterpret_cast<const __half2*>(qbuf + (at + 8 * i) * 2));
         }
         // Scale each row by a power of two that brings its largest value near
-        // 2^12: value and residual are then normal f16s.
+        // 2^12: value and residual are then normal f16s.  Rows past the group
+        // repeat its last one; nothing stores their results.
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) mx = fmaxf(mx, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
         mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
         const int ex = (int)(__float_as_uint(mx) >> 23);  // 255: Inf, which no scale helps
         const int fe = ex == 255 ? 127 : min(253, max(1, 266 - ex));
         const float f = __uint_as_float((uint32_t)fe << 23), finv = __uint_as_float((uint32_t)(254 - fe) << 23);
-        const bool resid = PACK && g >= 4;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const float y0 = x[ks][2 * hf] * f, y1 = x[ks][2 * hf + 1] * f;
-                const __half2 hi = __floats2half2_rn(y0, y1);
+        for (int i = 0; i < 2 * KS; ++i) {
+            const float y0 = x[i].x * f, y1 = x[i].y * f;
+            const __half2 hi = __floats2half2_rn(y0, y1);
+            qh[i >> 1][i & 1] = h2_bits(hi);
+            if constexpr (!Q16) {
                 const float2 back = __half22float2(hi);
-                const __half2 lo = __floats2half2_rn(y0 - back.x, y1 - back.y);
-                if constexpr (PACK) {
-                    qh[ks][hf] = h2_bits(resid ? lo : hi);
-                } else {
-                    qh[ks][hf] = h2_bits(hi);
-                    ql[ks][hf] = h2_bits(lo);
-                }
+                const uint32_t lo = h2_bits(__floats2half2_rn(y0 - back.x, y1 - back.y));
+                if constexpr (!PACK) ql[i >> 1][i & 1] = lo;
+                else if (g >= 4) qh[i >> 1][i & 1] = lo;
             }
         }
 #pragma unroll
@@ -749,7 +807,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
             if constexpr (SH) {
                 const int hh = O::head(c, t);
                 slope[c] = p.shape.slopes && hh < G
-                               ? __ldg(p.shape.slopes + pieces[ci & (kQ4Pieces - 1)].h * G + hh) * kLog2e
+                               ? __ldg(p.shape.slopes + ring->pieces[ci % kQ4Pieces].h * G + hh) * kLog2e
                                : 0.f;
             } else {
                 cmul[c] *= p.scale_log2;
@@ -761,7 +819,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
     // pool cell and into the staged tile.
     auto append = [&](uint8_t* tile) {
         constexpr int L = D / 4;  // lanes of one row
-        const Q4Piece dc = pieces[ci & (kQ4Pieces - 1)];
+        const Q4Piece dc = ring->pieces[ci % kQ4Pieces];
         const int slot = dc.pos % kBlock;
         uint8_t* cell_tile = reinterpret_cast<uint8_t*>(p.pool_layer_w) + ((size_t)dc.last_block * Hkv + dc.h) * TILE;
 #pragma unroll 1
@@ -819,7 +877,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
                                                h2_bits(q4_high(w8, magic))};
                         if (q2 == 0) mma16816_zero(tt, a, qh[ks][0], qh[ks][1]);
                         else mma16816_add(tt, a, qh[ks][0], qh[ks][1]);
-                        if constexpr (!PACK) mma16816_add(tt, a, ql[ks][0], ql[ks][1]);
+                        if constexpr (!PACK && !Q16) mma16816_add(tt, a, ql[ks][0], ql[ks][1]);
                     }
                     const float d0 = cc ? dg.y : dg.x, d1 = cc ? dg8.y : dg8.x;
                     const bool first = ch == 0 && cc == 0;
@@ -833,7 +891,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
         const int j0 = ct * kBlock;  // first position of the step in the piece
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            if constexpr (PACK) {
+            if constexpr (PACK && !Q16) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[u][e] += __shfl_xor_sync(kFull, sc[u][e], 2);
             }
@@ -938,24 +996,46 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
         }
     };
 
-    // The warp that holds tile x: the last w with floor(T * w / n) <= x.
+    // The worker that holds tile x: the last w with floor(T * w / n) <= x.
     auto warp_of = [&](int x) { return (int)(((long long)(x + 1) * p.n_warps - 1) / (long long)T); };
+    // Lane u < nt waits for the u-th of the next tiles; true for all lanes or none.
+    auto wait_tiles = [&](int nt) {
+        const int st = cstage + lane;
+        const bool wrap = st >= S;
+        const bool here = lane >= nt || mbar_wait_bounded(bar0 + 8u * (wrap ? st - S : st), (uint32_t)(cphase ^ wrap));
+        const bool all = __all_sync(kFull, here);
+        __syncwarp();  // the waiting lanes' view of the copied bytes reaches the others
+        return all;
+    };
     for (;;) {
-        try_issue();
-        const int nt = min(c_len - ct, NT);
-        {
-            // lane u waits for the u-th tile of the step
-            const int st = cstage + lane;
-            const bool wrap = st >= S;
-            const bool here = lane >= nt || mbar_wait_bounded(bar0 + 8u * (wrap ? st - S : st), (uint32_t)(cphase ^ wrap));
-            if (!__all_sync(kFull, here)) {
+        if (ct == c_len) {  // the next piece: its descriptor came before its first tile
+            if (!wait_tiles(1)) {
                 ok = false;
                 break;
             }
-            __syncwarp();  // the waiting lanes' view of the copied bytes reaches the others
+            if (ld_acquire_cta(&ring->none)) return;
+            const Q4Piece& c = ring->pieces[ci % kQ4Pieces];
+            const int base = (c.skip + c.b0) * kBlock;
+            c_len = c.b1 - c.b0;
+            c_end = c.pos + 1 - base;
+            c_lo = c.lo - base;
+            c_q = c.qpos - base;
+            ct = 0;
+            load_q(qbufs + qslot * QBUF);
+            qslot = qslot + 1 == nqb ? 0 : qslot + 1;
+            __syncwarp();
+            if (lane == 0) st_release_cta(&ring->q_taken, (uint32_t)ci + 1);
+#pragma unroll
+            for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
+            mb[0] = mb[1] = -INFINITY;
+            l_run[0] = l_run[1] = 0.f;
         }
-        if (ct == 0) load_q(qbufs + (nqb == 2 ? (ci & 1) * QBUF : 0));
-        const bool fill = !SH && p.k_new && ct + nt == c_len && pieces[ci & (kQ4Pieces - 1)].last_block >= 0;
+        const int nt = min(c_len - ct, NT);
+        if (!wait_tiles(nt)) {
+            ok = false;
+            break;
+        }
+        const bool fill = !SH && p.k_new && ct + nt == c_len && ring->pieces[ci % kQ4Pieces].last_block >= 0;
         if (fill) {
             const int st = cstage + nt - 1;
             append(stages + (size_t)(st >= S ? st - S : st) * TILE);
@@ -970,22 +1050,20 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
         ct += nt;
         if (fill) fence_proxy_async_smem();
         __syncwarp();
+        if (lane == 0) st_release_cta(&ring->consumed, (uint32_t)consumed);
         if (ct < c_len) continue;
 
         // ---- piece done ----
         // what: 0 store the output, 1 the warp's partial, 2 merge the following
         // warps' partials and store the output, 3 lead: combine the partials of
         // this warp and its next neighbours into a group partial.
-        const Q4Piece dc = pieces[ci & (kQ4Pieces - 1)];
-        const bool last_piece = ii == ci && !dn_valid;
-        int lead_to = 0;  // last warp of the group this one leads, 0: none
-        if (last_piece && f_cut && p.part2_o) {
-            // Helpers of a cut (token, head) are the warps after the one with
+        const Q4Piece dc = ring->pieces[ci % kQ4Pieces];
+        const bool last_piece = dc.last != 0;
+        if (dc.kind == 1 && p.part2_o) {  // the range's first piece
+            // Helpers of a cut (token, head) are the workers after the one with
             // its first tile; with more than kMergeGroup of them, every
-            // kMergeGroup-th leads, so that the merging warp reads one partial a group.
-            const TokenDesc td = toks[f_tok];
-            const int nb = td.pos / kBlock + 1 - td.skip, first = td.prefix * Hkv;
-            const int ps = first + (t0 - first) / nb * nb, ws = warp_of(ps), we = warp_of(ps + nb - 1);
+            // kMergeGroup-th leads, so that the merging one reads one partial a group.
+            const int ws = warp_of(dc.first), we = warp_of(dc.first + dc.pos / kBlock - dc.skip);
             if (we - ws > kMergeGroup && (gw - ws - 1) % kMergeGroup == 0) lead_to = min(gw + kMergeGroup - 1, we);
         }
         int what = dc.kind;
@@ -1013,9 +1091,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
                 int from = gw, to = lead_to, stride = 1;
                 bool groups = false;
                 if (what == 2) {
-                    const int nb = dc.pos / kBlock + 1 - dc.skip;
                     from = gw + 1;
-                    to = warp_of(dc.ps + nb - 1);
+                    to = warp_of(dc.first + dc.pos / kBlock - dc.skip);
                     groups = p.part2_o && to - gw > kMergeGroup;
                     stride = groups ? kMergeGroup : 1;
                 }
@@ -1067,87 +1144,100 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 3) attn_q4_kernel(const __grid_
             what = 3;
         }
         if (last_piece) break;
-#pragma unroll
-        for (int m = 0; m < KS; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
-        mb[0] = mb[1] = -INFINITY;
-        l_run[0] = l_run[1] = 0.f;
         ++ci;
-        take_piece();
     }
     if (!ok) {
-        // bounded drain of the copies still in flight, then report; the flag
-        // goes up all the same, so that no other warp waits its limit out
-        for (int jj = consumed; jj < issued; ++jj) mbar_wait_bounded(bar0 + 8u * (jj % S), (jj / S) & 1);
-        if (lane == 0) atomicOr(p.err, kErrTimeout);
+        // Stop the producer lanes (bounded), drain the copies in flight
+        // (bounded), report; the flag goes up all the same, so that no other
+        // worker waits its limit out.
+        if (lane == 0) {
+            atomicOr(p.err, kErrTimeout);
+            st_release_cta(&ring->stop, 1);
+            const uint64_t t_stop = global_ns();
+            while (!ld_acquire_cta(&ring->stopped) && global_ns() - t_stop < kWaitLimitNs / 4) __nanosleep(100);
+            const int issued = (int)ld_acquire_cta(&ring->issued);
+            for (int jj = consumed; jj < issued; ++jj) mbar_wait_bounded(bar0 + 8u * (jj % S), (jj / S) & 1);
+            st_release_gpu(p.flags + gw, p.epoch);
+        }
         __syncwarp();
-        if (lane == 0) st_release_gpu(p.flags + gw, p.epoch);
     }
     peer_done(p, lane, items_out);
 }
 
 // ------------------------------------------------------------- launches ----
-template <int D, bool PACK, bool SH>
+template <int D, bool PACK, bool SH, bool Q16>
 cudaError_t ensure_q4_attr(int dev) {
     static bool set[64] = {};
     if (set[dev]) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(attn_q4_kernel<D, PACK, SH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               q4_smem(PACK ? 4 : kMaxGroup, D, 1));
+    const cudaError_t e =
+        cudaFuncSetAttribute(attn_q4_kernel<D, PACK, SH, Q16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             q4_smem(PACK ? 4 : kMaxGroup, D, 1));
     if (e == cudaSuccess) set[dev] = true;
     return e;
 }
 
-template <int D, bool PACK, bool SH>
+template <int D, bool PACK, bool SH, bool Q16>
 int q4_warps_for(int dev, int group, int q_f32) {
     static int cache[64][kMaxGroup + 1][2] = {};
     int& c = cache[dev][group][q_f32 ? 1 : 0];
     if (c == 0) {
         int per_sm = 0, sms = 0;
-        if (ensure_q4_attr<D, PACK, SH>(dev) != cudaSuccess) return 0;
+        if (ensure_q4_attr<D, PACK, SH, Q16>(dev) != cudaSuccess) return 0;
         if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attn_q4_kernel<D, PACK, SH>, kQ4Warps * 32,
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attn_q4_kernel<D, PACK, SH, Q16>, kQ4Threads,
                                                           q4_smem(group, D, q_f32)) != cudaSuccess)
             return 0;
-        c = (per_sm < 1 ? 1 : per_sm) * sms * kQ4Warps;
+        c = (per_sm < 1 ? 1 : per_sm) * sms * kQ4Workers;
     }
     return c;
 }
 
 // Cooperative: merging warps wait for other CTAs' flags, so the whole grid
 // (sized to the resident capacity) is co-resident.
-template <int D, bool PACK, bool SH>
+template <int D, bool PACK, bool SH, bool Q16>
 cudaError_t launch_q4(const AttnParamsOf<SH>& p, cudaStream_t s) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if ((e = ensure_q4_attr<D, PACK, SH>(dev)) != cudaSuccess) return e;
-    const dim3 grid((p.n_warps + kQ4Warps - 1) / kQ4Warps), block(kQ4Warps * 32);
+    if ((e = ensure_q4_attr<D, PACK, SH, Q16>(dev)) != cudaSuccess) return e;
+    const dim3 grid((p.n_warps + kQ4Workers - 1) / kQ4Workers), block(kQ4Threads);
     void* args[] = {const_cast<AttnParamsOf<SH>*>(&p)};
-    return cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(&attn_q4_kernel<D, PACK, SH>), grid, block, args,
-                                       q4_smem(p.group, D, p.q_f32), s);
+    return cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(&attn_q4_kernel<D, PACK, SH, Q16>), grid, block,
+                                       args, q4_smem(p.group, D, p.q_f32), s);
+}
+
+// f(D, PACK, Q16 as integral constants) of a call: the one place that picks a variant.
+template <class F>
+auto q4_variant(int head_dim, int group, bool q16, F f) {
+    using std::false_type;
+    using std::true_type;
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    if (group <= 4) {
+        if (q16) return head_dim == 64 ? f(D64{}, true_type{}, true_type{}) : f(D128{}, true_type{}, true_type{});
+        return head_dim == 64 ? f(D64{}, true_type{}, false_type{}) : f(D128{}, true_type{}, false_type{});
+    }
+    if (q16) return head_dim == 64 ? f(D64{}, false_type{}, true_type{}) : f(D128{}, false_type{}, true_type{});
+    return head_dim == 64 ? f(D64{}, false_type{}, false_type{}) : f(D128{}, false_type{}, false_type{});
 }
 
 template <bool SH>
 cudaError_t launch_q4_any(const AttnParamsOf<SH>& p, int head_dim, cudaStream_t s) {
-    if (p.group <= 4) return head_dim == 64 ? launch_q4<64, true, SH>(p, s) : launch_q4<128, true, SH>(p, s);
-    return head_dim == 64 ? launch_q4<64, false, SH>(p, s) : launch_q4<128, false, SH>(p, s);
+    return q4_variant(head_dim, p.group, !p.q_f32, [&](auto d, auto pack, auto q16) {
+        return launch_q4<decltype(d)::value, decltype(pack)::value, SH, decltype(q16)::value>(p, s);
+    });
 }
 
 }  // namespace
 
 int attend_q4_warps(int device, int group, int head_dim, int q_f32, bool shaped) {
-    if (shaped) {
-        if (group <= 4)
-            return head_dim == 64 ? q4_warps_for<64, true, true>(device, group, q_f32)
-                                  : q4_warps_for<128, true, true>(device, group, q_f32);
-        return head_dim == 64 ? q4_warps_for<64, false, true>(device, group, q_f32)
-                              : q4_warps_for<128, false, true>(device, group, q_f32);
-    }
-    if (group <= 4)
-        return head_dim == 64 ? q4_warps_for<64, true, false>(device, group, q_f32)
-                              : q4_warps_for<128, true, false>(device, group, q_f32);
-    return head_dim == 64 ? q4_warps_for<64, false, false>(device, group, q_f32)
-                          : q4_warps_for<128, false, false>(device, group, q_f32);
+    return q4_variant(head_dim, group, !q_f32, [&](auto d, auto pack, auto q16) {
+        constexpr int D = decltype(d)::value;
+        constexpr bool PACK = decltype(pack)::value, Q16 = decltype(q16)::value;
+        return shaped ? q4_warps_for<D, PACK, true, Q16>(device, group, q_f32)
+                      : q4_warps_for<D, PACK, false, Q16>(device, group, q_f32);
+    });
 }
 
 cudaError_t launch_attend_q4(const AttnParams& p, int head_dim, cudaStream_t s) {
