@@ -339,8 +339,9 @@ lt_status lt_kv_profile_read_write(lt_kv* kv, double* total_ms, uint64_t* launch
 uint64_t lt_kv_launch_count(const lt_kv* kv);
 
 /* Attention launch sizing: each warp of the stream-K attention launch takes
- * at least `tiles` 16-position tiles (default 8), so small steps run on fewer
- * warps; large steps use every resident warp regardless.  Results do not
+ * at least `tiles` 16-position tiles (default 8; 4 for a small call over an
+ * LT_KV_Q4_0 cache or with shaped scores), so small steps run on fewer warps;
+ * large steps use every resident warp regardless.  Results do not
  * depend on it beyond f32 summation order of split merges. */
 lt_status lt_kv_set_min_tiles_per_warp(lt_kv* kv, uint32_t tiles);
 

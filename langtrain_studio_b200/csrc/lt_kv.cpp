@@ -31,6 +31,7 @@ constexpr int kSlots = 8;  // staging ring depth (pinned host + device pairs)
 constexpr uint32_t kCascadeMaxTokens = 1024;  // tokens of one call the prefix pass serves
 constexpr int kCascadeMinBlocks = 4;          // shortest shared prefix worth a pass (64 positions)
 constexpr size_t kExpandBytes = 128u << 20;   // f16 workspace of a 4-bit cache's prefix pass
+constexpr long long kSmallTiles = 1184;       // tiles of an attention call that counts as small
 constexpr uint32_t kClean = 0xFFFFFFFFu;
 
 struct Slot {
@@ -101,7 +102,7 @@ struct ProfRing {
 struct lt_kv {
     lt_kv_config cfg{};
     PeerGather peer;
-    uint32_t min_tiles_per_warp = 8;  // attention launch sizing (lt_kv_set_min_tiles_per_warp)
+    uint32_t min_tiles_per_warp = 0;  // attention launch sizing (lt_kv_set_min_tiles_per_warp); 0: the default
     // shared-prefix (cascade) pass: groups of >= cascade_min_tokens tokens
     // whose sequences share >= kCascadeMinBlocks leading blocks (0: off)
     uint32_t cascade_min_tokens = 8;
@@ -467,18 +468,32 @@ lt_status check_cells(lt_kv* kv, const int32_t* block, const int32_t* slot, uint
     return LT_OK;
 }
 
-// Two rows of one call for the same cell would race on its bytes; a 4-bit cell
-// (codes and scale of one row) must not mix two.  LT_KV_Q4_0 only: the other
-// formats' writes keep the order they had.
-lt_status check_distinct_cells(lt_kv* kv, const int32_t* block, const int32_t* slot, uint32_t n) {
-    if (kv->fmt != LT_KV_Q4_0 || n < 2) return LT_OK;
-    if (kv->cell_mark.empty()) kv->cell_mark.assign(kv->n_blocks, 0);
+// check_cells and the cells' upload image (cells_tmp) in one pass.  distinct:
+// refuse a cell named twice -- two rows for one cell would race on its bytes, and
+// a 4-bit cell (codes and scale of one row) must not mix two.  Only LT_KV_Q4_0
+// writes ask for it; the other formats' writes keep the order they had.
+lt_status take_cells(lt_kv* kv, const int32_t* block, const int32_t* slot, uint32_t n, bool distinct) {
+    if (n > kv->cfg.max_batch) return fail(kv, LT_E_ARG, "batch of %u tokens exceeds max_batch %u", n, kv->cfg.max_batch);
+    kv->cells_tmp.resize(n);
+    int2* out = kv->cells_tmp.data();
+    if (distinct && kv->cell_mark.empty()) kv->cell_mark.assign(kv->n_blocks, 0);
     const uint64_t ep = ++kv->cell_epoch << 16;
+    int32_t cur = -1;       // the run's block, and its slots so far
+    uint64_t mask = 0;
     for (uint32_t i = 0; i < n; ++i) {
-        uint64_t& m = kv->cell_mark[block[i]];
-        if ((m & ~0xFFFFull) != ep) m = ep;
-        if (m >> slot[i] & 1) return fail(kv, LT_E_ARG, "cell %u (block %d, slot %d) is named twice", i, block[i], slot[i]);
-        m |= 1ull << slot[i];
+        const int32_t b = block[i], s = slot[i];
+        if (b < 0 || (uint32_t)b >= kv->n_blocks || s < 0 || s >= kBlock)
+            return fail(kv, LT_E_ARG, "cell %u (block %d, slot %d) out of range", i, b, s);
+        out[i] = make_int2(b, s);
+        if (!distinct) continue;
+        if (b != cur) {
+            if (cur >= 0) kv->cell_mark[cur] = ep | mask;
+            cur = b;
+            const uint64_t m = kv->cell_mark[b];
+            mask = (m & ~0xFFFFull) == ep ? m & 0xFFFF : 0;
+        }
+        if (mask >> s & 1) return fail(kv, LT_E_ARG, "cell %u (block %d, slot %d) is named twice", i, b, s);
+        mask |= 1ull << s;
     }
     return LT_OK;
 }
@@ -732,7 +747,13 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
     // contexts) runs on fewer warps with fewer split merges instead of
     // paying every warp's ramp for one tile.
     const long long total_tiles = tiles * kv->cfg.n_kv_heads;
-    const long long want = (total_tiles + kv->min_tiles_per_warp - 1) / kv->min_tiles_per_warp;
+    // By default 8; a 4-bit or shaped call of at most kSmallTiles takes 4, which
+    // ends a small step sooner (one 17-token sequence of 4 heads: 13.1 us a call
+    // from 15.3; two of 300 tokens, 8 heads: 12.8 from 13.9) where a larger one
+    // loses more to merges (eight of 1000: 18.4 against 16.4).
+    long long min_tiles = kv->min_tiles_per_warp;
+    if (min_tiles == 0) min_tiles = (score || kv->fmt == LT_KV_Q4_0) && total_tiles <= kSmallTiles ? 4 : 8;
+    const long long want = (total_tiles + min_tiles - 1) / min_tiles;
     p.n_warps = (int32_t)std::min<long long>(max_warps, std::max<long long>(want, total_tiles ? 1 : 0));
     p.n_kv_heads = (int32_t)kv->cfg.n_kv_heads;
     p.group = (int32_t)kv->group;
@@ -1070,8 +1091,7 @@ lt_status lt_kv_write(lt_kv* kv, uint32_t layer, const int32_t* block, const int
     lt_status rc = check_dtypes(kv, {&dtype});
     if (rc || (rc = require_device(kv))) return rc;
     if (layer >= kv->cfg.n_layers) return fail(kv, LT_E_ARG, "layer %u out of range", layer);
-    if ((rc = check_cells(kv, block, slot, n))) return rc;
-    if ((rc = check_distinct_cells(kv, block, slot, n))) return rc;
+    if ((rc = take_cells(kv, block, slot, n, kv->fmt == LT_KV_Q4_0))) return rc;
     DeviceGuard g(kv->cfg.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (kv->fmt == LT_KV_Q4_0) {
@@ -1081,8 +1101,6 @@ lt_status lt_kv_write(lt_kv* kv, uint32_t layer, const int32_t* block, const int
     }
     if ((rc = flush(kv, st))) return rc;
     if (n == 0) return LT_OK;
-    kv->cells_tmp.resize(n);
-    for (uint32_t i = 0; i < n; ++i) kv->cells_tmp[i] = make_int2(block[i], slot[i]);
     const void* d_cells = nullptr;
     int s = -1;
     if ((rc = upload(kv, kv->cells_cache, kv->cells_tmp.data(), n * sizeof(int2), st, &d_cells, &s))) return rc;
@@ -1093,7 +1111,7 @@ lt_status lt_kv_write(lt_kv* kv, uint32_t layer, const int32_t* block, const int
         kv->write_in_bytes += (uint64_t)n * 2 * kv->cfg.n_kv_heads * kv->cfg.head_dim * (dtype == LT_F32 ? 4 : 2);
     }
     LT_CUDA(kv, ltkv::launch_write(kv->d_pool + (size_t)layer * kv->layer_elems, static_cast<const int2*>(d_cells),
-                                   (int)n, (int)kv->cfg.n_kv_heads, (int)kv->cfg.head_dim, k, v, dtype == LT_F32, kv->fmt,
+                                   (int)n, (int)kv->cfg.n_kv_heads, (int)kv->cfg.head_dim, slot[0], k, v, dtype == LT_F32, kv->fmt,
                                    st));
     if (ev_end) LT_CUDA(kv, cudaEventRecord(ev_end, st));
     kv->launches++;
@@ -1423,7 +1441,7 @@ lt_status lt_kv_read(lt_kv* kv, uint32_t layer, const int32_t* block, const int3
     lt_status rc = check_dtypes(kv, {&dtype});
     if (rc || (rc = require_device(kv))) return rc;
     if (layer >= kv->cfg.n_layers) return fail(kv, LT_E_ARG, "layer %u out of range", layer);
-    if ((rc = check_cells(kv, block, slot, n))) return rc;
+    if ((rc = take_cells(kv, block, slot, n, false))) return rc;
     if ((reinterpret_cast<uintptr_t>(k_out) & 15) || (reinterpret_cast<uintptr_t>(v_out) & 15))
         return fail(kv, LT_E_ARG, "k_out and v_out must be 16-byte aligned device pointers");
     DeviceGuard g(kv->cfg.device);
@@ -1431,13 +1449,11 @@ lt_status lt_kv_read(lt_kv* kv, uint32_t layer, const int32_t* block, const int3
     if ((rc = refuse_capture(kv, st, "lt_kv_read"))) return rc;
     if ((rc = flush(kv, st))) return rc;
     if (n == 0) return LT_OK;
-    kv->cells_tmp.resize(n);
-    for (uint32_t i = 0; i < n; ++i) kv->cells_tmp[i] = make_int2(block[i], slot[i]);
     const void* d_cells = nullptr;
     int s = -1;
     if ((rc = upload(kv, kv->cells_cache, kv->cells_tmp.data(), n * sizeof(int2), st, &d_cells, &s))) return rc;
     LT_CUDA(kv, ltkv::launch_read(kv->d_pool + (size_t)layer * kv->layer_elems, static_cast<const int2*>(d_cells),
-                                  (int)n, (int)kv->cfg.n_kv_heads, (int)kv->cfg.head_dim, k_out, v_out,
+                                  (int)n, (int)kv->cfg.n_kv_heads, (int)kv->cfg.head_dim, slot[0], k_out, v_out,
                                   dtype == LT_F32, kv->fmt, st));
     kv->launches++;
     return mark_slot_use(kv, s, st);

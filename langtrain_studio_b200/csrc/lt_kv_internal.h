@@ -189,10 +189,12 @@ int attend_launches(const AttnParams& p);
 cudaError_t launch_gather_permute(const void* gathered, void* out, int nranks, uint32_t n, size_t row_bytes,
                                   cudaStream_t s);
 
-cudaError_t launch_write(uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim,
+// first_slot: slot of cells[0], which the host knows (LT_KV_Q4_0 aligns blocks by it).
+cudaError_t launch_write(uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, int first_slot,
                          const void* k, const void* v, int in_f32, int fmt, cudaStream_t s);
-cudaError_t launch_write_q4(uint8_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, const void* k,
-                            const void* v, int in_f32, cudaStream_t s);
+// shift: slot of the call's first cell (0..15): blocks are tried from token -shift on.
+cudaError_t launch_write_q4(uint8_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, int shift,
+                            const void* k, const void* v, int in_f32, cudaStream_t s);
 
 // Blocks [0, count) of sequence root's table, expanded to f16 tiles as blocks
 // base, base + 1, ... of a workspace.
@@ -205,8 +207,8 @@ cudaError_t launch_expand_q4(const uint8_t* pool_layer, const int32_t* tables, i
                              cudaStream_t s);
 
 // Values of n cells of a pool of any format -> k_out, v_out [n][n_kv_heads*head_dim], f32 or f16.
-cudaError_t launch_read(const uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, void* k_out,
-                        void* v_out, int out_f32, int fmt, cudaStream_t s);
+cudaError_t launch_read(const uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim,
+                        int first_slot, void* k_out, void* v_out, int out_f32, int fmt, cudaStream_t s);
 
 // Block copies (copy-on-write and compaction moves) and table scatter.
 // copies: (src, dst) pairs; tw: (flat table index, value) pairs.  n_blocks

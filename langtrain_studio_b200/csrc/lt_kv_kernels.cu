@@ -300,6 +300,14 @@ __device__ __forceinline__ void merge_slots(const float* po, const float* pml, i
     }
 }
 
+constexpr float kResidualUp = 2048.f;
+
+// A row of O from its value and residual accumulators.
+template <bool UP>
+__device__ __forceinline__ float row_sum(float value, float residual) {
+    return UP ? fmaf(residual, 1.f / kResidualUp, value) : value + residual;
+}
+
 // S = Q K^T, online softmax and O += P V for one staged (block, head) tile.
 // SH: `sh` shapes the scores (before the mask) and masks the slots before its
 // first one too.
@@ -501,10 +509,14 @@ __device__ __forceinline__ void attend_tile_q8(const uint8_t* tile, int valid, c
         {
             const __half2 h01 = __floats2half2_rn(p0, p1), h23 = __floats2half2_rn(p2, p3);
             const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
+            // SH: the residual rows carry 2^11 times the residual (row_sum takes it
+            // off), or p * d ~ 0.01 would leave its residual below f16's smallest
+            // step: 4e-6 of an output against 5e-7.
+            constexpr float RS = SH ? kResidualUp : 1.f;
             pa[0] = h2_bits(h01);
-            pa[1] = h2_bits(__floats2half2_rn(p0 - f01.x, p1 - f01.y));
+            pa[1] = h2_bits(__floats2half2_rn((p0 - f01.x) * RS, (p1 - f01.y) * RS));
             pa[2] = h2_bits(h23);
-            pa[3] = h2_bits(__floats2half2_rn(p2 - f23.x, p3 - f23.y));
+            pa[3] = h2_bits(__floats2half2_rn((p2 - f23.x) * RS, (p3 - f23.y) * RS));
         }
         // columns 32c + 8*mi + r: one 16-byte run (16 slots) each
         uint32_t w0, w1, w2, w3, b0, b1;
@@ -849,8 +861,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
                     float acc[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        acc[nt][0] = o[nt][0] + o[nt][2];
-                        acc[nt][1] = o[nt][1] + o[nt][3];
+                        acc[nt][0] = row_sum<Q8 && SH>(o[nt][0], o[nt][2]);
+                        acc[nt][1] = row_sum<Q8 && SH>(o[nt][1], o[nt][3]);
                     }
                     if (!SH && dc.skip > 0) fold_prefix<D>(p, dc.tok, dc.h, g, t4, m_run, l, acc);
                     store_out<D>(p, dc.tok, dc.h, g, t4, acc, SH && l == 0.f ? 0.f : 1.f / l);
@@ -859,7 +871,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         *reinterpret_cast<float2*>(p.part_o + sl * GD + (size_t)g * D + nt * 8 + 2 * t4) =
-                            make_float2(o[nt][0] + o[nt][2], o[nt][1] + o[nt][3]);
+                            make_float2(row_sum<Q8 && SH>(o[nt][0], o[nt][2]), row_sum<Q8 && SH>(o[nt][1], o[nt][3]));
                     if (t4 == 0) {
                         p.part_ml[(sl * G + g) * 2] = m_run;
                         p.part_ml[(sl * G + g) * 2 + 1] = l;
@@ -950,8 +962,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
         float M = m_run, L = l, acc[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            acc[nt][0] = o[nt][0] + o[nt][2];
-            acc[nt][1] = o[nt][1] + o[nt][3];
+            acc[nt][0] = row_sum<Q8 && SH>(o[nt][0], o[nt][2]);
+            acc[nt][1] = row_sum<Q8 && SH>(o[nt][1], o[nt][3]);
         }
         merge_slots<D>(grouped ? p.part2_o : p.part_o, grouped ? p.part2_ml : p.part_ml, G, g, t4, gw + 1, w_last,
                        stride, M, L, acc);
@@ -1744,11 +1756,12 @@ cudaError_t launch_gather_permute(const void* gathered, void* out, int nranks, u
     return cudaGetLastError();
 }
 
-cudaError_t launch_write(uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, const void* k,
-                         const void* v, int in_f32, int fmt, cudaStream_t s) {
+cudaError_t launch_write(uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, int first_slot,
+                         const void* k, const void* v, int in_f32, int fmt, cudaStream_t s) {
     if (n == 0) return cudaSuccess;
     if (fmt == LT_KV_Q4_0)
-        return launch_write_q4(reinterpret_cast<uint8_t*>(pool_layer), cells, n, n_kv_heads, head_dim, k, v, in_f32, s);
+        return launch_write_q4(reinterpret_cast<uint8_t*>(pool_layer), cells, n, n_kv_heads, head_dim, first_slot, k, v,
+                               in_f32, s);
     const bool q8 = fmt == LT_KV_Q8_0;
     const int threads = n * n_kv_heads * 2 * (head_dim / 8);
     const int blocks = (threads + 255) / 256;

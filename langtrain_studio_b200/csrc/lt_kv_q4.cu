@@ -24,47 +24,61 @@ namespace {
 constexpr float kQ4MaxScale = 2720.0f;  // 8 significant bits, and 24 * d is still an f16
 
 // ------------------------------------------------------------ quantise ----
-// One 32-value group held as 4 values by each of 8 consecutive lanes (every
-// lane of the warp calls this).  Returns d; code[i] = clamp(floor(x / d + 1/2)
-// + 8, 0, 15), decided exactly: the borders (k + 1/2) * |d| have at most 13
-// significant bits, so comparing x with them in f32 settles what the rounded
-// quotient leaves open.  NaN: not counted in d, code 8 (value 0).
-__device__ __forceinline__ float q4_quant4(const float (&x)[4], uint32_t (&code)[4]) {
+// The scale of a 32-value group from its extremes top = max(x, 0) and low =
+// max(-x, 0): signed so that the larger magnitude takes code 0; |d| in ad.
+__device__ __forceinline__ float q4_scale(float top, float low, float& ad) {
+    const bool pos = top >= low;  // the positive extreme takes -8 * d
+    const float a = fminf(__bfloat162float(__float2bfloat16_rn((pos ? top : low) * 0.125f)), kQ4MaxScale);
+    ad = __half2float(__float2half_rn(a));
+    return pos ? -ad : ad;
+}
+
+// clamp(floor(x / d + 1/2) + 8, 0, 15) as the last byte of the result (the rest
+// is to be masked off), decided exactly.  xs = x with d's sign taken off, inv ~
+// 1 / |d|.  k, rounded from a quotient brought down by 2^-10 (far more than
+// its error), is the answer or one below it; the border (k + 1/2) * |d| has at
+// most 13 significant bits, so comparing xs with it in f32 settles which.  Adding
+// 1.5 * 2^23 rounds to an integer and leaves it in the last bits.  NaN, or d = 0:
+// code 8.
+__device__ __forceinline__ uint32_t q4_code(float xs, float ad, float inv) {
+    constexpr float kRound = 12582912.f;
+    const float x = fminf(fmaxf(xs, -8.f * ad), 7.f * ad);  // exact bounds: codes 0 and 15
+    float k = __fadd_rn(__fadd_rn(__fmaf_rn(x, inv, -0.0009765625f), kRound), -kRound);
+    if (x >= __fmaf_rn(k, ad, 0.5f * ad)) k += 1.f;
+    k = ad > 0.f && xs == xs ? k : 0.f;
+    return __float_as_uint(__fadd_rn(k, kRound + 8.f));
+}
+
+// One group held as N values by each of 32 / N consecutive lanes (every lane of
+// the warp calls this): its codes; returns d.  NaN does not count in the scale.
+template <int N>
+__device__ __forceinline__ float q4_quant(const float (&x)[N], uint32_t (&code)[N]) {
     float top = 0.f, low = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
         top = fmaxf(top, x[i]);
         low = fmaxf(low, -x[i]);
     }
 #pragma unroll
-    for (int m = 1; m < 8; m <<= 1) {
+    for (int m = 1; m < 32 / N; m <<= 1) {
         top = fmaxf(top, __shfl_xor_sync(kFull, top, m));
         low = fmaxf(low, __shfl_xor_sync(kFull, low, m));
     }
-    const bool pos = top >= low;  // the positive extreme takes -8 * d
-    const float a = fminf(__bfloat162float(__float2bfloat16_rn((pos ? top : low) * 0.125f)), kQ4MaxScale);
-    const float ad = __half2float(__float2half_rn(a));
-    const float inv = ad > 0.f ? 1.0f / ad : 0.f;
+    float ad;
+    const float d = q4_scale(top, low, ad);
+    const float inv = ad > 0.f ? __fdividef(1.0f, ad) : 0.f;
+    const bool neg = top >= low;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float xs = pos ? -x[i] : x[i];
-        float k = floorf(fmaf(xs, inv, 0.5f));
-        k = fminf(fmaxf(k, -9.f), 8.f);  // NaN -> -9, put right below
-        if (xs < (k - 0.5f) * ad) k -= 1.f;
-        else if (xs >= (k + 0.5f) * ad) k += 1.f;
-        k = fminf(fmaxf(k, -8.f), 7.f);
-        if (!(ad > 0.f) || xs != xs) k = 0.f;
-        code[i] = (uint32_t)((int)k + 8);
-    }
-    return pos ? -ad : ad;
+    for (int i = 0; i < N; ++i) code[i] = q4_code(neg ? -x[i] : x[i], ad, inv);  // (last bytes)
+    return d;
 }
 
-// Store a lane's four codes (dims 16i + 2t, +1, +8, +9) of slot `slot`, and
+// Store a lane's four codes (as q4_code gives them; dims 16i + 2t, +1, +8, +9) of slot `slot`, and
 // the group's scale from its first lane, into a tile.
 template <int D>
 __device__ __forceinline__ void q4_store4(uint8_t* tile, int kvsel, int i, int t, int slot, const uint32_t (&code)[4],
                                           float d) {
-    const uint8_t b0 = (uint8_t)(code[0] | (code[2] << 4)), b1 = (uint8_t)(code[1] | (code[3] << 4));
+    const uint8_t b0 = (uint8_t)((code[0] & 15) | (code[2] << 4)), b1 = (uint8_t)((code[1] & 15) | (code[3] << 4));
     const int e = 16 * i + 2 * t;
     if (kvsel == 0) {
         uint8_t* w = tile + q4_kbyte(slot, e);
@@ -95,32 +109,57 @@ __device__ __forceinline__ void load4_f32(const void* base, size_t idx, int in_f
 }
 
 // --------------------------------------------------------------- write ----
-// D/4 lanes per (token, head, K|V) row, four values a lane; 8 lanes share a
-// 32-value group.  Bytes belong to one slot, so rows of one block written by
-// different warps never touch the same byte.  Lanes past the end only take
-// part in the shuffles.
+// One CTA per (16 tokens of the call, head): D/8 lanes a row, eight values a lane, a
+// group is four lanes.  Bytes belong to one slot, so rows of one block written by
+// different warps or CTAs never touch the same byte; but stored one by one
+// straight to the pool they cost a 32-byte sector each (V's lie 64 bytes apart).
+// Tokens that fill a block (a prefill chunk; `shift` aligns the first block of
+// the call) therefore meet in a tile image in shared memory, stored 16 bytes a
+// thread.  4096 tokens of 8 x 128 f16: 23 us byte by byte with four values a lane, 20
+// through the image, issue-bound; eight values a lane halve what a group costs.
 template <int D>
-__global__ void __launch_bounds__(256) kv_write_q4_kernel(uint8_t* __restrict__ pool_layer,
-                                                          const int2* __restrict__ cells, int n, int n_kv_heads,
-                                                          const void* __restrict__ k, const void* __restrict__ v,
-                                                          int in_f32) {
-    constexpr int L = D / 4;
-    const long long gid = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const bool live = gid < (long long)n * n_kv_heads * 2 * L;
-    const int lane = (int)(gid % L);
-    long long r = gid / L;
-    const int kvsel = (int)(r & 1);
-    r >>= 1;
-    const int h = (int)(r % n_kv_heads);
-    const int tok = (int)(r / n_kv_heads);
-    const int i = lane >> 2, t = lane & 3;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live) load4_f32(kvsel ? v : k, ((size_t)tok * n_kv_heads + h) * D + 16 * i + 2 * t, in_f32, x);
-    uint32_t code[4];
-    const float d = q4_quant4(x, code);
-    if (!live) return;
-    const int2 cell = cells[tok];
-    q4_store4<D>(pool_layer + ((size_t)cell.x * n_kv_heads + h) * q4_tile_bytes(D), kvsel, i, t, cell.y, code, d);
+__global__ void __launch_bounds__(4 * D) kv_write_q4_kernel(uint8_t* __restrict__ pool_layer,
+                                                            const int2* __restrict__ cells, int n, int n_kv_heads,
+                                                            int shift, const void* __restrict__ k,
+                                                            const void* __restrict__ v, int in_f32) {
+    constexpr int TILE = q4_tile_bytes(D), L = D / 8;  // lanes of a row
+    __shared__ __align__(16) uint8_t image[TILE];
+    const int j = threadIdx.x / (2 * L), kvsel = threadIdx.x / L & 1, c = threadIdx.x % L;
+    const int h = blockIdx.x % n_kv_heads, tok0 = (int)(blockIdx.x / n_kv_heads) * kBlock - shift, tok = tok0 + j;
+    const bool live = tok >= 0 && tok < n;
+    const int2 cell = live ? __ldg(cells + tok) : make_int2(-1, -1);
+    const int block0 = tok0 >= 0 ? __ldg(cells + tok0).x : -1;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (live) load8_f32(kvsel ? v : k, ((size_t)tok * n_kv_heads + h) * D + 8 * c, in_f32, x);
+    const bool full = __syncthreads_and(live && cell.y == j && cell.x == block0);
+    uint8_t* tile = full ? image : pool_layer + ((size_t)max(cell.x, 0) * n_kv_heads + h) * TILE;
+    const int slot = max(cell.y, 0);
+    uint32_t code[8];
+    const float d = q4_quant<8>(x, code);
+    // One code a byte: values 0-3 and 4-7.  Units c and c^1 (dims 16i.. and 16i + 8 ..)
+    // share their bytes; the even lane stores dims 0-3 of the pair, the odd one 4-7.
+    const uint32_t lo = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
+    const uint32_t hi = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
+    const bool odd = c & 1;
+    const uint32_t got = __shfl_xor_sync(kFull, odd ? lo : hi, 1);
+    const uint32_t bytes = odd ? got | (hi << 4) : lo | (got << 4);
+    if (live) {
+        const int e = 16 * (c >> 1) + (odd ? 4 : 0);
+        // dims e .. e + 3: K in two words 16 bytes apart (bytes 0, 2 of each), V in four 64 bytes apart
+        uint8_t* at = tile + (kvsel ? 8 * D + q4_vbyte(slot, e) : q4_kbyte(slot, e));
+        const int step1 = kvsel ? 64 : 2, step2 = kvsel ? 128 : 16;
+        at[0] = (uint8_t)bytes;
+        at[step1] = (uint8_t)(bytes >> 8);
+        at[step2] = (uint8_t)(bytes >> 16);
+        at[step2 + step1] = (uint8_t)(bytes >> 24);
+        if ((c & 3) == 0)
+            *reinterpret_cast<uint16_t*>(tile + (kvsel ? q4_vscale<D>(slot, c >> 2) : q4_kscale<D>(slot, c >> 2))) =
+                __half_as_ushort(__float2half_rn(d));
+    }
+    if (!full) return;
+    __syncthreads();
+    uint4* dst = reinterpret_cast<uint4*>(pool_layer + ((size_t)block0 * n_kv_heads + h) * TILE);
+    if (threadIdx.x < TILE / 16) dst[threadIdx.x] = reinterpret_cast<const uint4*>(image)[threadIdx.x];
 }
 
 // ---------------------------------------------------------------- read ----
@@ -346,12 +385,122 @@ __host__ __device__ inline int q4_smem(int group, int head_dim, int q_f32) {
     return kQ4Workers * (q4_worker_smem(group, head_dim, q_f32) + (int)sizeof(Q4Ring));
 }
 
+// Turn a 4 x 4 array over within each quad: lane t gives r[s], s = 0..3, and
+// gets the r[t] of lanes 0..3.
+__device__ __forceinline__ void quad_transpose(uint32_t (&r)[4], int t) {
+    const bool odd = t & 1, top = t & 2;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const uint32_t got = __shfl_xor_sync(kFull, odd ? r[i] : r[i + 1], 1);
+        if (odd) r[i] = got; else r[i + 1] = got;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t got = __shfl_xor_sync(kFull, top ? r[i] : r[i + 2], 2);
+        if (top) r[i] = got; else r[i + 2] = got;
+    }
+}
+
+// Values of one part of a 4-bit tile: part = (K 0 | V 1) * D/64 + run ch, the
+// dims 64 ch ... of all 16 slots.  put(kvsel, slot, c, x) gets the f16 dims
+// 8c .. 8c+7 of a slot.  The words are read and dequantised as the attention
+// kernel's A fragments; V's are turned over by movmatrix, so that every register
+// is two neighbouring dims of a slot, and quads then gather eight of them.
+constexpr int q4_parts(int D) { return 2 * (D / 64); }
+
+template <int D, class Put>
+__device__ __forceinline__ void q4_part_values(const uint8_t* tile, int part, int lane, Put put) {
+    constexpr int G32 = D / 32, R = D / 64;
+    const int g = lane >> 2, t = lane & 3, kvsel = part / R, ch = part % R;
+    const Q4Magic magic{0x64006400u, 0x54005400u};
+    const uint4 wv = __ldg(reinterpret_cast<const uint4*>(tile + kvsel * 8 * D + ch * 512 + lane * 16));
+    const uint32_t ws[4] = {wv.x, wv.y, wv.z, wv.w};
+    uint32_t r[2][2][4];  // [slots g, g + 8][dims .., + 8][16-dim step]
+    if (kvsel == 0) {
+        const __half* ks = reinterpret_cast<const __half*>(tile + 16 * D + g * (4 * G32)) + 2 * ch;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const __half2 d0 = __half2half2(ks[s >> 1]), d1 = __half2half2(ks[G32 + (s >> 1)]);  // slots g, g + 8
+            const uint32_t w = ws[s], w8 = w >> 8;
+            r[0][0][s] = h2_bits(__hmul2(q4_low(w, magic), d0));
+            r[0][1][s] = h2_bits(__hmul2(q4_high(w, magic), d0));
+            r[1][0][s] = h2_bits(__hmul2(q4_low(w8, magic), d1));
+            r[1][1][s] = h2_bits(__hmul2(q4_high(w8, magic), d1));
+        }
+    } else {
+        const uint4 vd = __ldg(reinterpret_cast<const uint4*>(tile + 17 * D + (t * G32 + 2 * ch) * 8));
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const __half2 dA = as_h2(s < 2 ? vd.x : vd.z), dB = as_h2(s < 2 ? vd.y : vd.w);
+            const uint32_t w = ws[s], w8 = w >> 8;
+            r[0][0][s] = movmatrix_trans(h2_bits(__hmul2(q4_low(w, magic), dA)));
+            r[0][1][s] = movmatrix_trans(h2_bits(__hmul2(q4_high(w, magic), dA)));
+            r[1][0][s] = movmatrix_trans(h2_bits(__hmul2(q4_low(w8, magic), dB)));
+            r[1][1][s] = movmatrix_trans(h2_bits(__hmul2(q4_high(w8, magic), dB)));
+        }
+    }
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            quad_transpose(r[sl][hf], t);
+            put(kvsel, g + 8 * sl, 2 * (4 * ch + t) + hf,
+                make_uint4(r[sl][hf][0], r[sl][hf][1], r[sl][hf][2], r[sl][hf][3]));
+        }
+}
+
+// lt_kv_read of 4-bit cells, one CTA per (16 cells of the call, head) as in the
+// write: cells that fill a block are read as a tile, a part a warp; others a
+// cell a warp at a time, eight values a lane.
+template <int D>
+__global__ void __launch_bounds__(q4_parts(D) * 32) kv_read_q4_kernel(const uint8_t* __restrict__ pool_layer,
+                                                                      const int2* __restrict__ cells, int n,
+                                                                      int n_kv_heads, int shift,
+                                                                      void* __restrict__ k_out,
+                                                                      void* __restrict__ v_out, int out_f32) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.x % n_kv_heads, i0 = (int)(blockIdx.x / n_kv_heads) * kBlock - shift;
+    // lane l looks at cell i0 + l % 16: every warp finds the same answer
+    const int mine = i0 + (lane & 15);
+    const bool live = mine >= 0 && mine < n;
+    const int2 cell = live ? __ldg(cells + mine) : make_int2(-1, -1);
+    const int block0 = __shfl_sync(kFull, cell.x, 0);
+    if (__all_sync(kFull, live && cell.y == (lane & 15) && cell.x == block0)) {
+        const uint8_t* tile = pool_layer + ((size_t)block0 * n_kv_heads + h) * q4_tile_bytes(D);
+        q4_part_values<D>(tile, warp, lane, [&](int kvsel, int slot, int c, uint4 x) {
+            void* out = kvsel ? v_out : k_out;
+            const size_t at = ((size_t)(i0 + slot) * n_kv_heads + h) * D + 8 * c;
+            if (!out_f32) {
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = x;
+                return;
+            }
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 y = __half22float2(as_h2(w[j]));
+                f[2 * j] = y.x;
+                f[2 * j + 1] = y.y;
+            }
+            store8_as(out, at, 1, f);
+        });
+        return;
+    }
+    constexpr int CH = D / 8, W = q4_parts(D);
+    for (int j = warp; j < kBlock; j += W) {
+        const int blk = __shfl_sync(kFull, cell.x, j), slot = __shfl_sync(kFull, cell.y, j);
+        if (blk < 0 || lane >= 2 * CH) continue;
+        const int kvsel = lane / CH, c = lane % CH;
+        float x[8];
+        cell_values8<D, LT_KV_Q4_0>(pool_layer, (size_t)blk * n_kv_heads + h, kvsel, slot, c, x);
+        store8_as(kvsel ? v_out : k_out, ((size_t)(i0 + j) * n_kv_heads + h) * D + 8 * c, out_f32, x);
+    }
+}
+
 // -------------------------------------------------------------- expand ----
 // 4-bit tiles -> f16 tiles (lt_kv_layout.cuh) for the shared-prefix pass, whose
-// tensor-core operands they are.  One warp per (block, head).  The words are
-// read and dequantised as the attention kernel's A fragments; V's are turned
-// over by movmatrix, so that every register is two neighbouring dims of a slot
-// and four lanes store one 16-byte chunk.  Reads 18*D bytes and writes 64*D.
+// tensor-core operands they are.  One warp per (block, head, part).  Reads
+// 18*D bytes a tile and writes 64*D.
 struct ExpandParams {
     const uint8_t* pool;
     const int32_t* tables;
@@ -364,11 +513,11 @@ struct ExpandParams {
 
 template <int D>
 __global__ void __launch_bounds__(256) expand_q4_kernel(const __grid_constant__ ExpandParams p) {
-    constexpr int G32 = D / 32;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31;
     const int item = (int)((blockIdx.x * 256u + threadIdx.x) >> 5);
-    if (item >= p.total * p.n_kv_heads) return;
-    const int h = item % p.n_kv_heads, b = item / p.n_kv_heads;
+    constexpr int P = q4_parts(D);
+    if (item >= p.total * p.n_kv_heads * P) return;
+    const int part = item % P, h = item / P % p.n_kv_heads, b = item / P / p.n_kv_heads;
     int lo = 0, hi = p.n_groups - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -379,34 +528,9 @@ __global__ void __launch_bounds__(256) expand_q4_kernel(const __grid_constant__ 
     const int src = checked_block(__ldg(p.tables + (size_t)gr.root * p.max_blocks + i), p.n_blocks, p.err);
     const uint8_t* tile = p.pool + ((size_t)src * p.n_kv_heads + h) * q4_tile_bytes(D);
     uint16_t* out = p.out + ((size_t)(gr.base + i) * p.n_kv_heads + h) * (2 * kBlock * D);
-    const Q4Magic magic{0x64006400u, 0x54005400u};
-    auto put = [&](int kvsel, int slot, int e, __half2 v) {  // dims e, e + 1 of a slot
-        *reinterpret_cast<__half2*>(out + kvsel * kBlock * D + chunk_off(e >> 3, slot) + (e & 7)) = v;
-    };
-#pragma unroll
-    for (int ch = 0; ch < D / 64; ++ch) {
-        const uint4 kw = __ldg(reinterpret_cast<const uint4*>(tile + ch * 512 + lane * 16));
-        const uint4 vw = __ldg(reinterpret_cast<const uint4*>(tile + 8 * D + ch * 512 + lane * 16));
-        const uint4 vd = __ldg(reinterpret_cast<const uint4*>(tile + 17 * D + (t * G32 + 2 * ch) * 8));
-        const __half* ks = reinterpret_cast<const __half*>(tile + 16 * D + g * (4 * G32));
-        const uint32_t kws[4] = {kw.x, kw.y, kw.z, kw.w}, vws[4] = {vw.x, vw.y, vw.z, vw.w};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int e = 16 * (4 * ch + s) + 2 * t, c = 2 * ch + (s >> 1);
-            const __half2 d0 = __half2half2(ks[c]), d1 = __half2half2(ks[G32 + c]);  // slots g, g + 8
-            const uint32_t w = kws[s], w8 = w >> 8;
-            put(0, g, e, __hmul2(q4_low(w, magic), d0));
-            put(0, g, e + 8, __hmul2(q4_high(w, magic), d0));
-            put(0, g + 8, e, __hmul2(q4_low(w8, magic), d1));
-            put(0, g + 8, e + 8, __hmul2(q4_high(w8, magic), d1));
-            const uint32_t x = vws[s], x8 = x >> 8;
-            const __half2 dA = as_h2(s < 2 ? vd.x : vd.z), dB = as_h2(s < 2 ? vd.y : vd.w);
-            put(1, g, e, as_h2(movmatrix_trans(h2_bits(__hmul2(q4_low(x, magic), dA)))));
-            put(1, g, e + 8, as_h2(movmatrix_trans(h2_bits(__hmul2(q4_high(x, magic), dA)))));
-            put(1, g + 8, e, as_h2(movmatrix_trans(h2_bits(__hmul2(q4_low(x8, magic), dB)))));
-            put(1, g + 8, e + 8, as_h2(movmatrix_trans(h2_bits(__hmul2(q4_high(x8, magic), dB)))));
-        }
-    }
+    q4_part_values<D>(tile, part, lane, [&](int kvsel, int slot, int c, uint4 x) {
+        *reinterpret_cast<uint4*>(out + kvsel * kBlock * D + chunk_off(c, slot)) = x;
+    });
 }
 
 // The values of a (token, head)'s result that one lane holds once the columns
@@ -829,7 +953,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
             load4_f32(kvsel ? p.v_new : p.k_new, (size_t)dc.tok * Hkv * D + (size_t)dc.h * D + 16 * i + 2 * t, p.kv_f32,
                       x);
             uint32_t code[4];
-            const float d = q4_quant4(x, code);
+            const float d = q4_quant<4>(x, code);
             q4_store4<D>(tile, kvsel, i, t, slot, code, d);
             q4_store4<D>(cell_tile, kvsel, i, t, slot, code, d);
         }
@@ -1266,7 +1390,7 @@ cudaError_t launch_expand_q4(const uint8_t* pool_layer, const int32_t* tables, i
             p.first[i] = p.total;
             p.total += groups[g0 + i].count;
         }
-        const unsigned blocks = (unsigned)(((long long)p.total * n_kv_heads + 7) / 8);
+        const unsigned blocks = (unsigned)(((long long)p.total * n_kv_heads * q4_parts(head_dim) + 7) / 8);
         if (head_dim == 64) expand_q4_kernel<64><<<blocks, 256, 0, s>>>(p);
         else expand_q4_kernel<128><<<blocks, 256, 0, s>>>(p);
         const cudaError_t e = cudaGetLastError();
@@ -1275,14 +1399,14 @@ cudaError_t launch_expand_q4(const uint8_t* pool_layer, const int32_t* tables, i
     return cudaSuccess;
 }
 
-cudaError_t launch_write_q4(uint8_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, const void* k,
-                            const void* v, int in_f32, cudaStream_t s) {
-    const long long blocks = ((long long)n * n_kv_heads * 2 * (head_dim / 4) + 255) / 256;
+cudaError_t launch_write_q4(uint8_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, int shift,
+                            const void* k, const void* v, int in_f32, cudaStream_t s) {
+    const long long blocks = ((long long)n + shift + kBlock - 1) / kBlock * n_kv_heads;
     if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
     if (head_dim == 64)
-        kv_write_q4_kernel<64><<<(unsigned)blocks, 256, 0, s>>>(pool_layer, cells, n, n_kv_heads, k, v, in_f32);
+        kv_write_q4_kernel<64><<<(unsigned)blocks, 256, 0, s>>>(pool_layer, cells, n, n_kv_heads, shift, k, v, in_f32);
     else
-        kv_write_q4_kernel<128><<<(unsigned)blocks, 256, 0, s>>>(pool_layer, cells, n, n_kv_heads, k, v, in_f32);
+        kv_write_q4_kernel<128><<<(unsigned)blocks, 512, 0, s>>>(pool_layer, cells, n, n_kv_heads, shift, k, v, in_f32);
     return cudaGetLastError();
 }
 
@@ -1292,13 +1416,21 @@ cudaError_t launch_rows_q4(const uint8_t* pool_layer, const int32_t* table_row, 
                                        n_blocks, err, s);
 }
 
-cudaError_t launch_read(const uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, void* k_out,
-                        void* v_out, int out_f32, int fmt, cudaStream_t s) {
+cudaError_t launch_read(const uint16_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim,
+                        int first_slot, void* k_out, void* v_out, int out_f32, int fmt, cudaStream_t s) {
     if (n == 0) return cudaSuccess;
     const uint8_t* pool = reinterpret_cast<const uint8_t*>(pool_layer);
-    if (fmt == LT_KV_Q4_0)
-        return launch_read_fmt<LT_KV_Q4_0>(pool, cells, nullptr, n, n_kv_heads, head_dim, k_out, v_out, out_f32, 0,
-                                           nullptr, s);
+    if (fmt == LT_KV_Q4_0) {
+        const long long blocks = ((long long)n + first_slot + kBlock - 1) / kBlock * n_kv_heads;
+        if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+        if (head_dim == 64)
+            kv_read_q4_kernel<64><<<(unsigned)blocks, q4_parts(64) * 32, 0, s>>>(pool, cells, n, n_kv_heads, first_slot,
+                                                                               k_out, v_out, out_f32);
+        else
+            kv_read_q4_kernel<128><<<(unsigned)blocks, q4_parts(128) * 32, 0, s>>>(pool, cells, n, n_kv_heads, first_slot,
+                                                                                 k_out, v_out, out_f32);
+        return cudaGetLastError();
+    }
     if (fmt == LT_KV_Q8_0)
         return launch_read_fmt<LT_KV_Q8_0>(pool, cells, nullptr, n, n_kv_heads, head_dim, k_out, v_out, out_f32, 0,
                                            nullptr, s);
