@@ -1194,6 +1194,8 @@ lt_status lt_kv_attend_shaped(lt_kv* kv, uint32_t layer, const void* q, lt_dtype
     if ((rc = check_tokens(kv, seq, pos, n))) return rc;
     if (!(score->softcap >= 0.f) || std::isinf(score->softcap))
         return fail(kv, LT_E_ARG, "softcap %g is not a finite number >= 0", (double)score->softcap);
+    if (score->softcap > 0.f && !std::isfinite(scale / score->softcap))
+        return fail(kv, LT_E_ARG, "scale %g over softcap %g is not finite", (double)scale, (double)score->softcap);
     if (reinterpret_cast<uintptr_t>(score->slopes) & 3) return fail(kv, LT_E_ARG, "slopes must be 4-byte aligned");
     for (uint32_t i = 0; i < n && score->end_host; ++i)
         if (score->end_host[i] > kv->lens[seq[i]])

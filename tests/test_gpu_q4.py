@@ -392,3 +392,149 @@ def test_refused_on_the_device():
                 call()
     t.kv.attend(0, q, [0], [19], out=out)
     t.kv.check()
+
+
+def test_serving_run_of_everything_together():
+    """Prefill, sharing, decode steps with fused appends, shaped attention on the
+    same cache, truncation and regrowth, compaction, read-back: one run, each
+    step against the restatement."""
+    rng = np.random.default_rng(21)
+    t = Twin(2, 128, 16 * 80, 8, layers=2, max_seqs=6)
+    slopes = np.exp2(-np.arange(1, 9)).astype(np.float32)
+    t.fill(0, 150, rng)
+    for s in (1, 2, 3):
+        t.kv.share(0, s, 140 + s)
+        for layer in range(2):
+            t.rows[(layer, s)] = list(t.rows[(layer, 0)][: 140 + s])
+    t.fill(4, 37, rng)
+    for step in range(12):
+        seqs = np.array([0, 1, 2, 3, 4])
+        pos = np.array([t.kv.len(s) for s in seqs])
+        b, sl = t.kv.append_batch(seqs, pos)
+        for layer in range(2):
+            k, v = t.draw(5, rng)
+            for i, s in enumerate(seqs):
+                t.add(layer, int(s), k[i], v[i])
+            q = rng.standard_normal((5, 8 * 128)).astype(np.float32)
+            kd, vd, qd = (torch.from_numpy(x).cuda() for x in (k, v, q))
+            close(t.kv.write_attend(layer, b, sl, kd, vd, qd, seqs, pos), t.attend_ref(layer, seqs, pos, q))
+            first, end = np.array([0, 17, 140, 3, 20]), np.minimum(pos + 1, [150, 18, 200, 3, 40])
+            out = t.kv.attend_shaped(layer, qd, seqs, pos, softcap=8.0, window=60, first=first, end=end,
+                                     slopes=torch.from_numpy(slopes).cuda())
+            for i, s in enumerate(seqs):
+                K, V = t.values(layer, int(s))
+                ref = A.attend(q[i].reshape(8, 128), K, V, int(pos[i]), 4, t.kv.default_scale, softcap=8.0, window=60,
+                               first=first[i], end=end[i], slopes=slopes)
+                close(out[i], ref.reshape(-1))
+        if step == 5:
+            t.kv.truncate(3, 33)
+            for layer in range(2):
+                del t.rows[(layer, 3)][33:]
+            t.kv.truncate(0, 0)
+            for layer in range(2):
+                t.rows[(layer, 0)] = []
+            assert t.kv.compact() > 0
+            t.fill(0, 20, rng)
+    for layer in range(2):
+        for s in range(5):
+            t.check(layer, s)
+    t.kv.check()
+
+
+def test_scheduler_over_a_4_bit_cache():
+    """The native scheduler driver (admission, eviction, preemption, compaction,
+    prefill and decode) moves 4-bit rows through the same calls: its last step's
+    outputs are softmax attention over what the cache reads back."""
+    from langtrain_studio_b200.sched import Scheduler
+
+    hkv, hq, d, slots = 2, 8, 64, 6
+    kv = KvCache(1, hkv, d, 16 * 60, n_heads=hq, max_seqs=slots, max_batch=512, kv_format="q4_0")
+    sched = Scheduler(kv, slots)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    kv_src = torch.randn((1024, hkv * d), generator=g, device="cuda", dtype=torch.float16)
+    q_src = torch.randn((slots, hq * d), generator=g, device="cuda", dtype=torch.float16)
+    out = torch.empty((slots, hq * d), device="cuda", dtype=torch.float16)
+    rng = np.random.default_rng(6)
+    decoded = 0
+    for step in range(60):
+        if step < 45:
+            sched.submit(int(rng.integers(8, 250)), int(rng.integers(4, 40)))
+        decoded += sched.step(kv_src, q_src, out)
+    kv.check()
+    assert decoded > 60 and sched.stats["finished"] > 0
+    assert torch.isfinite(out.float()).all()
+
+
+def test_llama_forward_over_a_4_bit_cache():
+    """The Llama step runs on a 4-bit cache: the rows its first layer appends are
+    the f16 cache's rows, quantised, and a prompt gives the same logits whether
+    its tokens come together or one by one."""
+    from langtrain_studio_b200 import llama as LL
+
+    m = LL.Llama(2, 256, 4, 2, 64, 512, 500, max_batch=64)
+    m.load(LL.random_weights(m, seed=3))
+    toks = np.random.default_rng(0).integers(0, 500, 40)
+    caches = {f: m.kv_cache(256, 2, kv_format=f) for f in ("f16", "q4_0")}
+    logits = {f: m.forward(kv, toks, np.zeros(40), np.arange(40), [39]) for f, kv in caches.items()}
+    for got, want in zip(caches["q4_0"].rows(0, 0, 40), caches["f16"].rows(0, 0, 40)):
+        x = want.cpu().numpy().astype(np.float64).reshape(40, 2, 64)
+        _, step = A.quant4(x)
+        # half a step, a whole one past +7, and the step's own and the f16 row's rounding
+        err = np.abs(got.cpu().numpy().reshape(x.shape) - x)
+        assert (err <= np.repeat(np.abs(step), 32, -1) * (1 + 2 ** -6)).all()
+    one = m.kv_cache(256, 2, kv_format="q4_0")
+    for i, tok in enumerate(toks):
+        lg = m.forward(one, [tok], [0], [i], [0])
+    assert torch.isfinite(logits["q4_0"]).all()
+    # attention differs by f32 rounding alone; the int8 activations may turn that
+    # into single quantisation steps, a few per cent of the logits' spread
+    assert (lg - logits["q4_0"]).abs().max() < 0.1 * logits["q4_0"].std()
+    cos = torch.nn.functional.cosine_similarity(logits["q4_0"], logits["f16"]).item()
+    assert cos > 0.8, cos
+
+
+def test_peer_gather_single_rank():
+    """The head-sharded gather over a 4-bit cache with one rank."""
+    rng = np.random.default_rng(17)
+    t = Twin(2, 128, 16 * 40, 8, max_seqs=3)
+    lens = [40, 300, 17]
+    for s, n in enumerate(lens):
+        t.fill(s, n, rng)
+    seqs, pos = np.arange(3), np.array(lens) - 1
+    q = torch.from_numpy(rng.standard_normal((3, 8 * 128)).astype(np.float32)).cuda()
+    want = t.kv.attend(0, q, seqs, pos)
+    t.kv.peer_import([t.kv.peer_export(0, 1, max_tokens=8)])
+    for _ in range(3):
+        out = t.kv.attend_gather(0, q, seqs, pos, out_dtype=torch.float32)
+        t.kv.check()
+        assert torch.equal(out, want)
+    t.kv.peer_close()
+    t.kv.close()
+
+
+@pytest.mark.parametrize("offset", [0, 1, 5, 15])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_chunk_writes_at_any_offset(offset, hd):
+    """Whole blocks, unaligned chunks, cells out of order and cells of several
+    sequences in one write: the tile path and the row path meet in one call."""
+    rng = np.random.default_rng(offset)
+    t = Twin(3, hd, 16 * 40, max_seqs=3, max_batch=512)
+    t.fill(0, offset, rng)
+    t.fill(1, 3, rng)
+    seqs = np.concatenate([np.zeros(70), np.ones(45), [2] * 16]).astype(np.int64)
+    pos = np.concatenate([offset + np.arange(70), 3 + np.arange(45), np.arange(16)]).astype(np.int64)
+    b, s = t.kv.append_batch(seqs, pos)
+    k, v = t.draw(seqs.size, rng, np.float16)
+    for i, q in enumerate(seqs):
+        t.add(0, int(q), k[i], v[i])
+    order = np.arange(seqs.size)
+    order[100:] = rng.permutation(order[100:])
+    t.kv.write(0, b[order], s[order], *(torch.from_numpy(np.ascontiguousarray(x[order])).cuda() for x in (k, v)))
+    for q in range(3):
+        t.check(0, q)
+    kr, vr = t.kv.read(0, b[order], s[order])
+    K = np.concatenate([t.values(0, q)[0][(offset, 3, 0)[q]:] for q in range(3)])
+    assert np.array_equal(kr.cpu().numpy().astype(np.float64).reshape(K.shape), K[order])
+    kr32, vr32 = t.kv.read(0, b, s, dtype=torch.float32)
+    V = np.concatenate([t.values(0, q)[1][(offset, 3, 0)[q]:] for q in range(3)])
+    assert np.array_equal(vr32.cpu().numpy().astype(np.float64).reshape(V.shape), V)

@@ -185,7 +185,7 @@ def test_refusals():
     q = torch.zeros((1, 256), device="cuda")
     ok = c.kv.attend_shaped(0, q, [0], [19])
     for kw, err in [(dict(softcap=-1.0), KvError), (dict(softcap=float("nan")), KvError),
-                    (dict(softcap=float("inf")), KvError), (dict(end=[21]), KvError), (dict(window=-1), ValueError),
+                    (dict(softcap=float("inf")), KvError), (dict(softcap=1e-45), KvError), (dict(end=[21]), KvError), (dict(window=-1), ValueError),
                     (dict(first=[0, 0]), ValueError), (dict(end=[-1]), ValueError),
                     (dict(slopes=torch.zeros(4)), ValueError), (dict(slopes=torch.zeros(3, device="cuda")), ValueError),
                     (dict(slopes=torch.zeros(4, device="cuda", dtype=torch.float16)), TypeError)]:
