@@ -113,9 +113,9 @@ def workload(seed: int):
 
 
 def kv_row_bytes(kv_dim: int, kv_format: str = "f16") -> float:
-    """Cached bytes of one K (or V) row: f16 values, or Q8_0 int8 values plus
-    one f16 scale per 32."""
-    return kv_dim * 2 if kv_format == "f16" else kv_dim * 34 / 32
+    """Cached bytes of one K (or V) row: f16 values, or int8 (Q8_0) or 4-bit
+    (Q4_0) values plus one f16 scale per 32."""
+    return kv_dim * {"f16": 64, "q8_0": 34, "q4_0": 18}[kv_format] / 32
 
 
 IO_BYTES = 4  # q, new K/V rows and outputs cross the ABI as f32, the model runner's types (model.rs:393-400)
@@ -289,7 +289,8 @@ def c2_config(world: int, kv_format: str = "f16") -> dict:
         "kv_format": kv_format,
         "step": "append 1 token/seq + fused K/V write + decode attention (f32 softmax/accumulate); q, new K/V rows "
                 "and outputs in f32, the model runner's types (model.rs:393-400)"
-                + ("; K/V cached as Q8_0 (int8 + f16 scale per 32 values)" if kv_format == "q8_0" else ""),
+                + {"q8_0": "; K/V cached as Q8_0 (int8 + f16 scale per 32 values)",
+                   "q4_0": "; K/V cached as Q4_0 (4-bit codes + f16 scale per 32 values)"}.get(kv_format, ""),
         "kv_bytes_per_step": b["attn"],
         "l2": "inputs larger than L2: ~%.1f GB of K/V read per step vs 126 MB L2" % (b["attn"] / 1e9),
         "parallelism": f"seq-sharded x{world} (independent pools, no collective); every rank serves the same "
@@ -427,7 +428,7 @@ def run_ours(args, rank, world, local):
 
     result = None
     if rank == 0:
-        q8 = args.kv_format == "q8_0"
+        q8, q4 = args.kv_format == "q8_0", args.kv_format == "q4_0"
         peak, peak_kind = measured_peak()
         avg_attn_ms = attn_ms / max(attn_n, 1)
         per_launch_bytes = total_bytes / max(args.steps, 1)
@@ -450,10 +451,12 @@ def run_ours(args, rank, world, local):
             "hbm_gbs": total_bytes / (ms_max * 1e-3) / 1e9 * world,
             "roofline": {
                 "bound": "hbm",
-                "kernel": "paged_attn_kernel<128, %s> (fused append + attention)" % ("q8" if q8 else "f16"),
+                "kernel": "attn_q4_kernel<128> (fused append + attention)" if q4 else
+                          "paged_attn_kernel<128, %s> (fused append + attention)" % ("q8" if q8 else "f16"),
                 "achieved": achieved, "peak": peak, "peak_kind": peak_kind, "unit": "GB/s",
                 "frac": achieved / peak,
-                "traffic": ncu_traffic("paged_attn_q8_c2.md" if q8 else "paged_attn_c2.md"),
+                "traffic": ncu_traffic("paged_attn_q4_c2.md" if q4 else
+                                       "paged_attn_q8_c2.md" if q8 else "paged_attn_c2.md"),
                 "algorithmic_bytes_per_launch": int(per_launch_bytes), "avg_launch_ms": avg_attn_ms,
             },
             "e2e": {"value": tokens / (e2e_ms * 1e-3), "unit": "tokens/s", "h2d_bytes_per_step": h2d,
@@ -1494,7 +1497,7 @@ def main():
                          "a separate NCCL all-gather (nccl)")
     ap.add_argument("--emulate-ranks", type=int, default=1,
                     help="c4-*: on one GPU, run the per-rank work of an R-GPU run (sequences or KV heads / R)")
-    ap.add_argument("--kv-format", choices=["f16", "q8_0"], default="f16",
+    ap.add_argument("--kv-format", choices=["f16", "q8_0", "q4_0"], default="f16",
                     help="c2 / c4-*: cached K/V format (f16: the reference's; q8_0: int8 + f16 scale per 32)")
     ap.add_argument("--cpu-seconds", type=float, default=15.0,
                     help="CPU-baseline sample budget in seconds (rank 0, N=1); 0 skips it")
@@ -1520,7 +1523,8 @@ def main():
         return
     res = run_ours(args, rank, world, local)
     if rank == 0 and res is not None:
-        if world == 1 and args.cpu_seconds > 0:
+        # the restated reference path holds f16 and Q8_0 caches
+        if world == 1 and args.cpu_seconds > 0 and args.kv_format != "q4_0":
             threads = os.cpu_count() or 1
             value, steps, dt = cpu_run(workload(1234), 1234, budget_s=args.cpu_seconds, max_steps=10 ** 6,
                                        threads=threads, kv_format=args.kv_format)

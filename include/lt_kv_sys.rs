@@ -19,13 +19,20 @@ pub struct LtKvConfig {
     pub n_layers: u32, pub n_kv_heads: u32, pub head_dim: u32, pub n_heads: u32,
     pub n_tokens: u32, pub max_seqs: u32, pub max_batch: u32, pub max_blocks_per_seq: u32,
     pub device: i32,
-    pub kv_format: u32,  // LT_KV_F16 (0, the reference's cache) or LT_KV_Q8_0 (1)
+    pub kv_format: u32,  // LT_KV_F16 (0, the reference's cache), LT_KV_Q8_0 (1) or LT_KV_Q4_0 (2)
+}
+#[repr(C)]
+pub struct LtKvScore {
+    pub softcap: f32, pub window: u32,
+    pub slopes: usize,  // address of f32 [n_heads] on the device, or 0
+    pub first_host: usize, pub end_host: usize,  // addresses of u32 [n], or 0
 }
 #[repr(C)] pub struct LtKv { _p: [u8; 0] }
 pub const LT_F32: i32 = 0;
 pub const LT_F16: i32 = 1;
 pub const LT_KV_F16: u32 = 0;
 pub const LT_KV_Q8_0: u32 = 1;
+pub const LT_KV_Q4_0: u32 = 2;
 pub const LT_E_FULL: i32 = 1;
 pub const LT_E_NONCONTIG: i32 = 2;
 pub const LT_E_ARG: i32 = 3;
@@ -57,6 +64,15 @@ extern "C" {
                               q: *const c_void, q_dtype: i32, seq: *const u32, pos: *const u32,
                               n: u32, out: *mut c_void, out_dtype: i32, scale: f32,
                               stream: *mut c_void) -> i32;
+    // attention with shaped scores: tanh cap, window, distance slopes, per-token intervals
+    pub fn lt_kv_attend_shaped(kv: *mut LtKv, layer: u32, q: *const c_void, q_dtype: i32,
+                               seq: *const u32, pos: *const u32, n: u32, score: *const LtKvScore,
+                               out: *mut c_void, out_dtype: i32, scale: f32,
+                               stream: *mut c_void) -> i32;
+    // values of cells: the inverse of lt_kv_write
+    pub fn lt_kv_read(kv: *mut LtKv, layer: u32, block: *const i32, slot: *const i32, n: u32,
+                      k_out: *mut c_void, v_out: *mut c_void, dtype: i32,
+                      stream: *mut c_void) -> i32;
     pub fn lt_kv_truncate(kv: *mut LtKv, seq: u32, from: u32);
     pub fn lt_kv_share(kv: *mut LtKv, src: u32, dst: u32, len: u32);
     pub fn lt_kv_compact(kv: *mut LtKv, moved: *mut u32, stream: *mut c_void) -> i32;
