@@ -295,11 +295,11 @@ cudaError_t launch_read_fmt(const uint8_t* pool, const int2* cells, const int32_
 // A worker takes two tiles a step: their score chains (MMA, scale, max, 2^x,
 // transpose, MMA) are independent and fill one another's latencies.
 constexpr int kQ4Workers = 4;   // worker warps of a CTA
-constexpr int kQ4Stages = 8;    // tiles in a worker's ring
 constexpr int kQ4Step = 2;      // tiles a step
-constexpr int kQ4Pieces = 16;   // piece descriptors in its ring (> tiles ahead + 2; a power of two)
+constexpr int kQ4Stages = 4;    // steps' worth of tiles in a worker's ring (a power of two)
+constexpr int kQ4Pieces = 8;    // piece descriptors in its ring (> stages ahead + 2; a power of two)
 constexpr int kQ4Threads = (kQ4Workers + 1) * 32;
-constexpr int kQ4Lanes = kQ4Workers > 8 ? 2 : 4;  // producer lanes of a worker
+constexpr int kQ4Lanes = 4;  // producer lanes of a worker: two stages' tiles
 
 // D = A * B (f16 operands, f32 accumulators from zero).
 __device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -352,10 +352,12 @@ struct Q4Piece {
 };
 
 // What a worker and its producer lanes share.
+constexpr int kQ4QBufs = 4;  // q buffers at most
 struct Q4Ring {
-    unsigned long long full[kQ4Stages];
-    uint32_t consumed, q_taken;  // by the worker: tiles done, pieces whose q rows it has read
-    uint32_t issued;             // by the producer
+    unsigned long long full[kQ4Stages];   // a stage's tiles have arrived (one tile at a piece's odd end)
+    unsigned long long q_full[kQ4QBufs];  // a piece's q rows have arrived (they come ahead of its tiles)
+    uint32_t consumed, q_taken;  // by the worker: stages done, pieces whose q rows it has read
+    uint32_t issued, q_issued;   // by the producer: stages, q rows
     uint32_t none, stop, stopped;  // range without tiles; the worker gave up; the producer has seen it
     Q4Piece pieces[kQ4Pieces];
 };
@@ -372,13 +374,13 @@ __device__ __forceinline__ void st_release_cta(uint32_t* p, uint32_t v) {
 __host__ __device__ inline int q4_qbuf_bytes(int group, int head_dim, int q_f32) {
     return (group * head_dim * (q_f32 ? 4 : 2) + 127) & ~127;
 }
-// q buffers of a worker: 4 KiB worth, at most 4.
+// q buffers of a worker: 4 KiB worth, at most kQ4QBufs.
 __host__ __device__ inline int q4_qbufs(int group, int head_dim, int q_f32) {
     const int n = 4096 / q4_qbuf_bytes(group, head_dim, q_f32);
-    return n < 1 ? 1 : n > 4 ? 4 : n;
+    return n < 1 ? 1 : n > kQ4QBufs ? kQ4QBufs : n;
 }
 __host__ __device__ inline int q4_worker_smem(int group, int head_dim, int q_f32) {
-    return kQ4Stages * q4_tile_bytes(head_dim) +
+    return kQ4Stages * kQ4Step * q4_tile_bytes(head_dim) +
            q4_qbufs(group, head_dim, q_f32) * q4_qbuf_bytes(group, head_dim, q_f32);
 }
 __host__ __device__ inline int q4_smem(int group, int head_dim, int q_f32) {
@@ -551,7 +553,7 @@ __device__ __forceinline__ void q4_merge_slots(const float* po, const float* pml
                                                int last, int stride, float (&M)[2], float (&L)[2],
                                                float (&acc)[D / 16][Own<PACK>::N]) {
     using O = Own<PACK>;
-    constexpr int U = 2;
+    constexpr int U = PACK ? 4 : 2;
     const int h0 = O::head(0, t);
     const int lastv = first + ((last - first) / stride) * stride;
     for (int w = first; w <= lastv; w += U * stride) {
@@ -650,7 +652,7 @@ __device__ __forceinline__ void q4_store_rows(void* dst, bool f16, int G, int g,
 // The producer warp: kQ4Lanes lanes feed each worker.
 template <int D, bool SH>
 __device__ __forceinline__ void q4_produce(const AttnParamsOf<SH>& p, uint8_t* stages0, Q4Ring* rings, int lane) {
-    constexpr int TILE = q4_tile_bytes(D), S = kQ4Stages;
+    constexpr int TILE = q4_tile_bytes(D), S = kQ4Stages, NT = kQ4Step;
     const int G = p.group, Hkv = p.n_kv_heads, C = p.piece_cost;
     const int WSM = q4_worker_smem(G, D, p.q_f32), QBUF = q4_qbuf_bytes(G, D, p.q_f32), nqb = q4_qbufs(G, D, p.q_f32);
     const uint32_t qbytes = (uint32_t)(G * D * (p.q_f32 ? 4 : 2));
@@ -658,7 +660,7 @@ __device__ __forceinline__ void q4_produce(const AttnParamsOf<SH>& p, uint8_t* s
     const int c = min(lane / LN, kQ4Workers - 1), u = lane % LN;
     const int gw = blockIdx.x * kQ4Workers + c;
     Q4Ring* ring = rings + c;
-    const uint32_t stages = smem_u32(stages0) + c * WSM, qbufs = stages + S * TILE, bar0 = smem_u32(ring->full);
+    const uint32_t stages = smem_u32(stages0) + c * WSM, qbufs = stages + S * NT * TILE, bar0 = smem_u32(ring->full);
     const TokenDesc* toks = p.toks ? p.toks : p.inl;
     const uint8_t* pool = reinterpret_cast<const uint8_t*>(p.pool_layer);
     const uint32_t T = (uint32_t)p.tiles_per_head * Hkv, NW = (uint32_t)p.n_warps, quo = T / NW, rem = T % NW;
@@ -681,7 +683,7 @@ __device__ __forceinline__ void q4_produce(const AttnParamsOf<SH>& p, uint8_t* s
         gh = (int)(off / nv);
         go = (int)(off % nv);
     }
-    int stage = 0, qslot = nqb - 1;  // of the next tile, of the piece being issued
+    int qslot = nqb - 1;  // q buffer of the piece being issued
     int pi = -1, it = 0, len = 0, head = 0, tok = 0, b_last = -1;  // the piece being issued
     const int32_t* trow = p.tables;
     int id = 0;  // block of tile it + u
@@ -705,23 +707,25 @@ __device__ __forceinline__ void q4_produce(const AttnParamsOf<SH>& p, uint8_t* s
                 if (u == 0) st_release_cta(&ring->stopped, 1);
                 live = false;
             } else if (it < len) {
+                // lane u issues tile it + u, the u % NT-th of stage issued + u / NT
                 const int room = S - (int)(issued - done);
-                int n = min(min(LN, room), len - it);
+                int n = min(min(LN / NT, room), (len - it + NT - 1) / NT);
                 if (it == 0 && pi - (int)taken >= nqb) n = 0;  // no q buffer free
                 if (n > 0) {
-                    if (u < n) {
-                        const int st = stage + u >= S ? stage + u - S : stage + u;
-                        const bool with_q = it + u == 0;
-                        mbar_arrive_expect_tx(bar0 + 8u * st, TILE + (with_q ? qbytes : 0u));
-                        bulk_g2s(stages + st * TILE, pool + ((size_t)id * Hkv + head) * TILE, TILE, bar0 + 8u * st);
-                        if (with_q)
-                            bulk_g2s(qbufs + qslot * QBUF,
-                                     static_cast<const uint8_t*>(p.q) + ((size_t)tok * Hkv + head) * qbytes, qbytes,
-                                     bar0 + 8u * st);
+                    if (it == 0 && u == 0) {
+                        const uint32_t qbar = smem_u32(ring->q_full) + 8u * qslot;
+                        mbar_arrive_expect_tx(qbar, qbytes);
+                        bulk_g2s(qbufs + qslot * QBUF,
+                                 static_cast<const uint8_t*>(p.q) + ((size_t)tok * Hkv + head) * qbytes, qbytes, qbar);
+                        st_release_cta(&ring->q_issued, (uint32_t)pi + 1);
+                    }
+                    if (u < n * NT && it + u < len) {
+                        const uint32_t st = (issued + u / NT) % S, bar = bar0 + 8u * st;
+                        if (u % NT == 0) mbar_arrive_expect_tx(bar, TILE * min(NT, len - it - u));
+                        bulk_g2s(stages + (st * NT + u % NT) * TILE, pool + ((size_t)id * Hkv + head) * TILE, TILE, bar);
                     }
                     issued += n;
-                    it += n;
-                    stage = stage + n >= S ? stage + n - S : stage + n;
+                    it = min(it + n * NT, len);
                     if (u == 0) st_release_cta(&ring->issued, issued);
                     load_id();
                     moved = true;
@@ -738,7 +742,7 @@ __device__ __forceinline__ void q4_produce(const AttnParamsOf<SH>& p, uint8_t* s
                     live = false;
                     if (first && u == 0) {  // ... and has no tile: wake the worker
                         st_release_cta(&ring->none, 1);
-                        mbar_arrive(bar0);
+                        mbar_arrive(smem_u32(ring->q_full));
                     }
                 } else {
                     first = false;
@@ -820,7 +824,8 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
     if (warp < kQ4Workers) {
         Q4Ring* r = rings + warp;
         if (lane < S) mbar_init(smem_u32(r->full) + 8u * lane, 1);
-        if (lane == S) r->consumed = r->q_taken = r->issued = r->none = r->stop = r->stopped = 0;
+        else if (lane < S + kQ4QBufs) mbar_init(smem_u32(r->q_full) + 8u * (lane - S), 1);
+        if (lane == 31) r->consumed = r->q_taken = r->issued = r->q_issued = r->none = r->stop = r->stopped = 0;
         fence_mbar_init();
     }
     __syncthreads();
@@ -833,14 +838,14 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
 
     Q4Ring* ring = rings + warp;
     uint8_t* stages = smem + (size_t)warp * WSM;
-    uint8_t* qbufs = stages + S * TILE;
+    uint8_t* qbufs = stages + S * NT * TILE;
     const int QBUF = q4_qbuf_bytes(G, D, p.q_f32), nqb = q4_qbufs(G, D, p.q_f32);
     const uint32_t bar0 = smem_u32(ring->full);
     const uint32_t T = (uint32_t)p.tiles_per_head * Hkv;
     const int g = lane >> 2, t = lane & 3;
     int ci = 0, ct = 0;  // the piece in hand, and its tiles consumed
-    int consumed = 0, cstage = 0, cphase = 0;
-    int qslot = 0;  // q buffer of the next piece
+    uint32_t consumed = 0;  // stages
+    int qslot = 0, qphase = 0;  // q buffer of the next piece
     int c_len = 0, c_end = 0, c_lo = 0, c_q = 0;  // its length; its end, first position and own position from its start
     // an opaque zero keeps the exponent patterns in registers (see Q4Magic)
     const uint32_t zero = (uint32_t)p.n_warps >> 31;
@@ -965,11 +970,9 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
     // (weights 0, finite values): one copy of the code serves both.
     auto step = [&](int nt) {
         const uint8_t* tiles[NT];
+        tiles[0] = stages + (consumed % S) * (NT * TILE);
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            const int st = cstage + (u < nt ? u : 0);
-            tiles[u] = stages + (size_t)(st >= S ? st - S : st) * TILE;
-        }
+        for (int u = 1; u < NT; ++u) tiles[u] = u < nt ? tiles[0] + u * TILE : tiles[0];
         // S^T = K Q^T
         float sc[NT][4];  // (slot g | g+8) x (column 2t | 2t+1)
 #pragma unroll
@@ -1120,20 +1123,19 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
         }
     };
 
-    // The worker that holds tile x: the last w with floor(T * w / n) <= x.
-    auto warp_of = [&](int x) { return (int)(((long long)(x + 1) * p.n_warps - 1) / (long long)T); };
-    // Lane u < nt waits for the u-th of the next tiles; true for all lanes or none.
-    auto wait_tiles = [&](int nt) {
-        const int st = cstage + lane;
-        const bool wrap = st >= S;
-        const bool here = lane >= nt || mbar_wait_bounded(bar0 + 8u * (wrap ? st - S : st), (uint32_t)(cphase ^ wrap));
-        const bool all = __all_sync(kFull, here);
-        __syncwarp();  // the waiting lanes' view of the copied bytes reaches the others
-        return all;
+    // The worker that holds tile x: the last w with floor(T * w / n) <= x, from a
+    // rounded quotient (a 64-bit division costs ten times the correction).
+    auto warp_of = [&](int x) {
+        const uint32_t NW = (uint32_t)p.n_warps, quo = T / NW, rem = T % NW;
+        auto start = [&](int w) { return (int)(quo * (uint32_t)w + rem * (uint32_t)w / NW); };
+        int w = min(p.n_warps - 1, (int)__fdividef((float)x * (float)p.n_warps, (float)T));
+        while (w > 0 && start(w) > x) --w;
+        while (w + 1 < p.n_warps && start(w + 1) <= x) ++w;
+        return w;
     };
     for (;;) {
-        if (ct == c_len) {  // the next piece: its descriptor came before its first tile
-            if (!wait_tiles(1)) {
+        if (ct == c_len) {  // the next piece: its descriptor came before its q rows
+            if (!mbar_wait_bounded(smem_u32(ring->q_full) + 8u * qslot, (uint32_t)qphase)) {
                 ok = false;
                 break;
             }
@@ -1146,7 +1148,10 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
             c_q = c.qpos - base;
             ct = 0;
             load_q(qbufs + qslot * QBUF);
-            qslot = qslot + 1 == nqb ? 0 : qslot + 1;
+            if (++qslot == nqb) {
+                qslot = 0;
+                qphase ^= 1;
+            }
             __syncwarp();
             if (lane == 0) st_release_cta(&ring->q_taken, (uint32_t)ci + 1);
 #pragma unroll
@@ -1155,26 +1160,18 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
             l_run[0] = l_run[1] = 0.f;
         }
         const int nt = min(c_len - ct, NT);
-        if (!wait_tiles(nt)) {
+        if (!mbar_wait_bounded(bar0 + 8u * (consumed % S), consumed / S & 1)) {
             ok = false;
             break;
         }
         const bool fill = !SH && p.k_new && ct + nt == c_len && ring->pieces[ci % kQ4Pieces].last_block >= 0;
-        if (fill) {
-            const int st = cstage + nt - 1;
-            append(stages + (size_t)(st >= S ? st - S : st) * TILE);
-        }
+        if (fill) append(stages + ((consumed % S) * NT + nt - 1) * TILE);
         step(nt);
-        consumed += nt;
-        cstage += nt;
-        if (cstage >= S) {
-            cstage -= S;
-            cphase ^= 1;
-        }
+        ++consumed;
         ct += nt;
         if (fill) fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) st_release_cta(&ring->consumed, (uint32_t)consumed);
+        if (lane == 0) st_release_cta(&ring->consumed, consumed);
         if (ct < c_len) continue;
 
         // ---- piece done ----
@@ -1279,8 +1276,10 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
             st_release_cta(&ring->stop, 1);
             const uint64_t t_stop = global_ns();
             while (!ld_acquire_cta(&ring->stopped) && global_ns() - t_stop < kWaitLimitNs / 4) __nanosleep(100);
-            const int issued = (int)ld_acquire_cta(&ring->issued);
-            for (int jj = consumed; jj < issued; ++jj) mbar_wait_bounded(bar0 + 8u * (jj % S), (jj / S) & 1);
+            const uint32_t issued = ld_acquire_cta(&ring->issued), q_issued = ld_acquire_cta(&ring->q_issued);
+            for (uint32_t j = consumed; j < issued; ++j) mbar_wait_bounded(bar0 + 8u * (j % S), j / S & 1);
+            for (uint32_t j = ld_acquire_cta(&ring->q_taken); j < q_issued; ++j)
+                mbar_wait_bounded(smem_u32(ring->q_full) + 8u * (j % nqb), j / nqb & 1);
             st_release_gpu(p.flags + gw, p.epoch);
         }
         __syncwarp();
