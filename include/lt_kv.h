@@ -178,7 +178,7 @@ lt_status lt_kv_attend(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtyp
  * interval are not read, and nothing that a masked cell holds (Inf, NaN)
  * reaches an output. */
 typedef struct lt_kv_score {
-    float softcap;              /* finite, >= 0; 0: no cap                       */
+    float softcap;              /* 0 .. 1e30; 0: no cap                         */
     uint32_t window;            /* positions before and with the token's own;    0: all */
     const float* slopes;        /* device [n_heads], or NULL                     */
     const uint32_t* first_host; /* [n] first position attended, or NULL          */

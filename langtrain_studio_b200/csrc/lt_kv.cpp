@@ -761,7 +761,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
     p.q_f32 = q_f32;
     p.out = out;
     p.out_f32 = out_dtype == LT_F32;
-    p.scale_log2 = scale * 1.4426950408889634f;
+    p.scale_log2 = scale * ltkv::kLog2e;
     p.part_o = kv->d_part_o;
     p.part_ml = kv->d_part_ml;
     p.flags = kv->d_flags;
@@ -805,7 +805,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         const float cap = score->softcap;
         p.shape.capped = cap > 0.f;
         p.shape.scale_cap = cap > 0.f ? scale / cap : 0.f;
-        p.shape.cap_log2 = cap * 1.4426950408889634f;
+        p.shape.cap_log2 = cap * ltkv::kLog2e;
         p.shape.scale_log2 = p.scale_log2;
         p.shape.slopes = score->slopes;
         p.shapes = nullptr;
@@ -883,7 +883,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
                 rollback();
                 return fail(kv, LT_E_CUDA, "expand launch: %s", cudaGetErrorString(xe));
             }
-            kv->launches++;
+            kv->launches += (kv->exp_groups.size() + ltkv::kExpandGroups - 1) / ltkv::kExpandGroups;
             pp.pool_layer = kv->d_exp;
             pp.tables = kv->d_iota;
             pp.max_blocks = 1;
@@ -1192,8 +1192,8 @@ lt_status lt_kv_attend_shaped(lt_kv* kv, uint32_t layer, const void* q, lt_dtype
     if (!score) return fail(kv, LT_E_ARG, "attend_shaped without a score");
     if (layer >= kv->cfg.n_layers) return fail(kv, LT_E_ARG, "layer %u out of range", layer);
     if ((rc = check_tokens(kv, seq, pos, n))) return rc;
-    if (!(score->softcap >= 0.f) || std::isinf(score->softcap))
-        return fail(kv, LT_E_ARG, "softcap %g is not a finite number >= 0", (double)score->softcap);
+    if (!(score->softcap >= 0.f && score->softcap <= 1e30f))  // beyond, s / softcap and softcap * log2(e) leave f32's range
+        return fail(kv, LT_E_ARG, "softcap %g is not in [0, 1e30]", (double)score->softcap);
     if (score->softcap > 0.f && !std::isfinite(scale / score->softcap))
         return fail(kv, LT_E_ARG, "scale %g over softcap %g is not finite", (double)scale, (double)score->softcap);
     if (reinterpret_cast<uintptr_t>(score->slopes) & 3) return fail(kv, LT_E_ARG, "slopes must be 4-byte aligned");
@@ -1427,6 +1427,7 @@ lt_status lt_kv_rows(lt_kv* kv, uint32_t layer, uint32_t seq, uint32_t n, void* 
         return fail(kv, LT_E_ARG, "rows(layer %u, seq %u, n %u) out of range", layer, seq, n);
     DeviceGuard g(kv->cfg.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (kv->fmt == LT_KV_Q4_0 && (rc = refuse_capture(kv, st, "lt_kv_rows of a 4-bit cache"))) return rc;
     if ((rc = flush(kv, st))) return rc;
     LT_CUDA(kv, ltkv::launch_rows(kv->d_pool + (size_t)layer * kv->layer_elems,
                                   kv->d_tables + (size_t)seq * kv->max_blocks, (int)n, (int)kv->cfg.n_kv_heads,

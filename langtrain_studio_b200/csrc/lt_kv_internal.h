@@ -20,6 +20,7 @@ inline bool dtype_valid(const lt_dtype& d) {
     return v == (int32_t)LT_F32 || v == (int32_t)LT_F16;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;  // scores are in log2 units
 constexpr int kBlock = 16;           // tokens per block (kv.rs:13)
 constexpr int kMaxGroup = 8;         // q heads per KV head the attention kernel handles
 

@@ -115,8 +115,10 @@ __device__ __forceinline__ void load4_f32(const void* base, size_t idx, int in_f
 // straight to the pool they cost a 32-byte sector each (V's lie 64 bytes apart).
 // Tokens that fill a block (a prefill chunk; `shift` aligns the first block of
 // the call) therefore meet in a tile image in shared memory, stored 16 bytes a
-// thread.  4096 tokens of 8 x 128 f16: 23 us byte by byte with four values a lane, 20
-// through the image, issue-bound; eight values a lane halve what a group costs.
+// thread.  4096 tokens of 8 x 128 f16 (38 MB, 5.8 us at the copy rate): 23 us byte
+// by byte with four values a lane, 20 through the image, 16 with eight values a
+// lane, which halves what a group's extremes and scale cost.  Instruction issue
+// bounds it (the exact codes).
 template <int D>
 __global__ void __launch_bounds__(4 * D) kv_write_q4_kernel(uint8_t* __restrict__ pool_layer,
                                                             const int2* __restrict__ cells, int n, int n_kv_heads,
@@ -285,8 +287,11 @@ cudaError_t launch_read_fmt(const uint8_t* pool, const int2* cells, const int32_
 //
 // What bounds it: instruction issue.  An mma.sync m16n8k16 keeps its scheduler
 // from issuing anything else for 8 cycles on this chip, so a tile (D = 128)
-// costs 16 x 8 cycles of MMA (32 x 8 for larger groups) beside ~290 other
-// instructions, against ~380 cycles that its 2304 bytes take from HBM.
+// costs 16 x 8 scheduler cycles of MMA (32 x 8 for larger groups) beside ~290
+// other instructions, ~180 of them the half-rate unpacking, where its 2304 bytes
+// take ~400 scheduler cycles (4 schedulers x 148 SMs) from HBM.  64 sequences of 512
+// to 4096, 32 / 8 heads: 54 us (26 at the copy rate; 0.54 instructions issued a
+// cycle, DRAM 39 %); 16 of 32768, 64 / 8 heads, f16 q: 158 us (92).
 //
 // Q16 (f16 q): q has no residual, so PACK's columns 4-7 repeat the values and
 // the scores come out in both halves without an exchange; larger groups take

@@ -538,3 +538,47 @@ def test_chunk_writes_at_any_offset(offset, hd):
     kr32, vr32 = t.kv.read(0, b, s, dtype=torch.float32)
     V = np.concatenate([t.values(0, q)[1][(offset, 3, 0)[q]:] for q in range(3)])
     assert np.array_equal(vr32.cpu().numpy().astype(np.float64).reshape(V.shape), V)
+
+
+def test_rows_are_refused_in_a_capture():
+    t = Twin(1, 64, 64, 4, max_seqs=2)
+    t.fill(0, 20, np.random.default_rng(0))
+    st = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    pad = torch.zeros(16, device="cuda")
+    with torch.cuda.graph(graph, stream=st):
+        pad.add_(1)
+        with pytest.raises(KvError, match="captured"):
+            t.kv.rows(0, 0, 20, stream=st)
+    t.check(0, 0)
+
+
+def test_offsets_past_32_bits():
+    """A layer of more than 2^32 bytes: blocks behind them are written, read and attended."""
+    blocks, hkv, hd, hq, n = 236000, 8, 128, 32, 100
+    kv = KvCache(1, hkv, hd, 16 * blocks, n_heads=hq, max_seqs=2, max_batch=65536, max_blocks_per_seq=blocks,
+                 kv_format="q4_0")
+    assert kv.bytes() > 2 ** 32 + 2 ** 25
+    used = 16 * (blocks - 8)
+    for p0 in range(0, used, 65536):
+        p = np.arange(p0, min(used, p0 + 65536), dtype=np.uint32)
+        kv.append_batch(np.zeros(p.size, np.uint32), p)
+    cells = kv.append_batch(np.ones(n, np.uint32), np.arange(n, dtype=np.uint32))
+    assert int(min(cells[0])) * hkv * 18 * hd > 2 ** 32
+    rng = np.random.default_rng(41)
+    x = rng.standard_normal((2, n, hkv * hd)).astype(np.float32)
+    kv.write(0, *cells, *(torch.from_numpy(a).cuda() for a in x))
+    val = A.value4(*A.quant4(x.reshape(2, n, hkv, hd)))
+    for got, want in zip(kv.read(0, *cells), val):
+        assert np.array_equal(got.cpu().numpy().astype(np.float64), want.reshape(n, -1))
+    for got, want in zip(kv.rows(0, 1, n), val):
+        assert np.array_equal(got.cpu().numpy().astype(np.float64), want.reshape(n, -1))
+    q = rng.standard_normal((n, hq * hd)).astype(np.float32)
+    for first in (0, n - 1):  # a prefill chunk (through the prefix pass), a single token
+        pos = np.arange(first, n)
+        ref = np.stack([A.attend(q[i].reshape(hq, hd), *val, int(i), hq // hkv, kv.default_scale).reshape(-1) for i in pos])
+        out = kv.attend(0, torch.from_numpy(q[first:]).cuda(), np.ones(pos.size), pos)
+        shaped = kv.attend_shaped(0, torch.from_numpy(q[first:]).cuda(), np.ones(pos.size), pos, window=n)
+        kv.check()
+        for o in (out, shaped):
+            np.testing.assert_allclose(o.cpu().numpy(), ref, rtol=1e-4, atol=2e-5)

@@ -198,3 +198,19 @@ def test_refusals():
             c.kv.attend_shaped(*args)
     assert c.kv.attend_shaped(0, q[:0], [], []).shape == (0, 256)
     assert torch.equal(ok, c.kv.attend_shaped(0, q, [0], [19]))
+
+
+def test_large_caps():
+    """A cap that no score comes near leaves plain attention (tanhf keeps its
+    relative accuracy near 0).  Above 1e30 it is refused: s / softcap would fall
+    among the subnormals and softcap * log2(e) pass the largest f32."""
+    rng = np.random.default_rng(77)
+    for fmt in FORMATS:
+        c = Cache(fmt, 2, 128, 8, [40], rng)
+        q = torch.from_numpy(rng.standard_normal((1, 8 * 128)).astype(np.float32)).cuda()
+        for cap in (1e4, 1e15, 1e30):
+            out, ref = c.run([0], [39], q, softcap=cap)
+            close(out, ref)
+        for cap in (1.1e30, 3e38):
+            with pytest.raises(KvError, match="softcap"):
+                c.run([0], [39], q, softcap=cap)
