@@ -639,9 +639,60 @@ int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n
     if (!items.empty()) std::memcpy(kv->casc_buf.data(), items.data(), items.size() * sizeof(ltkv::PrefixItem));
     for (size_t k = 0; k < toks.size(); ++k) {
         kv->casc_buf[item_words + k] = toks[k];
-        kv->casc_buf[item_words + toks.size() + k] = kv->toks_tmp[toks[k]].skip;
+        kv->casc_buf[item_words + toks.size() + k] = kv->toks_tmp[toks[k]].skip * kBlock;
     }
     kv->casc_ntok = toks.size();
+    return (int)items.size();
+}
+
+// A call of prefill chunks alone over a 4-bit cache: every sequence has at least
+// cascade_min_tokens tokens in it, one after the other, the workspace holds all their blocks, and the
+// items (KV head x 128 / group tokens) leave no SMs to split long ones over.
+// Then the pass attends every token's positions, its own block's too, and writes
+// the outputs; nothing is left for the stream-K launch.  (4 x 256 tokens over
+// 2048 of 8 x 128, f16 q: 162 us with the own blocks in a launch of their own,
+// 123 without.)  Fills casc_buf and exp_groups as plan_cascade does, items for no
+// split; returns the number of items, or 0 where the call is not such.
+int plan_whole(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n) {
+    kv->exp_groups.clear();
+    if (kv->cascade_min_tokens == 0 || n < kv->cascade_min_tokens || n > kv->pre_cap) return 0;
+    uint32_t runs = 1;  // a decode step, a sequence a token, is told apart before anything is sorted
+    for (uint32_t i = 1; i < n; ++i) runs += seq[i] != seq[i - 1];
+    if ((uint64_t)runs * kv->cascade_min_tokens > n) return 0;
+    auto& ord = kv->casc_order;
+    ord.resize(n);
+    for (uint32_t i = 0; i < n; ++i) ord[i] = i;
+    auto before = [&](uint32_t a, uint32_t b) {
+        return seq[a] != seq[b] ? seq[a] < seq[b] : pos[a] != pos[b] ? pos[a] < pos[b] : a < b;
+    };
+    if (!std::is_sorted(ord.begin(), ord.end(), before)) std::sort(ord.begin(), ord.end(), before);
+    const uint32_t tpc = (uint32_t)ltkv::prefix_tokens_per_cta((int)kv->group), hkv = kv->cfg.n_kv_heads;
+    std::vector<ltkv::PrefixItem> items;
+    size_t used = 0, longest = 0;
+    for (uint32_t a = 0, b; a < n; a = b) {
+        for (b = a + 1; b < n && seq[ord[b]] == seq[ord[a]];) ++b;
+        const size_t count = pos[ord[b - 1]] / kBlock + 1;  // blocks up to the last token's
+        if (b - a < kv->cascade_min_tokens || used + count > kv->exp_cap) return 0;
+        kv->exp_groups.push_back({(int32_t)seq[ord[a]], (int32_t)used, (int32_t)count});
+        for (uint32_t c0 = a; c0 < b; c0 += tpc) {
+            const uint32_t c1 = std::min(b, c0 + tpc);
+            for (uint32_t h = 0; h < hkv; ++h)
+                items.push_back({(int32_t)used, 0, (int32_t)(pos[ord[c1 - 1]] / kBlock + 1), 0, (int32_t)h,
+                                 (int32_t)c0, (int32_t)(c1 - c0)});
+        }
+        used += count;
+        longest = std::max(longest, count);
+    }
+    if (items.size() * 2 <= (size_t)kv->sm_count && longest >= 2 * 4) return 0;  // plan_cascade would split these
+    const size_t item_words = items.size() * (sizeof(ltkv::PrefixItem) / 4);
+    kv->casc_buf.resize(item_words + 2 * (size_t)n);
+    std::memcpy(kv->casc_buf.data(), items.data(), items.size() * sizeof(ltkv::PrefixItem));
+    for (uint32_t k = 0; k < n; ++k) {
+        kv->casc_buf[item_words + k] = (int32_t)ord[k];
+        kv->casc_buf[item_words + n + k] = (int32_t)pos[ord[k]] + 1;
+    }
+    kv->casc_splits = 1;
+    kv->casc_ntok = n;
     return (int)items.size();
 }
 
@@ -692,7 +743,9 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
     }
     // sets skip of the tokens it covers; Q8_0 tiles are not f16 tensor-core
     // operands (Q4_0 blocks are expanded for it), and the pass does not shape scores
-    const int n_items = kv->fmt == LT_KV_Q8_0 || score ? 0 : plan_cascade(kv, seq, pos, n);
+    int n_items = kv->fmt == LT_KV_Q4_0 && !score && !fused && !gather ? plan_whole(kv, seq, pos, n) : 0;
+    const bool whole = n_items > 0;
+    if (!whole) n_items = kv->fmt == LT_KV_Q8_0 || score ? 0 : plan_cascade(kv, seq, pos, n);
     long long tiles = 0;
     const int piece_cost = kv->fmt == LT_KV_Q4_0 ? ltkv::kQ4PieceCost : 0;
     for (uint32_t i = 0; i < n; ++i) {
@@ -704,13 +757,14 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
     // The kernel writes every token's last table entry itself.  For the
     // highest position of each sequence in the call that entry is read by no
     // other token from the table, so its pending upload is dropped; the
-    // shadow is restored if the launch fails.
+    // shadow is restored if the launch fails.  (Not `whole`: the expansion reads
+    // the tables.)
     kv->fold_tmp.clear();
     if (++kv->fold_epoch == 0) {  // wrapped: start the marks afresh
         std::fill(kv->fold_mark.begin(), kv->fold_mark.end(), 0u);
         kv->fold_epoch = 1;
     }
-    for (uint32_t i = n; i-- > 0;) {
+    for (uint32_t i = whole ? 0 : n; i-- > 0;) {
         if (kv->fold_mark[seq[i]] == kv->fold_epoch && kv->fold_pos[seq[i]] >= pos[i]) continue;
         kv->fold_mark[seq[i]] = kv->fold_epoch;
         kv->fold_pos[seq[i]] = pos[i];
@@ -788,7 +842,9 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
     p.v_new = v;
     p.kv_f32 = kv_dtype == LT_F32;
     int s_plan = -1;
-    if (n <= (uint32_t)ltkv::kInlineTokens) {
+    if (whole) {
+        p.toks = nullptr;  // no stream-K launch
+    } else if (n <= (uint32_t)ltkv::kInlineTokens) {
         p.toks = nullptr;  // descriptors travel in the kernel parameters
         std::memcpy(p.inl, kv->toks_tmp.data(), n * sizeof(ltkv::TokenDesc));
     } else {
@@ -871,6 +927,8 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         pp.pre_o = kv->d_pre_o;
         pp.pre_ml = kv->d_pre_ml;
         pp.split_rows = p.pre_split_rows;
+        pp.out = whole ? out : nullptr;
+        pp.out_f32 = p.out_f32;
         pp.err = kv->d_err;
         if (kv->fmt == LT_KV_Q4_0) {
             // One launch for all groups' blocks; the pass then reads the
@@ -897,13 +955,15 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         kv->launches++;
         kv->cascade_launches++;
     }
-    const cudaError_t le = score ? ltkv::launch_attend_shaped(p, (int)kv->cfg.head_dim, st)
-                                 : ltkv::launch_attend(p, (int)kv->cfg.head_dim, st);
-    if (le != cudaSuccess) {
-        rollback();
-        return fail(kv, LT_E_CUDA, "attention launch: %s", cudaGetErrorString(le));
+    if (!whole) {
+        const cudaError_t le = score ? ltkv::launch_attend_shaped(p, (int)kv->cfg.head_dim, st)
+                                     : ltkv::launch_attend(p, (int)kv->cfg.head_dim, st);
+        if (le != cudaSuccess) {
+            rollback();
+            return fail(kv, LT_E_CUDA, "attention launch: %s", cudaGetErrorString(le));
+        }
+        kv->launches += ltkv::attend_launches(p);
     }
-    kv->launches += ltkv::attend_launches(p);
     if (ev_end) LT_CUDA(kv, cudaEventRecord(ev_end, st));
     if (gather) {
         const PeerGather& pg = kv->peer;

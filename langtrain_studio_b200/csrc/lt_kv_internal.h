@@ -158,7 +158,7 @@ struct PrefixParams {
     int32_t n_blocks;  // blocks in the pool, for LT_BOUNDS_CHECK builds (0: not checked)
     const PrefixItem* items;
     const int32_t* tok_list;  // token indices of the call (into q, pre_o, pre_ml)
-    const int32_t* tok_lim;   // parallel to tok_list: the token attends blocks [0, tok_lim) here
+    const int32_t* tok_lim;   // parallel to tok_list: the token attends positions [0, tok_lim) here
     int32_t n_kv_heads, group;
     const void* q;
     int32_t q_f32;
@@ -166,6 +166,9 @@ struct PrefixParams {
     float* pre_o;
     float* pre_ml;
     int64_t split_rows;  // rows between split slabs of pre_o / pre_ml
+    void* out;           // not null: every token's positions are all attended here, by one split; rows of
+                         // [token][n_heads][head_dim] go to out instead of pre_o, pre_ml
+    int32_t out_f32;
     int32_t* err;
 };
 // Tokens one prefix CTA covers: 128 query rows / group.

@@ -982,8 +982,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
 // The group's shared blocks stream through a 3-stage shared-memory ring, four
 // blocks (64 positions) a step, each (block, head) K and V sub-tile
 // bulk-copied once for all 128 rows.  Per step:
-//   S = Q K^T      tcgen05.mma, A = Q (f16 value, then its f16 residual,
-//                  both accumulating into S: ~22-bit q), B = K, D = S in TMEM;
+//   S = Q K^T      tcgen05.mma, A = Q (f16 value, then, for f32 q, its f16
+//                  residual, both accumulating into S: ~22-bit q), B = K, D = S
+//                  in TMEM;
 //   softmax        thread r reads its S row from TMEM, keeps a running
 //                  maximum m that only moves up by more than 2^8 (so O and l
 //                  are rescaled rarely), writes P = 2^(s*scale - m) as f16
@@ -992,7 +993,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
 //                  D = O in TMEM.
 // The pool's 16 x 64 sub-tiles are already the 128-byte-swizzled K-major (K)
 // and MN-major (V) operand layouts, so the tiles go from the bulk copy
-// straight to the tensor cores.  At the end each row writes (m, l, O).
+// straight to the tensor cores.  At the end each row writes (m, l, O), or, of
+// a call whose every token is attended here whole (p.out), O / l as its output.
 // Every wait is bounded; on a timeout the CTA sets the error flag, drains
 // its copies and still frees its TMEM.  The warp-collective tcgen05 ops
 // (alloc, ld, st, wait, dealloc) are only ever reached by whole warps.
@@ -1043,6 +1045,28 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+    __syncwarp();
+    uint32_t r[64];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
@@ -1188,9 +1212,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
     const int t_item = r / G, hg = r % G;
     const bool live = r < kPreRows && t_item < item.n_tok && t_item < kPreRows / G;
     const int tok = live ? p.tok_list[item.tok_off + t_item] : 0;
-    // Row r attends positions [0, lim) of the item's blocks: the token's own
-    // skip (a prefill chunk's tokens, causally), or all of them.
-    const int lim = live ? p.tok_lim[item.tok_off + t_item] * kBlock : 0x7fffffff;
+    // Row r attends positions [0, lim) of the item's blocks: those of the shared
+    // blocks, or those up to its token (a prefill chunk, causally).
+    const int lim = live ? p.tok_lim[item.tok_off + t_item] : 0x7fffffff;
     if (r < kPreRows) {
         const int qelem = p.q_f32 ? 4 : 2;
         const uint8_t* qrow = static_cast<const uint8_t*>(p.q) + (((size_t)tok * Hkv + item.head) * G + hg) * D * qelem;
@@ -1287,7 +1311,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                     const uint64_t qoff = ((uint64_t)(kk >> 2) * (kPreRows * 128) + (kk & 3) * 32) >> 4;
                     const uint64_t koff = ((uint64_t)(kk >> 2) * HALF_ROWS_BYTES + (kk & 3) * 32) >> 4;
                     umma_f16(tmem + 64 * bb, dq_hi + qoff, dk + koff, idesc_s, kk > 0 ? 1u : 0u);
-                    umma_f16(tmem + 64 * bb, dq_lo + qoff, dk + koff, idesc_s, 1u);
+                    if (p.q_f32) umma_f16(tmem + 64 * bb, dq_lo + qoff, dk + koff, idesc_s, 1u);  // f16 q has none
                 }
                 umma_commit(s_full + 8u * bb);
                 return true;
@@ -1315,30 +1339,26 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             bool w_ok = mbar_wait_bounded(s_full + 8u * bb, (j >> 1) & 1);
             if (!__all_sync(0xffffffffu, w_ok)) { ok = false; break; }
             tc_fence_after();
-            float sv_[64];
-            {
-                float tmp[32];
-                tmem_ld32(tmem + 64 * bb + lane_off, tmp);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) sv_[i] = tmp[i];
-                if (npos > 32) {
-                    tmem_ld32(tmem + 64 * bb + lane_off + 32, tmp);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) sv_[32 + i] = tmp[i];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) sv_[32 + i] = 0.f;
-                }
-            }
+            float sv_[64];  // (columns past npos: whatever an earlier step left, masked below)
+            tmem_ld64(tmem + 64 * bb + lane_off, sv_);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive1(s_free + 8u * bb);  // S buffer bb may be overwritten
             float mx = -INFINITY;
             const int pos0 = (item.blk0 + j * kPreStepBlocks) * kBlock;
+            const int left = min(npos, lim - pos0);  // columns this row attends
+            if (__all_sync(0xffffffffu, left >= 64)) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
-                sv_[i] = i < npos && pos0 + i < lim ? sv_[i] * scale_log2 : -INFINITY;
-                mx = fmaxf(mx, sv_[i]);
+                for (int i = 0; i < 64; ++i) {
+                    sv_[i] *= scale_log2;
+                    mx = fmaxf(mx, sv_[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) {
+                    sv_[i] = i < left ? sv_[i] * scale_log2 : -INFINITY;
+                    mx = fmaxf(mx, sv_[i]);
+                }
             }
             float alpha = 1.f;
             bool rescale = false;
@@ -1401,18 +1421,33 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
         if (ok) {
             tc_fence_after();
             const size_t row = ((size_t)tok * Hkv + item.head) * G + hg + (size_t)item.split * p.split_rows;
+            const float inv = p.out ? 1.f / l_run : 1.f;  // p.out: the token's own position at least counts
+            float* dst = p.out ? static_cast<float*>(p.out) : p.pre_o;
+            const bool half_out = p.out && !p.out_f32;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
                 float o[32];
                 tmem_ld32(tmem_o + lane_off + c0, o);
                 if (live) {
+                    if (half_out) {
+                        uint4* hdst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * D + c0);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4*>(p.pre_o + row * D + c0 + i) =
-                            make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[e] = h2_bits(__floats2half2_rn(o[8 * i + 2 * e] * inv, o[8 * i + 2 * e + 1] * inv));
+                            hdst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<float4*>(dst + row * D + c0 + i) =
+                                make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                    }
                 }
             }
-            if (live) {
+            if (live && !p.out) {
                 p.pre_ml[row * 2] = m_use;
                 p.pre_ml[row * 2 + 1] = l_run;
             }

@@ -582,3 +582,60 @@ def test_offsets_past_32_bits():
         kv.check()
         for o in (out, shaped):
             np.testing.assert_allclose(o.cpu().numpy(), ref, rtol=1e-4, atol=2e-5)
+
+
+@pytest.mark.parametrize("hd,hq,hkv", [(128, 32, 8), (64, 8, 2), (128, 16, 2), (64, 5, 1), (64, 16, 16)])
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.float32, torch.float32), (torch.float16, torch.float16),
+                                             (torch.float16, torch.float32)])
+def test_whole_chunks(hd, hq, hkv, dtype, out_dtype):
+    """Calls of prefill chunks alone, which the pass attends whole: chunks from
+    position 0, behind cached tokens, ends inside a block, tokens out of order
+    and named twice, rows of a tile that no token has."""
+    rng = np.random.default_rng(hd * hq + hkv)
+    t = Twin(hkv, hd, 16 * 260, hq, max_seqs=8, max_batch=2048)
+    for s, n in enumerate((8, 61, 127, 300, 1030, 97)):
+        t.fill(s, n, rng)
+    t.kv.share(4, 6, 600)  # two sequences on one prefix, each with its own chunk
+    t.rows[(0, 6)] = list(t.rows[(0, 4)][:600])
+    t.fill(6, 650, rng)
+    chunks = [[(0, np.arange(8))], [(1, np.arange(61)), (2, np.arange(30, 127))],
+              [(3, np.arange(300)), (4, np.arange(700, 1030)), (0, np.arange(8)), (6, np.arange(560, 650))],
+              [(5, rng.permutation(97)), (4, np.r_[np.arange(1020, 1030), np.arange(1021, 1030)])]]
+    for chunk in chunks:
+        seqs = np.concatenate([np.full(p.size, s) for s, p in chunk])
+        pos = np.concatenate([p for _, p in chunk])
+        q = torch.from_numpy(rng.standard_normal((seqs.size, hq * hd)).astype(np.float32)).cuda().to(dtype)
+        ref = t.attend_ref(0, seqs, pos, q.float().cpu().numpy())
+        guard = torch.full((seqs.size + 2, hq * hd), 7.0, dtype=out_dtype, device="cuda")
+        t.kv.attend(0, q, seqs, pos, out=guard[1:-1])
+        t.kv.check()
+        close(guard[1:-1], ref, out_dtype)
+        assert (guard[0] == 7).all() and (guard[-1] == 7).all()
+
+
+def test_whole_chunks_take_one_pass():
+    """Of a call that the pass attends whole the tables are read by it alone:
+    new blocks' entries are there, launches are its two, and what follows
+    (a decode step, an append) finds everything as after any call."""
+    rng = np.random.default_rng(3)
+    t = Twin(8, 128, 16 * 300, 32, max_seqs=4, max_batch=1024)
+    for s in range(4):
+        t.fill(s, 200 + s, rng)
+    for step in range(2):
+        seqs, pos = np.repeat(np.arange(4), 80), np.concatenate([np.arange(80) + t.kv.len(s) for s in range(4)])
+        cells = t.kv.append_batch(seqs, pos)
+        k, v = t.draw(320, rng)
+        q = rng.standard_normal((320, 32 * 128)).astype(np.float32)
+        for s in range(4):
+            t.add(0, s, k[seqs == s], v[seqs == s])
+        c0, l0 = t.kv.cascade_launches(), t.kv.launch_count()
+        out = t.kv.write_attend(0, *cells, *(torch.from_numpy(a).cuda() for a in (k, v, q)), seqs, pos)
+        assert t.kv.cascade_launches() == c0 + 1
+        assert t.kv.launch_count() - l0 <= 4  # plan, write, expansion, pass
+        close(out, t.attend_ref(0, seqs, pos, q))
+        s1, p1 = np.arange(4), np.array([t.kv.len(s) - 1 for s in range(4)])
+        q1 = rng.standard_normal((4, 32 * 128)).astype(np.float32)
+        close(t.kv.attend(0, torch.from_numpy(q1).cuda(), s1, p1), t.attend_ref(0, s1, p1, q1))
+        for s in range(4):
+            t.check(0, s)
+    t.kv.check()
