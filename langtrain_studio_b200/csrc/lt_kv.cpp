@@ -646,13 +646,13 @@ int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n
 }
 
 // A call of prefill chunks alone over a 4-bit cache: every sequence has at least
-// cascade_min_tokens tokens in it, one after the other, the workspace holds all their blocks, and the
-// items (KV head x 128 / group tokens) leave no SMs to split long ones over.
-// Then the pass attends every token's positions, its own block's too, and writes
-// the outputs; nothing is left for the stream-K launch.  (4 x 256 tokens over
-// 2048 of 8 x 128, f16 q: 162 us with the own blocks in a launch of their own,
-// 123 without.)  Fills casc_buf and exp_groups as plan_cascade does, items for no
-// split; returns the number of items, or 0 where the call is not such.
+// cascade_min_tokens tokens in it, one after the other, the workspace holds all
+// their blocks, and the items (KV head x 128 / group tokens) leave no SMs to
+// split long ones over.  Then the pass attends every token's positions, its own
+// block's too, and writes the outputs; nothing is left for the stream-K launch.
+// (Of 160 us for 4 x 256 tokens over 2048, 8 x 128, the launch for the tokens'
+// own blocks took 30.)  Fills casc_buf and exp_groups as plan_cascade does, items
+// for no split; returns the number of items, or 0 where the call is not such.
 int plan_whole(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n) {
     kv->exp_groups.clear();
     if (kv->cascade_min_tokens == 0 || n < kv->cascade_min_tokens || n > kv->pre_cap) return 0;

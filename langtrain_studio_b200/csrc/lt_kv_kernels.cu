@@ -985,16 +985,21 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
 //   S = Q K^T      tcgen05.mma, A = Q (f16 value, then, for f32 q, its f16
 //                  residual, both accumulating into S: ~22-bit q), B = K, D = S
 //                  in TMEM;
-//   softmax        thread r reads its S row from TMEM, keeps a running
-//                  maximum m that only moves up by more than 2^8 (so O and l
-//                  are rescaled rarely), writes P = 2^(s*scale - m) as f16
-//                  value + residual rows into shared memory;
+//   softmax        two threads a row, one for each 32 columns, read S from
+//                  TMEM, share the row's running maximum m, which only moves
+//                  up by more than 2^8 (so O and l are rescaled rarely), and
+//                  write P = 2^(s*scale - m) as f16 value + residual rows into
+//                  shared memory;
 //   O += P V       tcgen05.mma, A = P (value, then residual), B = V (MN-major),
 //                  D = O in TMEM.
 // The pool's 16 x 64 sub-tiles are already the 128-byte-swizzled K-major (K)
 // and MN-major (V) operand layouts, so the tiles go from the bulk copy
 // straight to the tensor cores.  At the end each row writes (m, l, O), or, of
 // a call whose every token is attended here whole (p.out), O / l as its output.
+// What bounds it: the chain P(j) -> P V and S two steps on -> softmax, ~1.25 us a
+// step of 64 positions where the MMAs alone need ~0.45.  Half the columns a
+// thread gave 1 % (the exponentials are not the bound: without them the time is the
+// same), a fourth stage for f16 q 4 % (it has no place beside an f32 q's residual).
 // Every wait is bounded; on a timeout the CTA sets the error flag, drains
 // its copies and still frees its TMEM.  The warp-collective tcgen05 ops
 // (alloc, ld, st, wait, dealloc) are only ever reached by whole warps.
@@ -1012,19 +1017,28 @@ __device__ __forceinline__ uint32_t f16_idesc(int n, bool b_mn_major) {
     return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
+// Called by a whole converged warp, one elected lane of which issues.  (In a
+// branch that one lane alone takes the compiler cannot hold the operands in
+// uniform registers and moves all of them there for every instruction: the
+// issue, not the tensor cores, then bounds the pass; 4 x 256 tokens over 2048,
+// f16 q: 123 us against 106.)
 __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                 : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar)
+        : "memory");
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -1045,28 +1059,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
-    __syncwarp();
-    uint32_t r[64];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
@@ -1091,16 +1083,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) 
 constexpr int kPreRows = 128;        // tcgen05 M: query rows of a CTA
 constexpr int kPreStepBlocks = 4;    // blocks (16 positions each) per step: N = 64
 constexpr int kPreStages = 3;        // K/V ring: copies run kPreStages - 2 steps ahead of their use
-constexpr int kPreThreads = 192;     // warps 0..3: softmax of rows 32w..32w+31; warp 4: MMA issue; warp 5: copies
+constexpr int kPreThreads = 320;     // warps 0..7: softmax; warp 8: MMA issue; warp 9: copies
+constexpr int kPreMmaWarp = 8, kPreCopyWarp = 9;
 constexpr int kPreTmemCols = 256;    // S buffers at columns 0 and 64, O at 128
 constexpr float kRescaleLog2 = 8.f;  // a row's maximum moves only when it grows by more than this
 
 // Shared-memory layout of the prefix CTA (offsets from a 1024-aligned base):
 // Q value and residual [D/64][128 rows][128 B]; kPreStages K/V stages, each
 // K [D/64][64 rows][128 B] then V alike; two P buffers, each value and
-// residual [128 rows][128 B]; the mbarriers.
+// residual [128 rows][128 B]; the mbarriers; the half rows' maxima
+// [2 buffers][2 halves][128 rows] f32.
 struct PreSmem {
-    uint32_t q_hi, q_lo, stage0, stage_bytes, p0, bars, total;
+    uint32_t q_hi, q_lo, stage0, stage_bytes, p0, bars, maxima, total;
     __host__ __device__ explicit PreSmem(int D) {
         const uint32_t qbytes = (uint32_t)kPreRows * D * 2;
         stage_bytes = (uint32_t)2 * kPreStepBlocks * kBlock * D * 2;
@@ -1109,8 +1103,12 @@ struct PreSmem {
         stage0 = q_lo + qbytes;
         p0 = stage0 + kPreStages * stage_bytes;  // P buffer b: value at p0 + b*2*16K, residual +16K
         bars = p0 + 2 * 2 * kPreRows * 128;
-        total = bars + 256;
+        maxima = bars + 160;
+        total = maxima + 2 * 2 * kPreRows * 4;
     }
+    // Allocated: total and what alignment may take, as far as a CTA can have it.
+    // (Dynamic shared memory starts 1024-aligned here; the kernel checks.)
+    size_t alloc() const { return total + 1024 < 232448u ? total + 1024 : 232448u; }
 };
 
 // mbarrier arrive (count 1) from a thread.
@@ -1130,6 +1128,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* sbase = smem_raw + (base - smem_u32(smem_raw));
     const PreSmem L(D);
+    uint32_t dyn;
+    asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn));
+    if (base + L.total > smem_u32(smem_raw) + dyn) {
+        if (threadIdx.x == 0) atomicOr(p.err, kErrBounds);
+        return;
+    }
     const uint32_t STAGE = L.stage_bytes, KPART = STAGE / 2;
     const PrefixItem item = p.items[blockIdx.x];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -1138,6 +1142,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
     const uint32_t kv_full = base + L.bars, kv_empty = kv_full + 8u * kPreStages;
     const uint32_t s_full = kv_empty + 8u * kPreStages, s_free = s_full + 16u, p_full = s_free + 16u,
                    p_free = p_full + 16u, pv_done = p_free + 16u;
+    const uint32_t pair = base + L.bars + 128;  // 4: the two warps of 32 rows
     uint32_t* tmem_word = reinterpret_cast<uint32_t*>(sbase + L.bars + 8 * (2 * kPreStages + 9));
     if (tid == 0) {
         for (int st = 0; st < kPreStages; ++st) {
@@ -1146,10 +1151,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
         }
         for (int bb = 0; bb < 2; ++bb) {
             mbar_init(s_full + 8u * bb, 1);
-            mbar_init(s_free + 8u * bb, 4);  // one arrival per softmax warp
-            mbar_init(p_full + 8u * bb, 4);
+            mbar_init(s_free + 8u * bb, 8);  // one arrival per softmax warp
+            mbar_init(p_full + 8u * bb, 8);
             mbar_init(p_free + 8u * bb, 1);
         }
+        for (int w = 0; w < 4; ++w) mbar_init(pair + 8u * w, 2);
         mbar_init(pv_done, 1);
         fence_mbar_init();
     }
@@ -1198,7 +1204,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
         ++issued;
     };
     int nxt_ids[kPreStepBlocks] = {};  // ids of the next refill (step kPreStages, ...)
-    if (tid == kPreRows + 32) {
+    if (tid == kPreCopyWarp * 32) {
         for (int j = 0; j < min(kPreStages, n_steps); ++j) {
             int ids[kPreStepBlocks] = {};
             load_ids(j, ids);
@@ -1207,19 +1213,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
         load_ids(kPreStages, nxt_ids);
     }
 
-    // Q rows (warps 0..3): row r = token r / G, head r % G; value and f16 residual
-    const int r = tid;
+    // Q rows (warps 0..7, half a row a thread): row r = token r / G, head r % G; value and f16 residual
+    const int r = tid % kPreRows, half = tid / kPreRows;
     const int t_item = r / G, hg = r % G;
-    const bool live = r < kPreRows && t_item < item.n_tok && t_item < kPreRows / G;
+    const bool live = half < 2 && t_item < item.n_tok && t_item < kPreRows / G;
     const int tok = live ? p.tok_list[item.tok_off + t_item] : 0;
     // Row r attends positions [0, lim) of the item's blocks: those of the shared
     // blocks, or those up to its token (a prefill chunk, causally).
     const int lim = live ? p.tok_lim[item.tok_off + t_item] : 0x7fffffff;
-    if (r < kPreRows) {
+    if (half < 2) {
         const int qelem = p.q_f32 ? 4 : 2;
         const uint8_t* qrow = static_cast<const uint8_t*>(p.q) + (((size_t)tok * Hkv + item.head) * G + hg) * D * qelem;
 #pragma unroll 1
-        for (int c = 0; c < D / 8; ++c) {
+        for (int c = half * (D / 16); c < (half + 1) * (D / 16); ++c) {
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = 0.f;
@@ -1259,7 +1265,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
 
     bool ok = true;
     int j_fail = 0;
-    if (warp == 5) {
+    if (warp == kPreCopyWarp) {
         // ===== copy producer (one lane): refill a stage once its MMAs have read it =====
         if (lane == 0) {
             for (int j = 0; j + kPreStages < n_steps && ok; ++j) {
@@ -1275,62 +1281,68 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                 atomicOr(p.err, kErrTimeout);
             }
         }
-    } else if (warp == 4) {
-        // ===== MMA issuer (one lane) =====
-        if (lane == 0) {
-            // descriptors: the start-address field is the low 14 bits (address >> 4),
-            // so offsets inside shared memory are added to a base descriptor
-            const uint64_t dq_hi = sw128_desc(base + L.q_hi, 16, 1024), dq_lo = sw128_desc(base + L.q_lo, 16, 1024);
-            const uint64_t dp0 = sw128_desc(base + L.p0, 16, 1024);
-            const uint32_t idesc_pv = f16_idesc(D, true);
-            auto issue_pv = [&](int j) {  // O += P(j) V(j), then free its stage and P buffer
-                const int st = j % kPreStages, bb = j & 1;
-                const int nblk = step_blocks(j);
-                const uint64_t dv = sw128_desc(base + L.stage0 + st * STAGE + KPART, HALF_ROWS_BYTES, 1024);
-                const uint64_t dp = dp0 + ((uint64_t)(bb * PBUF) >> 4);
-                for (int ks = 0; ks < nblk; ++ks) {
-                    const uint64_t bdesc = dv + ((uint64_t)(ks * (kBlock * 128)) >> 4);
-                    umma_f16(tmem_o, dp + (uint64_t)(ks * 2), bdesc, idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
-                    umma_f16(tmem_o, dp + ((uint64_t)(kPreRows * 128 + ks * 32) >> 4), bdesc, idesc_pv, 1u);
-                }
-                umma_commit(kv_empty + 8u * st);
-                umma_commit(p_free + 8u * bb);
-                umma_commit(pv_done);
-            };
-            // S(j) = Q K(j)^T into S buffer j&1, once its copies landed and
-            // softmax(j-2) has read that buffer
-            auto issue_s = [&](int j) -> bool {
-                const int st = j % kPreStages, bb = j & 1;
-                if (!mbar_wait_bounded(kv_full + 8u * st, (j / kPreStages) & 1)) return false;
-                if (j >= 2 && !mbar_wait_bounded(s_free + 8u * bb, ((j - 2) >> 1) & 1)) return false;
-                tc_fence_after();
-                const uint64_t dk = sw128_desc(base + L.stage0 + st * STAGE, 16, 1024);
-                const uint32_t idesc_s = f16_idesc(step_blocks(j) * kBlock, false);
+    } else if (warp == kPreMmaWarp) {
+        // ===== MMA issuer =====
+        // descriptors: the start-address field is the low 14 bits (address >> 4),
+        // so offsets inside shared memory are added to a base descriptor
+        const uint64_t dq_hi = sw128_desc(base + L.q_hi, 16, 1024), dq_lo = sw128_desc(base + L.q_lo, 16, 1024);
+        const uint64_t dp0 = sw128_desc(base + L.p0, 16, 1024);
+        const uint32_t idesc_pv = f16_idesc(D, true);
+        auto wait_all = [](uint32_t bar, uint32_t parity) {
+            return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0;
+        };
+        auto issue_pv = [&](int j) {  // O += P(j) V(j), then free its stage and P buffer
+            const int st = j % kPreStages, bb = j & 1;
+            const int nblk = step_blocks(j);
+            const uint64_t dv = sw128_desc(base + L.stage0 + st * STAGE + KPART, HALF_ROWS_BYTES, 1024);
+            const uint64_t dp = dp0 + ((uint64_t)(bb * PBUF) >> 4);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint64_t qoff = ((uint64_t)(kk >> 2) * (kPreRows * 128) + (kk & 3) * 32) >> 4;
-                    const uint64_t koff = ((uint64_t)(kk >> 2) * HALF_ROWS_BYTES + (kk & 3) * 32) >> 4;
-                    umma_f16(tmem + 64 * bb, dq_hi + qoff, dk + koff, idesc_s, kk > 0 ? 1u : 0u);
-                    if (p.q_f32) umma_f16(tmem + 64 * bb, dq_lo + qoff, dk + koff, idesc_s, 1u);  // f16 q has none
-                }
-                umma_commit(s_full + 8u * bb);
-                return true;
-            };
-            // The tensor cores run S two steps ahead of P V: S(0), S(1), PV(0),
-            // S(2), PV(1), ... so softmax(j+1) never waits on PV(j).
-            for (int j = 0; j < min(2, n_steps) && ok; ++j) ok = issue_s(j);
-            for (int j = 0; j < n_steps && ok; ++j) {
-                ok = mbar_wait_bounded(p_full + 8u * (j & 1), (j >> 1) & 1);
-                if (!ok) { j_fail = j; break; }
-                tc_fence_after();
-                issue_pv(j);
-                if (j + 2 < n_steps && !(ok = issue_s(j + 2))) { j_fail = j; break; }
+            for (int ks = 0; ks < kPreStepBlocks; ++ks) {
+                if (ks >= nblk) break;
+                const uint64_t bdesc = dv + ((uint64_t)(ks * (kBlock * 128)) >> 4);
+                umma_f16(tmem_o, dp + (uint64_t)(ks * 2), bdesc, idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
+                umma_f16(tmem_o, dp + ((uint64_t)(kPreRows * 128 + ks * 32) >> 4), bdesc, idesc_pv, 1u);
             }
-            if (!ok) atomicOr(p.err, kErrTimeout);
+            umma_commit(kv_empty + 8u * st);
+            umma_commit(p_free + 8u * bb);
+            umma_commit(pv_done);
+        };
+        // S(j) = Q K(j)^T into S buffer j&1, once its copies landed and
+        // softmax(j-2) has read that buffer
+        auto issue_s = [&](int j) -> bool {
+            const int st = j % kPreStages, bb = j & 1;
+            if (!wait_all(kv_full + 8u * st, (j / kPreStages) & 1)) return false;
+            if (j >= 2 && !wait_all(s_free + 8u * bb, ((j - 2) >> 1) & 1)) return false;
+            tc_fence_after();
+            const uint64_t dk = sw128_desc(base + L.stage0 + st * STAGE, 16, 1024);
+            const uint32_t idesc_s = f16_idesc(step_blocks(j) * kBlock, false);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                const uint64_t qoff = ((uint64_t)(kk >> 2) * (kPreRows * 128) + (kk & 3) * 32) >> 4;
+                const uint64_t koff = ((uint64_t)(kk >> 2) * HALF_ROWS_BYTES + (kk & 3) * 32) >> 4;
+                umma_f16(tmem + 64 * bb, dq_hi + qoff, dk + koff, idesc_s, kk > 0 ? 1u : 0u);
+                if (p.q_f32) umma_f16(tmem + 64 * bb, dq_lo + qoff, dk + koff, idesc_s, 1u);  // f16 q has none
+            }
+            umma_commit(s_full + 8u * bb);
+            return true;
+        };
+        // The tensor cores run S two steps ahead of P V: S(0), S(1), PV(0),
+        // S(2), PV(1), ... so softmax(j+1) never waits on PV(j).
+        for (int j = 0; j < min(2, n_steps) && ok; ++j) ok = issue_s(j);
+        for (int j = 0; j < n_steps && ok; ++j) {
+            ok = wait_all(p_full + 8u * (j & 1), (j >> 1) & 1);
+            if (!ok) { j_fail = j; break; }
+            tc_fence_after();
+            issue_pv(j);
+            if (j + 2 < n_steps && !(ok = issue_s(j + 2))) { j_fail = j; break; }
         }
+        if (!ok && lane == 0) atomicOr(p.err, kErrTimeout);
     } else {
-        // ===== softmax warps: thread r owns query row r (TMEM lane r) =====
-        const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+        // ===== softmax warps: a thread takes half the columns of query row r
+        // (TMEM lane r), warps w and w + 4 the halves of the same rows =====
+        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t my_pair = pair + 8u * (warp & 3);
+        float* maxima = reinterpret_cast<float*>(sbase + L.maxima);
         const float scale_log2 = p.scale_log2;
         float m_use = -INFINITY, l_run = 0.f;
         for (int j = 0; j < n_steps; ++j) {
@@ -1339,27 +1351,34 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             bool w_ok = mbar_wait_bounded(s_full + 8u * bb, (j >> 1) & 1);
             if (!__all_sync(0xffffffffu, w_ok)) { ok = false; break; }
             tc_fence_after();
-            float sv_[64];  // (columns past npos: whatever an earlier step left, masked below)
-            tmem_ld64(tmem + 64 * bb + lane_off, sv_);
+            float sv_[32];  // (columns past npos: whatever an earlier step left, masked below)
+            tmem_ld32(tmem + 64 * bb + lane_off + 32 * half, sv_);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive1(s_free + 8u * bb);  // S buffer bb may be overwritten
             float mx = -INFINITY;
             const int pos0 = (item.blk0 + j * kPreStepBlocks) * kBlock;
-            const int left = min(npos, lim - pos0);  // columns this row attends
-            if (__all_sync(0xffffffffu, left >= 64)) {
+            const int left = min(npos, lim - pos0) - 32 * half;  // columns of this half that the row attends
+            if (__all_sync(0xffffffffu, left >= 32)) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {
+                for (int i = 0; i < 32; ++i) {
                     sv_[i] *= scale_log2;
                     mx = fmaxf(mx, sv_[i]);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {
+                for (int i = 0; i < 32; ++i) {
                     sv_[i] = i < left ? sv_[i] * scale_log2 : -INFINITY;
                     mx = fmaxf(mx, sv_[i]);
                 }
             }
+            // the row's maximum over both halves
+            maxima[(bb * 2 + half) * kPreRows + r] = mx;
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(my_pair);
+            w_ok = mbar_wait_bounded(my_pair, j & 1);
+            if (!__all_sync(0xffffffffu, w_ok)) { ok = false; break; }
+            mx = fmaxf(mx, maxima[(bb * 2 + 1 - half) * kPreRows + r]);
             float alpha = 1.f;
             bool rescale = false;
             if (mx > m_use + kRescaleLog2 || m_use == -INFINITY) {
@@ -1379,7 +1398,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                 if (!__all_sync(0xffffffffu, w_ok)) { ok = false; break; }
                 tc_fence_after();
 #pragma unroll 1
-                for (int c0 = 0; c0 < D; c0 += 32) {
+                for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
                     float o[32];
                     tmem_ld32(tmem_o + lane_off + c0, o);
 #pragma unroll
@@ -1393,11 +1412,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             const float m_ref = m_use == -INFINITY ? 0.f : m_use;
             float lsum = 0.f;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
+            for (int cc = 0; cc < 4; ++cc) {
+                const int c = 4 * half + cc;
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float p0 = ex2(sv_[8 * c + 2 * e] - m_ref), p1 = ex2(sv_[8 * c + 2 * e + 1] - m_ref);
+                    const float p0 = ex2(sv_[8 * cc + 2 * e] - m_ref), p1 = ex2(sv_[8 * cc + 2 * e + 1] - m_ref);
                     lsum += p0 + p1;
                     const __half2 h = __floats2half2_rn(p0, p1);
                     const float2 hf = __half22float2(h);
@@ -1418,6 +1438,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             const bool w_ok = mbar_wait_bounded(pv_done, (n_steps - 1) & 1);
             ok = __all_sync(0xffffffffu, w_ok);
         }
+        if (ok && n_steps > 0) {  // the row's sum over both halves, through the P buffers, now free
+            float* sums = reinterpret_cast<float*>(sbase + L.p0);
+            sums[half * kPreRows + r] = l_run;
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(my_pair);
+            const bool w_ok = mbar_wait_bounded(my_pair, n_steps & 1);
+            ok = __all_sync(0xffffffffu, w_ok);
+            l_run = sums[r] + sums[kPreRows + r];
+        }
         if (ok) {
             tc_fence_after();
             const size_t row = ((size_t)tok * Hkv + item.head) * G + hg + (size_t)item.split * p.split_rows;
@@ -1425,7 +1454,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             float* dst = p.out ? static_cast<float*>(p.out) : p.pre_o;
             const bool half_out = p.out && !p.out_f32;
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
+            for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
                 float o[32];
                 tmem_ld32(tmem_o + lane_off + c0, o);
                 if (live) {
@@ -1447,7 +1476,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                     }
                 }
             }
-            if (live && !p.out) {
+            if (live && !p.out && half == 0) {
                 p.pre_ml[row * 2] = m_use;
                 p.pre_ml[row * 2 + 1] = l_run;
             }
@@ -1764,7 +1793,7 @@ cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, cuda
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     static bool attr[64][2] = {};
-    const size_t smem = PreSmem(head_dim).total + 1024;  // + alignment slack
+    const size_t smem = PreSmem(head_dim).alloc();
     const int hi = head_dim == 64 ? 0 : 1;
     if (!attr[dev][hi]) {
         e = head_dim == 64
