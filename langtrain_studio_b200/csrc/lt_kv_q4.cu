@@ -39,13 +39,15 @@ __device__ __forceinline__ float q4_scale(float top, float low, float& ad) {
 // its error), is the answer or one below it; the border (k + 1/2) * |d| has at
 // most 13 significant bits, so comparing xs with it in f32 settles which.  Adding
 // 1.5 * 2^23 rounds to an integer and leaves it in the last bits.  NaN, or d = 0:
-// code 8.
+// code 8.  PLAIN: no NaN, and |d| a normal f16 within 2^-8 of max|x| / 8, so that
+// no quotient is below -8.1.
+template <bool PLAIN>
 __device__ __forceinline__ uint32_t q4_code(float xs, float ad, float inv) {
     constexpr float kRound = 12582912.f;
-    const float x = fminf(fmaxf(xs, -8.f * ad), 7.f * ad);  // exact bounds: codes 0 and 15
+    const float x = fminf(PLAIN ? xs : fmaxf(xs, -8.f * ad), 7.f * ad);  // exact bounds: codes 0 and 15
     float k = __fadd_rn(__fadd_rn(__fmaf_rn(x, inv, -0.0009765625f), kRound), -kRound);
     if (x >= __fmaf_rn(k, ad, 0.5f * ad)) k += 1.f;
-    k = ad > 0.f && xs == xs ? k : 0.f;
+    if (!PLAIN) k = ad > 0.f && xs == xs ? k : 0.f;
     return __float_as_uint(__fadd_rn(k, kRound + 8.f));
 }
 
@@ -68,8 +70,18 @@ __device__ __forceinline__ float q4_quant(const float (&x)[N], uint32_t (&code)[
     const float d = q4_scale(top, low, ad);
     const float inv = ad > 0.f ? __fdividef(1.0f, ad) : 0.f;
     const bool neg = top >= low;
+    if constexpr (N == 8) {  // rows of a write, which it shortens from 16.2 to 14.9 us (4096 tokens of 8 x 128 f16)
+        float odd = 0.f;  // becomes NaN with a NaN or an infinity among the values
 #pragma unroll
-    for (int i = 0; i < N; ++i) code[i] = q4_code(neg ? -x[i] : x[i], ad, inv);  // (last bytes)
+        for (int i = 0; i < N; ++i) odd = fmaf(x[i], 0.f, odd);
+        if (__all_sync(kFull, odd == odd && ad >= 6.103515625e-5f && fmaxf(top, low) <= 8.f * kQ4MaxScale)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) code[i] = q4_code<true>(neg ? -x[i] : x[i], ad, inv);
+            return d;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) code[i] = q4_code<false>(neg ? -x[i] : x[i], ad, inv);  // (last bytes)
     return d;
 }
 
@@ -117,7 +129,8 @@ __device__ __forceinline__ void load4_f32(const void* base, size_t idx, int in_f
 // the call) therefore meet in a tile image in shared memory, stored 16 bytes a
 // thread.  4096 tokens of 8 x 128 f16 (38 MB, 5.8 us at the copy rate): 23 us byte
 // by byte with four values a lane, 20 through the image, 16 with eight values a
-// lane, which halves what a group's extremes and scale cost.  Instruction issue
+// lane, which halves what a group's extremes and scale cost, 15 with the odd values'
+// steps left to the warps that hold one.  Instruction issue
 // bounds it (the exact codes).
 template <int D>
 __global__ void __launch_bounds__(4 * D) kv_write_q4_kernel(uint8_t* __restrict__ pool_layer,
