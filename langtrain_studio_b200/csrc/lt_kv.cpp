@@ -468,32 +468,36 @@ lt_status check_cells(lt_kv* kv, const int32_t* block, const int32_t* slot, uint
     return LT_OK;
 }
 
-// check_cells and the cells' upload image (cells_tmp) in one pass.  distinct:
-// refuse a cell named twice -- two rows for one cell would race on its bytes, and
-// a 4-bit cell (codes and scale of one row) must not mix two.  Only LT_KV_Q4_0
-// writes ask for it; the other formats' writes keep the order they had.
+// check_cells and the cells' upload image (cells_tmp).  distinct: refuse a cell
+// named twice -- two rows for one cell would race on its bytes, and a 4-bit cell
+// (codes and scale of one row) must not mix two.  Only LT_KV_Q4_0 writes ask for
+// it; the other formats' writes keep the order they had.
 lt_status take_cells(lt_kv* kv, const int32_t* block, const int32_t* slot, uint32_t n, bool distinct) {
     if (n > kv->cfg.max_batch) return fail(kv, LT_E_ARG, "batch of %u tokens exceeds max_batch %u", n, kv->cfg.max_batch);
     kv->cells_tmp.resize(n);
     int2* out = kv->cells_tmp.data();
-    if (distinct && kv->cell_mark.empty()) kv->cell_mark.assign(kv->n_blocks, 0);
+    const uint32_t n_blocks = kv->n_blocks;
+    uint32_t bad = 0;
+    for (uint32_t i = 0; i < n; ++i) {  // (no early exit: the compiler takes several cells at a time)
+        bad |= (uint32_t)((uint32_t)block[i] >= n_blocks) | (uint32_t)((uint32_t)slot[i] >= (uint32_t)kBlock);
+        out[i].x = block[i];
+        out[i].y = slot[i];
+    }
+    if (bad) return check_cells(kv, block, slot, n);
+    if (!distinct) return LT_OK;
+    if (kv->cell_mark.empty()) kv->cell_mark.assign(n_blocks, 0);
     const uint64_t ep = ++kv->cell_epoch << 16;
-    int32_t cur = -1;       // the run's block, and its slots so far
-    uint64_t mask = 0;
-    for (uint32_t i = 0; i < n; ++i) {
-        const int32_t b = block[i], s = slot[i];
-        if (b < 0 || (uint32_t)b >= kv->n_blocks || s < 0 || s >= kBlock)
-            return fail(kv, LT_E_ARG, "cell %u (block %d, slot %d) out of range", i, b, s);
-        out[i] = make_int2(b, s);
-        if (!distinct) continue;
-        if (b != cur) {
-            if (cur >= 0) kv->cell_mark[cur] = ep | mask;
-            cur = b;
-            const uint64_t m = kv->cell_mark[b];
-            mask = (m & ~0xFFFFull) == ep ? m & 0xFFFF : 0;
-        }
-        if (mask >> s & 1) return fail(kv, LT_E_ARG, "cell %u (block %d, slot %d) is named twice", i, b, s);
-        mask |= 1ull << s;
+    for (uint32_t i = 0; i < n;) {  // runs of cells of one block, and the slots the call has named of it
+        const int32_t b = block[i];
+        const uint32_t i0 = i;
+        uint32_t mask = 0;
+        do mask |= 1u << slot[i++];
+        while (i < n && block[i] == b);
+        const uint64_t m = kv->cell_mark[b];
+        const uint32_t seen = (m & ~0xFFFFull) == ep ? (uint32_t)(m & 0xFFFF) : 0;
+        if ((seen & mask) || (uint32_t)__builtin_popcount(mask) != i - i0)
+            return fail(kv, LT_E_ARG, "cells %u .. %u (block %d): one of them is named twice", i0, i - 1, b);
+        kv->cell_mark[b] = ep | seen | mask;
     }
     return LT_OK;
 }

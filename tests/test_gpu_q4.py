@@ -639,3 +639,24 @@ def test_whole_chunks_take_one_pass():
         for s in range(4):
             t.check(0, s)
     t.kv.check()
+
+
+def test_a_cell_named_again_later_is_refused():
+    t = Twin(1, 64, 64, 4, max_seqs=2)
+    t.fill(0, 40, np.random.default_rng(0))
+    b = t.kv.seq_blocks(0)
+    k = torch.zeros((18, 64), device="cuda")
+    for blocks, slots in (([b[0], b[1], b[0]], [3, 3, 3]), ([b[0], b[0], b[1], b[0]], [1, 2, 2, 2]),
+                          ([b[0]] * 17 + [b[1]], list(range(16)) + [5, 0])):
+        with pytest.raises(KvError, match="named twice"):
+            t.kv.write(0, blocks, slots, k[:len(blocks)], k[:len(blocks)])
+    t.check(0, 0)
+    with pytest.raises(KvError, match="out of range"):
+        t.kv.write(0, [b[0], b[0]], [3, 16], k[:2], k[:2])
+    with pytest.raises(KvError, match="out of range"):
+        t.kv.read(0, [b[0], -1], [3, 0])
+    again = [b[1], b[0], b[1], b[0]], [3, 3, 4, 4]  # different slots of blocks that come again
+    t.kv.write(0, *again, k[:4], k[:4])
+    for got in t.kv.read(0, *again):
+        assert not got.any()
+    t.kv.check()
