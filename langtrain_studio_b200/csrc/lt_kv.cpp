@@ -598,7 +598,7 @@ int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n
             size_t covered = P;  // blocks the group's tokens cover
             for (uint32_t k = a; k < b && one_seq; ++k) covered = std::max<size_t>(covered, pos[ord[k]] / kBlock);
             if (P >= (size_t)kCascadeMinBlocks && (!expand || exp_used + covered <= kv->exp_cap)) {
-                if (expand) kv->exp_groups.push_back({(int32_t)root, (int32_t)exp_used, (int32_t)covered});
+                if (expand) kv->exp_groups.push_back({(int32_t)root, (int32_t)exp_used, (int32_t)covered, 0});
                 groups.push_back({expand ? (int32_t)exp_used : (int32_t)root, (int32_t)P, (int32_t)toks.size(), (int32_t)(b - a), one_seq});
                 for (uint32_t k = a; k < b; ++k) {
                     toks.push_back((int32_t)ord[k]);
@@ -657,7 +657,10 @@ int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n
 // (Of 160 us for 4 x 256 tokens over 2048, 8 x 128, the launch for the tokens'
 // own blocks took 30.)  Fills casc_buf and exp_groups as plan_cascade does, items
 // for no split; returns the number of items, or 0 where the call is not such.
-int plan_whole(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n) {
+// shapes: of a shaped call (pos then being the last position a token attends);
+// an item then covers the blocks of its tokens' intervals alone, and the tokens'
+// first and own positions follow their limits in casc_buf.
+int plan_whole(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, const ltkv::ShapeDesc* shapes, uint32_t n) {
     kv->exp_groups.clear();
     if (kv->cascade_min_tokens == 0 || n < kv->cascade_min_tokens || n > kv->pre_cap) return 0;
     uint32_t runs = 1;  // a decode step, a sequence a token, is told apart before anything is sorted
@@ -672,28 +675,47 @@ int plan_whole(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n) 
     if (!std::is_sorted(ord.begin(), ord.end(), before)) std::sort(ord.begin(), ord.end(), before);
     const uint32_t tpc = (uint32_t)ltkv::prefix_tokens_per_cta((int)kv->group), hkv = kv->cfg.n_kv_heads;
     std::vector<ltkv::PrefixItem> items;
-    size_t used = 0, longest = 0;
+    size_t used = 0;
+    int32_t longest = 0;
     for (uint32_t a = 0, b; a < n; a = b) {
         for (b = a + 1; b < n && seq[ord[b]] == seq[ord[a]];) ++b;
-        const size_t count = pos[ord[b - 1]] / kBlock + 1;  // blocks up to the last token's
+        const int32_t last = (int32_t)(pos[ord[b - 1]] / kBlock);  // block of the last position attended
+        // first block of the interval of token ord[k]; past every block if it is empty
+        auto first_block = [&](uint32_t k) {
+            if (!shapes) return 0;
+            const ltkv::ShapeDesc& sd = shapes[ord[k]];
+            return sd.lo > (int32_t)pos[ord[k]] ? last : sd.lo / (int32_t)kBlock;
+        };
+        int32_t first = last;
+        for (uint32_t k = a; k < b; ++k) first = std::min(first, first_block(k));
+        const size_t count = (size_t)(last - first + 1);
         if (b - a < kv->cascade_min_tokens || used + count > kv->exp_cap) return 0;
-        kv->exp_groups.push_back({(int32_t)seq[ord[a]], (int32_t)used, (int32_t)count});
+        kv->exp_groups.push_back({(int32_t)seq[ord[a]], (int32_t)used, (int32_t)count, first});
         for (uint32_t c0 = a; c0 < b; c0 += tpc) {
             const uint32_t c1 = std::min(b, c0 + tpc);
+            const int32_t blk1 = (int32_t)(pos[ord[c1 - 1]] / kBlock) + 1;
+            int32_t blk0 = blk1 - 1;
+            for (uint32_t k = c0; k < c1; ++k) blk0 = std::min(blk0, first_block(k));
+            blk0 = std::max(blk0, first);  // (a chunk of empty intervals alone may lie before the group's first)
+            longest = std::max(longest, blk1 - blk0);
             for (uint32_t h = 0; h < hkv; ++h)
-                items.push_back({(int32_t)used, 0, (int32_t)(pos[ord[c1 - 1]] / kBlock + 1), 0, (int32_t)h,
-                                 (int32_t)c0, (int32_t)(c1 - c0)});
+                items.push_back({(int32_t)used - first, blk0, std::max(blk1, blk0 + 1), 0, (int32_t)h, (int32_t)c0,
+                                 (int32_t)(c1 - c0)});
         }
         used += count;
-        longest = std::max(longest, count);
     }
     if (items.size() * 2 <= (size_t)kv->sm_count && longest >= 2 * 4) return 0;  // plan_cascade would split these
     const size_t item_words = items.size() * (sizeof(ltkv::PrefixItem) / 4);
-    kv->casc_buf.resize(item_words + 2 * (size_t)n);
+    kv->casc_buf.resize(item_words + (shapes ? 4 : 2) * (size_t)n);
     std::memcpy(kv->casc_buf.data(), items.data(), items.size() * sizeof(ltkv::PrefixItem));
+    int32_t* list = kv->casc_buf.data() + item_words;
     for (uint32_t k = 0; k < n; ++k) {
-        kv->casc_buf[item_words + k] = (int32_t)ord[k];
-        kv->casc_buf[item_words + n + k] = (int32_t)pos[ord[k]] + 1;
+        list[k] = (int32_t)ord[k];
+        list[n + k] = (int32_t)pos[ord[k]] + 1;
+        if (shapes) {
+            list[2 * (size_t)n + k] = shapes[ord[k]].lo;
+            list[3 * (size_t)n + k] = shapes[ord[k]].qpos;
+        }
     }
     kv->casc_splits = 1;
     kv->casc_ntok = n;
@@ -746,8 +768,11 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         t.skip = score && kv->shapes_tmp[i].lo <= t.pos ? kv->shapes_tmp[i].lo / kBlock : 0;
     }
     // sets skip of the tokens it covers; Q8_0 tiles are not f16 tensor-core
-    // operands (Q4_0 blocks are expanded for it), and the pass does not shape scores
-    int n_items = kv->fmt == LT_KV_Q4_0 && !score && !fused && !gather ? plan_whole(kv, seq, pos, n) : 0;
+    // operands (Q4_0 blocks are expanded for it), and the pass shapes scores of
+    // calls that it attends whole alone
+    int n_items = 0;
+    if (kv->fmt == LT_KV_Q4_0 && !fused && !gather)
+        n_items = plan_whole(kv, seq, pos, score ? kv->shapes_tmp.data() : nullptr, n);
     const bool whole = n_items > 0;
     if (!whole) n_items = kv->fmt == LT_KV_Q8_0 || score ? 0 : plan_cascade(kv, seq, pos, n);
     long long tiles = 0;
@@ -869,7 +894,9 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         p.shape.scale_log2 = p.scale_log2;
         p.shape.slopes = score->slopes;
         p.shapes = nullptr;
-        if (n <= (uint32_t)ltkv::kInlineTokens) {
+        if (whole) {
+            // the pass reads them from casc_buf
+        } else if (n <= (uint32_t)ltkv::kInlineTokens) {
             std::memcpy(p.inl_shapes, kv->shapes_tmp.data(), n * sizeof(ltkv::ShapeDesc));
         } else {
             const void* d_shapes = nullptr;
@@ -933,6 +960,11 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         pp.split_rows = p.pre_split_rows;
         pp.out = whole ? out : nullptr;
         pp.out_f32 = p.out_f32;
+        if (score) {
+            pp.tok_lo = pp.tok_lim + n;
+            pp.tok_qpos = pp.tok_lo + n;
+            pp.shape = p.shape;
+        }
         pp.err = kv->d_err;
         if (kv->fmt == LT_KV_Q4_0) {
             // One launch for all groups' blocks; the pass then reads the
@@ -951,7 +983,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
             pp.max_blocks = 1;
             pp.n_blocks = (int32_t)kv->exp_cap;
         }
-        const cudaError_t pe = ltkv::launch_prefix(pp, n_items, (int)kv->cfg.head_dim, st);
+        const cudaError_t pe = ltkv::launch_prefix(pp, n_items, (int)kv->cfg.head_dim, score != nullptr, st);
         if (pe != cudaSuccess) {
             rollback();
             return fail(kv, LT_E_CUDA, "prefix launch: %s", cudaGetErrorString(pe));

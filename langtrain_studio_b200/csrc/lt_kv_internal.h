@@ -142,7 +142,8 @@ using AttnParamsOf = typename AttnParamsSel<SH>::type;
 // each K/V tile staged once for all of them, and writes (m, l, O) partials
 // that the stream-K launch folds into the tokens' outputs.
 struct PrefixItem {
-    int32_t root_seq;  // a member whose table row holds the shared blocks
+    int32_t root_seq;  // a member whose table row holds the shared blocks (LT_KV_Q4_0: where block 0 would
+                       // lie in the workspace)
     int32_t blk0;      // this item's part of the shared blocks: [blk0, blk1)
     int32_t blk1;
     int32_t split;     // which partial slab it writes
@@ -169,11 +170,15 @@ struct PrefixParams {
     void* out;           // not null: every token's positions are all attended here, by one split; rows of
                          // [token][n_heads][head_dim] go to out instead of pre_o, pre_ml
     int32_t out_f32;
+    // Shaped scores (launch_prefix's `shaped`; with out alone): parallel to tok_list
+    const int32_t* tok_lo;    // first position attended
+    const int32_t* tok_qpos;  // the token's own position
+    ShapeTerms shape;
     int32_t* err;
 };
 // Tokens one prefix CTA covers: 128 query rows / group.
 inline int prefix_tokens_per_cta(int group) { return 128 / group; }
-cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, cudaStream_t s);
+cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, bool shaped, cudaStream_t s);
 
 // Warps of one attention launch on `device` (all resident at once), or 0.
 // fmt: lt_kv_format of the pool; shaped: the launch is launch_attend_shaped.
@@ -200,10 +205,10 @@ cudaError_t launch_write(uint16_t* pool_layer, const int2* cells, int n, int n_k
 cudaError_t launch_write_q4(uint8_t* pool_layer, const int2* cells, int n, int n_kv_heads, int head_dim, int shift,
                             const void* k, const void* v, int in_f32, cudaStream_t s);
 
-// Blocks [0, count) of sequence root's table, expanded to f16 tiles as blocks
-// base, base + 1, ... of a workspace.
+// Blocks [first, first + count) of sequence root's table, expanded to f16 tiles
+// as blocks base, base + 1, ... of a workspace.
 struct ExpandGroup {
-    int32_t root, base, count;
+    int32_t root, base, count, first;
 };
 constexpr int kExpandGroups = 128;  // groups of one launch (kernel parameters)
 cudaError_t launch_expand_q4(const uint8_t* pool_layer, const int32_t* tables, int max_blocks, const ExpandGroup* groups,

@@ -994,7 +994,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
 //                  D = O in TMEM.
 // The pool's 16 x 64 sub-tiles are already the 128-byte-swizzled K-major (K)
 // and MN-major (V) operand layouts, so the tiles go from the bulk copy
-// straight to the tensor cores.  At the end each row writes (m, l, O), or, of
+// straight to the tensor cores.  SH: scores of lt_kv_score, of 4-bit caches alone,
+// whose masked cells hold no Inf or NaN that 0 * V could spread.  At the end each row writes (m, l, O), or, of
 // a call whose every token is attended here whole (p.out), O / l as its output.
 // What bounds it: the chain P(j) -> P V and S two steps on -> softmax, ~1.25 us a
 // step of 64 positions where the MMAs alone need ~0.45.  Half the columns a
@@ -1116,7 +1117,7 @@ __device__ __forceinline__ void mbar_arrive1(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-template <int D>
+template <int D, bool SH>
 __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
     // The decode launch that folds these partials in may start on the SMs
     // this launch leaves free; it waits for this grid before the fold.
@@ -1174,7 +1175,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
 
     const int nbk = item.blk1 - item.blk0;  // >= 1: the host gives every split at least one step
     const int n_steps = (nbk + kPreStepBlocks - 1) / kPreStepBlocks;
-    const int32_t* trow = p.tables + (size_t)item.root_seq * p.max_blocks + item.blk0;
+    const int32_t* trow = p.tables + (int64_t)item.root_seq * p.max_blocks + item.blk0;
     const size_t tile_elems = 2 * kBlock * D;
     auto step_blocks = [&](int j) { return min(kPreStepBlocks, nbk - j * kPreStepBlocks); };
     int issued = 0;  // warp 5 lane 0: steps whose copies were issued
@@ -1344,6 +1345,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
         const uint32_t my_pair = pair + 8u * (warp & 3);
         float* maxima = reinterpret_cast<float*>(sbase + L.maxima);
         const float scale_log2 = p.scale_log2;
+        int lo = 0, qpos = 0;  // SH: the row attends [lo, lim), and its own position
+        float slope = 0.f;
+        if (SH && live) {
+            lo = p.tok_lo[item.tok_off + t_item];
+            qpos = p.tok_qpos[item.tok_off + t_item];
+            if (p.shape.slopes) slope = __ldg(p.shape.slopes + item.head * G + hg) * kLog2e;
+        }
         float m_use = -INFINITY, l_run = 0.f;
         for (int j = 0; j < n_steps; ++j) {
             const int bb = j & 1;
@@ -1359,7 +1367,29 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             float mx = -INFINITY;
             const int pos0 = (item.blk0 + j * kPreStepBlocks) * kBlock;
             const int left = min(npos, lim - pos0) - 32 * half;  // columns of this half that the row attends
-            if (__all_sync(0xffffffffu, left >= 32)) {
+            if constexpr (SH) {
+                // TileShape's score, a term at a time over all columns: the branches
+                // are the call's (4 x 256 tokens over 2048 without a term: 109 us
+                // from 219 with every term in one loop; cap and window 89 from 138)
+                const int at = pos0 + 32 * half, q_off = qpos - at, from = lo - at;
+                if (p.shape.capped) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sv_[i] = p.shape.cap_log2 * tanhf(sv_[i] * p.shape.scale_cap);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sv_[i] *= scale_log2;
+                }
+                if (p.shape.slopes) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sv_[i] -= slope * (float)abs(q_off - i);
+                }
+                if (!__all_sync(0xffffffffu, left >= 32 && from <= 0)) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sv_[i] = i < left && i >= from ? sv_[i] : -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, sv_[i]);
+            } else if (__all_sync(0xffffffffu, left >= 32)) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     sv_[i] *= scale_log2;
@@ -1450,7 +1480,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
         if (ok) {
             tc_fence_after();
             const size_t row = ((size_t)tok * Hkv + item.head) * G + hg + (size_t)item.split * p.split_rows;
-            const float inv = p.out ? 1.f / l_run : 1.f;  // p.out: the token's own position at least counts
+            // p.out: the token's own position at least counts, or (SH) its interval is empty
+            const float inv = !p.out ? 1.f : SH && lo >= lim ? 0.f : 1.f / l_run;
             float* dst = p.out ? static_cast<float*>(p.out) : p.pre_o;
             const bool half_out = p.out && !p.out_f32;
 #pragma unroll 1
@@ -1786,27 +1817,27 @@ cudaError_t launch_attend_shaped(const AttnShapedParams& p, int head_dim, cudaSt
 
 int attend_launches(const AttnParams& p) { return p.n_warps == 0 ? 0 : 1; }
 
-cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, cudaStream_t s) {
-    if (n_items <= 0) return cudaSuccess;
+template <int D, bool SH>
+cudaError_t launch_prefix_d(const PrefixParams& p, int n_items, cudaStream_t s) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    static bool attr[64][2] = {};
-    const size_t smem = PreSmem(head_dim).alloc();
-    const int hi = head_dim == 64 ? 0 : 1;
-    if (!attr[dev][hi]) {
-        e = head_dim == 64
-                ? cudaFuncSetAttribute(prefix_attn_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
-                : cudaFuncSetAttribute(prefix_attn_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static bool attr[64] = {};
+    const size_t smem = PreSmem(D).alloc();
+    if (!attr[dev]) {
+        e = cudaFuncSetAttribute(prefix_attn_kernel<D, SH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
-        attr[dev][hi] = true;
+        attr[dev] = true;
     }
-    if (head_dim == 64)
-        prefix_attn_kernel<64><<<n_items, kPreThreads, smem, s>>>(p);
-    else
-        prefix_attn_kernel<128><<<n_items, kPreThreads, smem, s>>>(p);
+    prefix_attn_kernel<D, SH><<<n_items, kPreThreads, smem, s>>>(p);
     return cudaGetLastError();
+}
+
+cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, bool shaped, cudaStream_t s) {
+    if (n_items <= 0) return cudaSuccess;
+    if (shaped) return head_dim == 64 ? launch_prefix_d<64, true>(p, n_items, s) : launch_prefix_d<128, true>(p, n_items, s);
+    return head_dim == 64 ? launch_prefix_d<64, false>(p, n_items, s) : launch_prefix_d<128, false>(p, n_items, s);
 }
 
 cudaError_t launch_gather_permute(const void* gathered, void* out, int nranks, uint32_t n, size_t row_bytes,

@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(256) expand_q4_kernel(const __grid_constant__ 
     }
     const ExpandGroup gr = p.groups[lo];
     const int i = b - p.first[lo];
-    const int src = checked_block(__ldg(p.tables + (size_t)gr.root * p.max_blocks + i), p.n_blocks, p.err);
+    const int src = checked_block(__ldg(p.tables + (size_t)gr.root * p.max_blocks + gr.first + i), p.n_blocks, p.err);
     const uint8_t* tile = p.pool + ((size_t)src * p.n_kv_heads + h) * q4_tile_bytes(D);
     uint16_t* out = p.out + ((size_t)(gr.base + i) * p.n_kv_heads + h) * (2 * kBlock * D);
     q4_part_values<D>(tile, part, lane, [&](int kvsel, int slot, int c, uint4 x) {

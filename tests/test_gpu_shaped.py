@@ -214,3 +214,55 @@ def test_large_caps():
         for cap in (1.1e30, 3e38):
             with pytest.raises(KvError, match="softcap"):
                 c.run([0], [39], q, softcap=cap)
+
+
+@pytest.mark.parametrize("hd,hq,hkv", [(128, 32, 8), (64, 16, 16), (64, 6, 2)])
+@pytest.mark.parametrize("terms", ["nothing", "window", "all", "documents", "prefix"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_chunks_over_the_4_bit_cache(hd, hq, hkv, terms, dtype):
+    """Prefill chunks with shaped scores, which the tensor-core pass attends whole
+    over the blocks of their intervals: windows and documents that start inside a
+    block, empty intervals (alone in a 128-row tile too), ends past the token."""
+    rng = np.random.default_rng(hd + hq + len(terms))
+    lens = [300, 61, 700, 8]
+    c = Cache("q4_0", hkv, hd, hq, lens, rng)
+    seqs = np.concatenate([np.full(260, 0), np.full(61, 1), np.full(330, 2), np.full(8, 3)])
+    pos = np.concatenate([np.arange(40, 300), np.arange(61), np.arange(370, 700), np.arange(8)])
+    shape = {}
+    if terms == "window":
+        shape = dict(window=50)
+    elif terms == "all":
+        shape = dict(softcap=20.0, window=130, slopes=slopes_of(hq))
+    elif terms == "documents":
+        first = pos // 90 * 90
+        end = pos + 1
+        first[(seqs == 2) & (pos < 520)] = 600  # empty: they start past their end
+        shape = dict(first=first, end=end, slopes=slopes_of(hq))
+    elif terms == "prefix":
+        shape = dict(end=np.minimum(np.array(lens)[seqs], np.maximum(pos + 1, 200)), softcap=5.0)
+    q = torch.from_numpy(rng.standard_normal((seqs.size, hq * hd)).astype(np.float32)).cuda().to(dtype)
+    c0 = c.kv.cascade_launches()
+    out, ref = c.run(seqs, pos, q, dtype, **shape)
+    close(out, ref, dtype)
+    if hkv > 2:  # enough tiles for the device (groups of 3 on 2 heads leave most of it free)
+        assert c.kv.cascade_launches() == c0 + 1
+    if terms == "documents":
+        assert not out[torch.from_numpy((seqs == 2) & (pos < 520)).cuda()].any()
+    # the same tokens in another order give the same rows
+    mix = np.concatenate([rng.permutation(260) + 260 * 0, 321 + rng.permutation(330), 260 + rng.permutation(61)])
+    part = {k: (v[mix] if k in ("first", "end") else v) for k, v in shape.items()}
+    out2, ref2 = c.run(seqs[mix], pos[mix], q[torch.from_numpy(mix).cuda()].contiguous(), dtype, **part)
+    close(out2, ref2, dtype)
+
+
+def test_short_chunks_over_the_4_bit_cache():
+    """Chunks whose intervals are short are attended whole however few they are."""
+    rng = np.random.default_rng(5)
+    c = Cache("q4_0", 1, 128, 4, [2000], rng)
+    pos = np.arange(1500, 1520)
+    q = torch.from_numpy(rng.standard_normal((20, 512)).astype(np.float32)).cuda()
+    for window in (1, 16, 17, 60, 1000):
+        c0 = c.kv.cascade_launches()
+        out, ref = c.run(np.zeros(20, int), pos, q, window=window)
+        close(out, ref)
+        assert c.kv.cascade_launches() == c0 + (window < 1000)
