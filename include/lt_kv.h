@@ -357,7 +357,7 @@ lt_status lt_kv_set_min_tiles_per_warp(lt_kv* kv, uint32_t tiles);
  * call over an f16 cache.  An LT_KV_Q4_0 cache expands the shared blocks into an f16 workspace
  * first (128 MiB at most, allocated with the handle); groups that do not fit
  * it go through the decode launch.  A call over such a cache whose every
- * sequence has min_group_tokens tokens in it, one after the other (prefill
+ * sequence has min_group_tokens (and 8) tokens in it, one after the other (prefill
  * chunks; shaped or not), is attended by the pass alone, without a decode
  * launch, where its CTAs suffice to fill the device or its sequences are short. */
 lt_status lt_kv_set_cascade(lt_kv* kv, uint32_t min_group_tokens);

@@ -31,6 +31,7 @@ constexpr int kSlots = 8;  // staging ring depth (pinned host + device pairs)
 constexpr uint32_t kCascadeMaxTokens = 1024;  // tokens of one call the prefix pass serves
 constexpr int kCascadeMinBlocks = 4;          // shortest shared prefix worth a pass (64 positions)
 constexpr size_t kExpandBytes = 128u << 20;   // f16 workspace of a 4-bit cache's prefix pass
+constexpr uint32_t kWholeMinTokens = 8;       // tokens of a sequence in a call that the prefix pass attends whole
 constexpr long long kSmallTiles = 1184;       // tiles of an attention call that counts as small
 constexpr uint32_t kClean = 0xFFFFFFFFu;
 
@@ -650,22 +651,24 @@ int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n
 }
 
 // A call of prefill chunks alone over a 4-bit cache: every sequence has at least
-// cascade_min_tokens tokens in it, one after the other, the workspace holds all
-// their blocks, and the items (KV head x 128 / group tokens) leave no SMs to
-// split long ones over.  Then the pass attends every token's positions, its own
-// block's too, and writes the outputs; nothing is left for the stream-K launch.
-// (Of 160 us for 4 x 256 tokens over 2048, 8 x 128, the launch for the tokens'
-// own blocks took 30.)  Fills casc_buf and exp_groups as plan_cascade does, items
-// for no split; returns the number of items, or 0 where the call is not such.
+// cascade_min_tokens tokens in it (and kWholeMinTokens: fewer would leave the
+// pass's 128 rows empty), one after the other, the workspace holds all their
+// blocks, and the items (KV head x 128 / group tokens) leave no SMs to split long
+// ones over.  Then the pass attends every token's positions, its own block's too,
+// and writes the outputs; nothing is left for the stream-K launch.  (Of 160 us for
+// 4 x 256 tokens over 2048, 8 x 128, the launch for the tokens' own blocks took 30.)
+// Fills casc_buf and exp_groups as plan_cascade does, items for no split; returns
+// the number of items, or 0 where the call is not such.
 // shapes: of a shaped call (pos then being the last position a token attends);
 // an item then covers the blocks of its tokens' intervals alone, and the tokens'
 // first and own positions follow their limits in casc_buf.
 int plan_whole(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, const ltkv::ShapeDesc* shapes, uint32_t n) {
     kv->exp_groups.clear();
-    if (kv->cascade_min_tokens == 0 || n < kv->cascade_min_tokens || n > kv->pre_cap) return 0;
+    const uint32_t least = std::max(kv->cascade_min_tokens, kWholeMinTokens);
+    if (kv->cascade_min_tokens == 0 || n < least || n > kv->pre_cap) return 0;
     uint32_t runs = 1;  // a decode step, a sequence a token, is told apart before anything is sorted
     for (uint32_t i = 1; i < n; ++i) runs += seq[i] != seq[i - 1];
-    if ((uint64_t)runs * kv->cascade_min_tokens > n) return 0;
+    if ((uint64_t)runs * least > n) return 0;
     auto& ord = kv->casc_order;
     ord.resize(n);
     for (uint32_t i = 0; i < n; ++i) ord[i] = i;
@@ -689,7 +692,7 @@ int plan_whole(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, const ltkv::
         int32_t first = last;
         for (uint32_t k = a; k < b; ++k) first = std::min(first, first_block(k));
         const size_t count = (size_t)(last - first + 1);
-        if (b - a < kv->cascade_min_tokens || used + count > kv->exp_cap) return 0;
+        if (b - a < least || used + count > kv->exp_cap) return 0;
         kv->exp_groups.push_back({(int32_t)seq[ord[a]], (int32_t)used, (int32_t)count, first});
         for (uint32_t c0 = a; c0 < b; c0 += tpc) {
             const uint32_t c1 = std::min(b, c0 + tpc);

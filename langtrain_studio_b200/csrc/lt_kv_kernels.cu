@@ -995,8 +995,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
 // The pool's 16 x 64 sub-tiles are already the 128-byte-swizzled K-major (K)
 // and MN-major (V) operand layouts, so the tiles go from the bulk copy
 // straight to the tensor cores.  SH: scores of lt_kv_score, of 4-bit caches alone,
-// whose masked cells hold no Inf or NaN that 0 * V could spread.  At the end each row writes (m, l, O), or, of
-// a call whose every token is attended here whole (p.out), O / l as its output.
+// whose masked cells hold no Inf or NaN that 0 * V could spread.  At the end each
+// row writes (m, l, O), or, of a call whose every token is attended here whole
+// (p.out), O / l as its output.
 // What bounds it: the chain P(j) -> P V and S two steps on -> softmax, ~1.25 us a
 // step of 64 positions where the MMAs alone need ~0.45.  Half the columns a
 // thread gave 1 % (the exponentials are not the bound: without them the time is the

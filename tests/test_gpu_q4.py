@@ -660,3 +660,20 @@ def test_a_cell_named_again_later_is_refused():
     for got in t.kv.read(0, *again):
         assert not got.any()
     t.kv.check()
+
+
+def test_short_runs_are_not_attended_whole():
+    """Fewer than 8 tokens a sequence stay with the decode launch, whatever set_cascade says."""
+    rng = np.random.default_rng(8)
+    t = Twin(8, 128, 16 * 200, 32, max_seqs=20)
+    for s in range(20):
+        t.fill(s, 100 + s, rng)
+    seqs = np.repeat(np.arange(20), 3)
+    pos = np.array([t.kv.len(s) - 1 for s in seqs]) - np.tile([2, 1, 0], 20)
+    q = rng.standard_normal((60, 32 * 128)).astype(np.float32)
+    ref = t.attend_ref(0, seqs, pos, q)
+    t.kv.set_cascade(4)
+    c0 = t.kv.cascade_launches()
+    close(t.kv.attend(0, torch.from_numpy(q).cuda(), seqs, pos), ref)
+    assert t.kv.cascade_launches() == c0
+    t.kv.check()
