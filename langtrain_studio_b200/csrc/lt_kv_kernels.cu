@@ -990,8 +990,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
 //                  up by more than 2^8 (so O and l are rescaled rarely), and
 //                  write P = 2^(s*scale - m) as f16 value + residual rows into
 //                  shared memory;
-//   O += P V       tcgen05.mma, A = P (value, then residual), B = V (MN-major),
-//                  D = O in TMEM.
+//   O += P V       tcgen05.mma, A = P's values, B = V (MN-major), D = O in TMEM;
+//                  P's residuals alike into an O of their own, added at the end
+//                  (each accumulation of the tensor core rounds O towards zero).
 // The pool's 16 x 64 sub-tiles are already the 128-byte-swizzled K-major (K)
 // and MN-major (V) operand layouts, so the tiles go from the bulk copy
 // straight to the tensor cores.  SH: scores of lt_kv_score, of 4-bit caches alone,
@@ -1087,7 +1088,8 @@ constexpr int kPreStepBlocks = 4;    // blocks (16 positions each) per step: N =
 constexpr int kPreStages = 3;        // K/V ring: copies run kPreStages - 2 steps ahead of their use
 constexpr int kPreThreads = 320;     // warps 0..7: softmax; warp 8: MMA issue; warp 9: copies
 constexpr int kPreMmaWarp = 8, kPreCopyWarp = 9;
-constexpr int kPreTmemCols = 256;    // S buffers at columns 0 and 64, O at 128
+constexpr int kPreTmemCols = 512;    // S buffers at columns 0 and 64, O at 128, O of P's residuals at 256
+constexpr uint32_t kPreResidualO = 128;  // columns from O to the residuals' O
 constexpr float kRescaleLog2 = 8.f;  // a row's maximum moves only when it grows by more than this
 
 // Shared-memory layout of the prefix CTA (offsets from a 1024-aligned base):
@@ -1303,7 +1305,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                 if (ks >= nblk) break;
                 const uint64_t bdesc = dv + ((uint64_t)(ks * (kBlock * 128)) >> 4);
                 umma_f16(tmem_o, dp + (uint64_t)(ks * 2), bdesc, idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
-                umma_f16(tmem_o, dp + ((uint64_t)(kPreRows * 128 + ks * 32) >> 4), bdesc, idesc_pv, 1u);
+                umma_f16(tmem_o + kPreResidualO, dp + ((uint64_t)(kPreRows * 128 + ks * 32) >> 4), bdesc, idesc_pv,
+                         (j > 0 || ks > 0) ? 1u : 0u);
             }
             umma_commit(kv_empty + 8u * st);
             umma_commit(p_free + 8u * bb);
@@ -1318,12 +1321,17 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             tc_fence_after();
             const uint64_t dk = sw128_desc(base + L.stage0 + st * STAGE, 16, 1024);
             const uint32_t idesc_s = f16_idesc(step_blocks(j) * kBlock, false);
+            // f32 q's residual first, while S is small: the accumulation rounds towards zero
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                const uint64_t qoff = ((uint64_t)(kk >> 2) * (kPreRows * 128) + (kk & 3) * 32) >> 4;
-                const uint64_t koff = ((uint64_t)(kk >> 2) * HALF_ROWS_BYTES + (kk & 3) * 32) >> 4;
-                umma_f16(tmem + 64 * bb, dq_hi + qoff, dk + koff, idesc_s, kk > 0 ? 1u : 0u);
-                if (p.q_f32) umma_f16(tmem + 64 * bb, dq_lo + qoff, dk + koff, idesc_s, 1u);  // f16 q has none
+            for (int part = 0; part < 2; ++part) {
+                if (part == 0 && !p.q_f32) continue;  // f16 q has none
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint64_t qoff = ((uint64_t)(kk >> 2) * (kPreRows * 128) + (kk & 3) * 32) >> 4;
+                    const uint64_t koff = ((uint64_t)(kk >> 2) * HALF_ROWS_BYTES + (kk & 3) * 32) >> 4;
+                    umma_f16(tmem + 64 * bb, (part == 0 ? dq_lo : dq_hi) + qoff, dk + koff, idesc_s,
+                             kk > 0 || (part == 1 && p.q_f32) ? 1u : 0u);
+                }
             }
             umma_commit(s_full + 8u * bb);
             return true;
@@ -1430,11 +1438,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                 tc_fence_after();
 #pragma unroll 1
                 for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
-                    float o[32];
-                    tmem_ld32(tmem_o + lane_off + c0, o);
+#pragma unroll 1
+                    for (uint32_t at = tmem_o + lane_off + c0, n = 0; n < 2; ++n, at += kPreResidualO) {
+                        float o[32];
+                        tmem_ld32(at, o);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] *= alpha;
-                    tmem_st32(tmem_o + lane_off + c0, o);
+                        for (int i = 0; i < 32; ++i) o[i] *= alpha;
+                        tmem_st32(at, o);
+                    }
                 }
             }
             const uint32_t pb = L.p0 + bb * PBUF;
@@ -1487,8 +1498,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             const bool half_out = p.out && !p.out_f32;
 #pragma unroll 1
             for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
-                float o[32];
+                float o[32], o2[32];
                 tmem_ld32(tmem_o + lane_off + c0, o);
+                tmem_ld32(tmem_o + kPreResidualO + lane_off + c0, o2);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] += o2[i];
                 if (live) {
                     if (half_out) {
                         uint4* hdst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * D + c0);

@@ -303,8 +303,8 @@ cudaError_t launch_read_fmt(const uint8_t* pool, const int2* cells, const int32_
 // costs 16 x 8 scheduler cycles of MMA (32 x 8 for larger groups) beside ~290
 // other instructions, ~180 of them the half-rate unpacking, where its 2304 bytes
 // take ~400 scheduler cycles (4 schedulers x 148 SMs) from HBM.  64 sequences of 512
-// to 4096, 32 / 8 heads: 54 us (26 at the copy rate; 0.54 instructions issued a
-// cycle, DRAM 39 %); 16 of 32768, 64 / 8 heads, f16 q: 158 us (92).
+// to 4096, 32 / 8 heads: 55 us (26 at the copy rate; 0.54 instructions issued a
+// cycle, DRAM 39 %); 16 of 32768, 64 / 8 heads, f16 q: 160 us (92).
 //
 // Q16 (f16 q): q has no residual, so PACK's columns 4-7 repeat the values and
 // the scores come out in both halves without an exchange; larger groups take
@@ -1119,24 +1119,34 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
             }
         }
 
-        // O^T += V^T P^T
+        // O^T += V^T P^T.  The MMA's own accumulation rounds towards zero, which over
+        // the ~100 tiles of a range would shrink O by 100 * 2^-25; so the step's
+        // products are summed from zero there and added in f32, to nearest.
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
+        for (int ch = 0; ch < D / 64; ++ch) {
+            uint4 wv[NT], vd[NT];
 #pragma unroll
-            for (int ch = 0; ch < D / 64; ++ch) {
-                const uint4 wv = *reinterpret_cast<const uint4*>(tiles[u] + 8 * D + ch * 512 + lane * 16);
-                const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w};
-                const uint4 vd = *reinterpret_cast<const uint4*>(tiles[u] + 17 * D + (t * G32 + 2 * ch) * 8);
+            for (int u = 0; u < NT; ++u) {
+                wv[u] = *reinterpret_cast<const uint4*>(tiles[u] + 8 * D + ch * 512 + lane * 16);
+                vd[u] = *reinterpret_cast<const uint4*>(tiles[u] + 17 * D + (t * G32 + 2 * ch) * 8);
+            }
 #pragma unroll
-                for (int mm = 0; mm < 4; ++mm) {
-                    const int m = 4 * ch + mm;
-                    const __half2 dA = as_h2(mm < 2 ? vd.x : vd.z), dB = as_h2(mm < 2 ? vd.y : vd.w);
+            for (int mm = 0; mm < 4; ++mm) {
+                const int m = 4 * ch + mm;
+                float tt[4];
+#pragma unroll
+                for (int u = 0; u < NT; ++u) {
+                    const uint32_t w[4] = {wv[u].x, wv[u].y, wv[u].z, wv[u].w};
+                    const __half2 dA = as_h2(mm < 2 ? vd[u].x : vd[u].z), dB = as_h2(mm < 2 ? vd[u].y : vd[u].w);
                     const uint32_t w0 = w[mm], w8 = w0 >> 8;
                     const uint32_t a[4] = {h2_bits(__hmul2(q4_low(w0, magic), dA)), h2_bits(__hmul2(q4_high(w0, magic), dA)),
                                            h2_bits(__hmul2(q4_low(w8, magic), dB)), h2_bits(__hmul2(q4_high(w8, magic), dB))};
-                    mma16816_add(o[m], a, ph[u][0], ph[u][1]);
-                    if constexpr (!PACK) mma16816_add(o[m], a, pl[u][0], pl[u][1]);
+                    if (u == 0) mma16816_zero(tt, a, ph[u][0], ph[u][1]);
+                    else mma16816_add(tt, a, ph[u][0], ph[u][1]);
+                    if constexpr (!PACK) mma16816_add(tt, a, pl[u][0], pl[u][1]);
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[m][e] += tt[e];
             }
         }
     };
