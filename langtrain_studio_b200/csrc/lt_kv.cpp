@@ -157,6 +157,7 @@ struct lt_kv {
     size_t slot_bytes = 0;
     Slot slots[kSlots];
     int next_slot = 0;
+    uint32_t held = 0;  // slots that the launches of the call in hand read (SlotHold)
 
     // ---- queued device work ----
     std::vector<int2> pend_copies;
@@ -252,10 +253,23 @@ void free_device(lt_kv* kv) {
     kv->d_err = nullptr;
 }
 
-// Next staging slot; waits until every kernel that read its previous
-// contents has finished (the slot's event).
+// The slots that a call has uploaded to, or found its contents in, are its own
+// until its launches are made and their events recorded: a later upload of the
+// same call must not take one of them.
+struct SlotHold {
+    lt_kv* kv;
+    explicit SlotHold(lt_kv* k) : kv(k) { kv->held = 0; }
+    ~SlotHold() { kv->held = 0; }
+    SlotHold(const SlotHold&) = delete;
+    SlotHold& operator=(const SlotHold&) = delete;
+};
+
+// Next staging slot that the call does not hold (three at most are); waits
+// until every kernel that read its previous contents has finished (the slot's
+// event).
 int acquire_slot(lt_kv* kv) {
-    const int s = kv->next_slot;
+    int s = kv->next_slot;
+    while (kv->held >> s & 1u) s = (s + 1) % kSlots;
     kv->next_slot = (s + 1) % kSlots;
     Slot& sl = kv->slots[s];
     if (sl.used) cudaEventSynchronize(sl.ev);
@@ -270,7 +284,8 @@ lt_status mark_slot_use(lt_kv* kv, int s, cudaStream_t st) {
 }
 
 // Upload `bytes` of `src` through the staging ring, reusing the previous
-// upload of the same contents while its slot has not been recycled.
+// upload of the same contents while its slot has not been recycled.  Under the
+// caller's SlotHold.
 lt_status upload(lt_kv* kv, UploadCache& cache, const void* src, size_t bytes, cudaStream_t st, const void** dptr,
                  int* slot_out) {
     if (bytes > kv->slot_bytes) return fail(kv, LT_E_ARG, "upload of %zu bytes exceeds staging slot", bytes);
@@ -278,9 +293,11 @@ lt_status upload(lt_kv* kv, UploadCache& cache, const void* src, size_t bytes, c
         std::memcmp(cache.key.data(), src, bytes) == 0) {
         *dptr = kv->slots[cache.slot].dev;
         *slot_out = cache.slot;
+        kv->held |= 1u << cache.slot;
         return LT_OK;
     }
     const int s = acquire_slot(kv);
+    kv->held |= 1u << s;
     std::memcpy(kv->slots[s].host, src, bytes);
     LT_CUDA(kv, cudaMemcpyAsync(kv->slots[s].dev, kv->slots[s].host, bytes, cudaMemcpyHostToDevice, st));
     cache.key.assign(static_cast<const char*>(src), static_cast<const char*>(src) + bytes);
@@ -742,6 +759,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
     if (score || kv->fmt == LT_KV_Q4_0)
         if (lt_status crc = refuse_capture(kv, st, score ? "lt_kv_attend_shaped" : "attention over a 4-bit cache"))
             return crc;
+    SlotHold hold(kv);
     // Per-token descriptors; the kernel derives its stream-K partition from them.
     const int q_f32 = q_dtype == LT_F32;
     const int max_warps = ltkv::attend_warps(kv->cfg.device, (int)kv->group, (int)kv->cfg.head_dim, q_f32, kv->fmt,
@@ -1200,6 +1218,7 @@ lt_status lt_kv_write(lt_kv* kv, uint32_t layer, const int32_t* block, const int
     }
     if ((rc = flush(kv, st))) return rc;
     if (n == 0) return LT_OK;
+    SlotHold hold(kv);
     const void* d_cells = nullptr;
     int s = -1;
     if ((rc = upload(kv, kv->cells_cache, kv->cells_tmp.data(), n * sizeof(int2), st, &d_cells, &s))) return rc;
@@ -1551,6 +1570,7 @@ lt_status lt_kv_read(lt_kv* kv, uint32_t layer, const int32_t* block, const int3
     if ((rc = refuse_capture(kv, st, "lt_kv_read"))) return rc;
     if ((rc = flush(kv, st))) return rc;
     if (n == 0) return LT_OK;
+    SlotHold hold(kv);
     const void* d_cells = nullptr;
     int s = -1;
     if ((rc = upload(kv, kv->cells_cache, kv->cells_tmp.data(), n * sizeof(int2), st, &d_cells, &s))) return rc;

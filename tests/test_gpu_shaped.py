@@ -266,3 +266,25 @@ def test_short_chunks_over_the_4_bit_cache():
         out, ref = c.run(np.zeros(20, int), pos, q, window=window)
         close(out, ref)
         assert c.kv.cascade_launches() == c0 + (window < 1000)
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8_0"])
+def test_large_calls_with_changing_intervals(fmt):
+    """Calls of more than 512 tokens, whose tokens and intervals are staged apart:
+    the same tokens again and again with other intervals (global and windowed
+    layers, packed documents), more calls than the staging has places."""
+    rng = np.random.default_rng(23)
+    c = Cache(fmt, 1, 64, 2, [160] * 4, rng)
+    seqs, pos = np.repeat(np.arange(4), 144), np.tile(np.arange(16, 160), 4)
+    q = torch.from_numpy(rng.standard_normal((seqs.size, 2 * 64)).astype(np.float32)).cuda()
+    outs = []
+    for call in range(20):
+        first = (np.arange(seqs.size) + 5 * call) % 16
+        outs.append((c.kv.attend_shaped(0, q, seqs, pos, first=first), first))
+    c.kv.check()
+    for out, first in outs:
+        ref = np.zeros((seqs.size, 128))
+        for i, (s, p) in enumerate(zip(seqs, pos)):
+            ref[i] = A.attend(q[i].cpu().numpy().reshape(2, 64), *c.vals[s], int(p), 2, c.kv.default_scale,
+                              first=first[i]).reshape(-1)
+        close(out, ref)
