@@ -1142,10 +1142,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
     const PrefixItem item = p.items[blockIdx.x];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = p.group, Hkv = p.n_kv_heads;
-    // barriers: kv_full[3], kv_empty[3], s_full[2], s_free[2], p_full[2], p_free[2], pv_done, tmem word
+    // barriers: kv_full[3], kv_empty[3], s_full[2], s_free[2], p_full[2], p_free[2]; at 120: tmem word
     const uint32_t kv_full = base + L.bars, kv_empty = kv_full + 8u * kPreStages;
     const uint32_t s_full = kv_empty + 8u * kPreStages, s_free = s_full + 16u, p_full = s_free + 16u,
-                   p_free = p_full + 16u, pv_done = p_free + 16u;
+                   p_free = p_full + 16u;
     const uint32_t pair = base + L.bars + 128;  // 4: the two warps of 32 rows
     uint32_t* tmem_word = reinterpret_cast<uint32_t*>(sbase + L.bars + 8 * (2 * kPreStages + 9));
     if (tid == 0) {
@@ -1160,7 +1160,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             mbar_init(p_free + 8u * bb, 1);
         }
         for (int w = 0; w < 4; ++w) mbar_init(pair + 8u * w, 2);
-        mbar_init(pv_done, 1);
         fence_mbar_init();
     }
     __syncwarp();  // tcgen05.alloc is warp-collective: warp 0 converged after thread 0's setup
@@ -1309,8 +1308,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                          (j > 0 || ks > 0) ? 1u : 0u);
             }
             umma_commit(kv_empty + 8u * st);
-            umma_commit(p_free + 8u * bb);
-            umma_commit(pv_done);
+            umma_commit(p_free + 8u * bb);  // and with it PV(j) and all before it are done
         };
         // S(j) = Q K(j)^T into S buffer j&1, once its copies landed and
         // softmax(j-2) has read that buffer
@@ -1362,6 +1360,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             if (p.shape.slopes) slope = __ldg(p.shape.slopes + item.head * G + hg) * kLog2e;
         }
         float m_use = -INFINITY, l_run = 0.f;
+        // Wait until PV(k), k >= j - 2 in step j, is done.  A wait for a parity takes
+        // phase k - 2 of a barrier for phase k, so it holds only for a warp that has
+        // seen the phase before: here p_free of the steps of k's parity, whose phases
+        // a warp waits for one after the other (step j waits for PV(j - 2)).  One
+        // barrier completed by every PV would not do: S(j) does not follow PV(j - 2),
+        // so in its last step a warp may be two products ahead of it
+        // (tests/test_prefix_waits.py searches the orders).
+        auto wait_pv = [&](int k) {
+            return __all_sync(0xffffffffu, mbar_wait_bounded(p_free + 8u * (k & 1), (k >> 1) & 1)) != 0;
+        };
         for (int j = 0; j < n_steps; ++j) {
             const int bb = j & 1;
             const int npos = step_blocks(j) * kBlock;
@@ -1425,16 +1433,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                 rescale = m_use != -INFINITY;
                 m_use = mx;
             }
-            // P buffer bb is free once PV(j-2) has read it (waited before the
-            // rescale, so pv_done is at most one phase behind PV(j-1))
-            if (j >= 2) {
-                w_ok = mbar_wait_bounded(p_free + 8u * bb, ((j - 2) >> 1) & 1);
-                if (!__all_sync(0xffffffffu, w_ok)) { ok = false; break; }
-            }
+            // P buffer bb is free once PV(j-2) has read it
+            if (j >= 2 && !wait_pv(j - 2)) { ok = false; break; }
             if (__any_sync(0xffffffffu, rescale)) {
                 // this warp's O rows are scaled once PV(j-1) has finished
-                w_ok = mbar_wait_bounded(pv_done, (j - 1) & 1);
-                if (!__all_sync(0xffffffffu, w_ok)) { ok = false; break; }
+                if (!wait_pv(j - 1)) { ok = false; break; }
                 tc_fence_after();
 #pragma unroll 1
                 for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
@@ -1476,10 +1479,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             __syncwarp();
             if (lane == 0) mbar_arrive1(p_full + 8u * bb);
         }
-        if (ok && n_steps > 0) {
-            const bool w_ok = mbar_wait_bounded(pv_done, (n_steps - 1) & 1);
-            ok = __all_sync(0xffffffffu, w_ok);
-        }
+        if (ok && n_steps > 0) ok = wait_pv(n_steps - 1);
         if (ok && n_steps > 0) {  // the row's sum over both halves, through the P buffers, now free
             float* sums = reinterpret_cast<float*>(sbase + L.p0);
             sums[half * kPreRows + r] = l_run;

@@ -288,3 +288,34 @@ def test_large_calls_with_changing_intervals(fmt):
             ref[i] = A.attend(q[i].cpu().numpy().reshape(2, 64), *c.vals[s], int(p), 2, c.kv.default_scale,
                               first=first[i]).reshape(-1)
         close(out, ref)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("length", [100, 128, 190, 1100])
+def test_warps_of_the_pass_run_apart(hd, length):
+    """Prompts through the tensor-core pass whose rows move their maximum at every
+    step in some warps (steep slopes) and never in others (an interval that ends
+    early, no q), over 2, 3 and many steps of 64 positions: a warp that has nothing
+    to rescale runs ahead of one that has.  Every repetition gives the same bits."""
+    rng = np.random.default_rng(hd + length)
+    seqs_n, chunk, hq, hkv = 4, 100, 32, 8
+    c = Cache("q4_0", hkv, hd, hq, [length] * seqs_n, rng)
+    seqs = np.repeat(np.arange(seqs_n), chunk)
+    pos = np.tile(np.arange(length - chunk, length), seqs_n)
+    end = pos + 1
+    early = np.tile(np.arange(chunk) % 16 < 8, seqs_n)  # 8 tokens are the 32 rows of a warp
+    end[early & (seqs < 2)] = 17
+    q = rng.standard_normal((seqs.size, hq * hd)).astype(np.float32)
+    q[early & (seqs >= 2)] = 0
+    q[~early] *= 3
+    slopes = np.where(np.arange(hq) % 4 == 0, 0.0, 1.0).astype(np.float32)
+    c0 = c.kv.cascade_launches()
+    qd = torch.from_numpy(q).cuda()
+    out, ref = c.run(seqs, pos, qd, end=end, slopes=slopes)
+    assert c.kv.cascade_launches() == c0 + 1
+    close(out, ref)
+    sd = torch.from_numpy(slopes).cuda()
+    again = [c.kv.attend_shaped(0, qd, seqs, pos, end=end, slopes=sd) for _ in range(100)]
+    c.kv.check()
+    for a in again:
+        assert torch.equal(a, out)
