@@ -313,7 +313,16 @@ def test_warps_of_the_pass_run_apart(hd, length):
     qd = torch.from_numpy(q).cuda()
     out, ref = c.run(seqs, pos, qd, end=end, slopes=slopes)
     assert c.kv.cascade_launches() == c0 + 1
-    close(out, ref)
+    # Where an interval ends far before its token, every distance in it is near D =
+    # pos: slope * D * log2(e) < 2^11 has a spacing of 2^-13 in f32, its product and
+    # the difference round by half of that each, so a weight is off by a factor of
+    # 2^(2^-13) at most, and an output by 2 * ln(2) * 2^-13 * max|v|.  The other rows
+    # keep the bar above: what weighs in them lies near the token.
+    far = torch.from_numpy(end == 17)
+    close(out[~far], ref[~far.numpy()])
+    most = max(np.abs(v).max() for _, v in c.vals)
+    spacing = np.spacing(np.float32(length * np.log2(np.e)))
+    assert np.abs(out[far].cpu().numpy() - ref[far.numpy()]).max() <= 2e-5 + 2 * np.log(2) * spacing * most
     sd = torch.from_numpy(slopes).cuda()
     again = [c.kv.attend_shaped(0, qd, seqs, pos, end=end, slopes=sd) for _ in range(100)]
     c.kv.check()
