@@ -196,6 +196,15 @@ __device__ __forceinline__ void load8_f32(const void* base, size_t idx, int in_f
     }
 }
 
+// A power of two that brings a row of q whose largest magnitude is mx near 2^12, and
+// its inverse: value and residual of the row are then normal f16s.
+__device__ __forceinline__ void q_row_scale(float mx, float& mul, float& inv) {
+    const int ex = (int)(__float_as_uint(mx) >> 23);  // 255: Inf, which no scale helps
+    const int fe = ex == 255 ? 127 : min(253, max(1, 266 - ex));
+    mul = __uint_as_float((uint32_t)fe << 23);
+    inv = __uint_as_float((uint32_t)(254 - fe) << 23);
+}
+
 // Peer gather: a warp is done and stored the output rows of `items`
 // (token, head) items into this rank's gather half (local memory).  Only
 // such warps take part: after the warp barrier, lane 0 adds the items to

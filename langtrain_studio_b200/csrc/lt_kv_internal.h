@@ -163,6 +163,7 @@ struct PrefixParams {
     int32_t n_kv_heads, group;
     const void* q;
     int32_t q_f32;
+    int32_t scale_q;     // LT_KV_Q4_0: rows of q go to the tensor core times a power of two
     float scale_log2;
     float* pre_o;
     float* pre_ml;

@@ -1224,37 +1224,43 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
     // Row r attends positions [0, lim) of the item's blocks: those of the shared
     // blocks, or those up to its token (a prefill chunk, causally).
     const int lim = live ? p.tok_lim[item.tok_off + t_item] : 0x7fffffff;
+    const size_t q_at = (((size_t)tok * Hkv + item.head) * G + hg) * D;
+    float* maxima = reinterpret_cast<float*>(sbase + L.maxima);
+    // p.scale_q: rows times a power of two as in the stream-K launch over the same
+    // cache, so that q far from 1 keeps its bits here too; q_inv takes it off S
+    float q_mul = 1.f, q_inv = 1.f;
+    if (p.scale_q) {
+        if (half < 2) {
+            float mx = 0.f;
+            if (live) {
+#pragma unroll 2
+                for (int c = half * (D / 16); c < (half + 1) * (D / 16); ++c) {
+                    float x[8];
+                    load8_f32(p.q, q_at + 8 * c, p.q_f32, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+                }
+            }
+            maxima[half * kPreRows + r] = mx;
+        }
+        __syncthreads();
+        if (half < 2) q_row_scale(fmaxf(maxima[r], maxima[kPreRows + r]), q_mul, q_inv);
+    }
     if (half < 2) {
-        const int qelem = p.q_f32 ? 4 : 2;
-        const uint8_t* qrow = static_cast<const uint8_t*>(p.q) + (((size_t)tok * Hkv + item.head) * G + hg) * D * qelem;
 #pragma unroll 1
         for (int c = half * (D / 16); c < (half + 1) * (D / 16); ++c) {
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = 0.f;
-            if (live) {
-                if (p.q_f32) {
-                    const float4 a = *reinterpret_cast<const float4*>(qrow + c * 32);
-                    const float4 b2 = *reinterpret_cast<const float4*>(qrow + c * 32 + 16);
-                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b2.x; x[5] = b2.y; x[6] = b2.z; x[7] = b2.w;
-                } else {
-                    const uint4 u = *reinterpret_cast<const uint4*>(qrow + c * 16);
-                    const __half2* h2 = reinterpret_cast<const __half2*>(&u);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = __half22float2(h2[e]);
-                        x[2 * e] = f.x;
-                        x[2 * e + 1] = f.y;
-                    }
-                }
-            }
+            if (live) load8_f32(p.q, q_at + 8 * c, p.q_f32, x);
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const __half2 h = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+                const float x0 = x[2 * e] * q_mul, x1 = x[2 * e + 1] * q_mul;
+                const __half2 h = __floats2half2_rn(x0, x1);
                 const float2 hf = __half22float2(h);
                 hi[e] = h2_bits(h);
-                lo[e] = h2_bits(__floats2half2_rn(x[2 * e] - hf.x, x[2 * e + 1] - hf.y));
+                lo[e] = h2_bits(__floats2half2_rn(x0 - hf.x, x1 - hf.y));
             }
             const uint32_t off = (uint32_t)(c >> 3) * (kPreRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
             *reinterpret_cast<uint4*>(sbase + L.q_hi + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -1350,8 +1356,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
         // (TMEM lane r), warps w and w + 4 the halves of the same rows =====
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t my_pair = pair + 8u * (warp & 3);
-        float* maxima = reinterpret_cast<float*>(sbase + L.maxima);
-        const float scale_log2 = p.scale_log2;
+        const float scale_log2 = p.scale_log2 * q_inv;
+        [[maybe_unused]] const float scale_cap = SH ? p.shape.scale_cap * q_inv : 0.f;
         int lo = 0, qpos = 0;  // SH: the row attends [lo, lim), and its own position
         float slope = 0.f;
         if (SH && live) {
@@ -1391,7 +1397,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                 const int at = pos0 + 32 * half, q_off = qpos - at, from = lo - at;
                 if (p.shape.capped) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sv_[i] = p.shape.cap_log2 * tanhf(sv_[i] * p.shape.scale_cap);
+                    for (int i = 0; i < 32; ++i) sv_[i] = p.shape.cap_log2 * tanhf(sv_[i] * scale_cap);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sv_[i] *= scale_log2;

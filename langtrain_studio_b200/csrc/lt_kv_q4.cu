@@ -925,17 +925,14 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
             for (int i = 0; i < 2 * KS; ++i)
                 x[i] = __half22float2(*reinterpret_cast<const __half2*>(qbuf + (at + 8 * i) * 2));
         }
-        // Scale each row by a power of two that brings its largest value near
-        // 2^12: value and residual are then normal f16s.  Rows past the group
-        // repeat its last one; nothing stores their results.
+        // Rows past the group repeat its last one; nothing stores their results.
         float mx = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * KS; ++i) mx = fmaxf(mx, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
         mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
-        const int ex = (int)(__float_as_uint(mx) >> 23);  // 255: Inf, which no scale helps
-        const int fe = ex == 255 ? 127 : min(253, max(1, 266 - ex));
-        const float f = __uint_as_float((uint32_t)fe << 23), finv = __uint_as_float((uint32_t)(254 - fe) << 23);
+        float f, finv;
+        q_row_scale(mx, f, finv);
 #pragma unroll
         for (int i = 0; i < 2 * KS; ++i) {
             const float y0 = x[i].x * f, y1 = x[i].y * f;

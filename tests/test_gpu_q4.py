@@ -677,3 +677,38 @@ def test_short_runs_are_not_attended_whole():
     close(t.kv.attend(0, torch.from_numpy(q).cuda(), seqs, pos), ref)
     assert t.kv.cascade_launches() == c0
     t.kv.check()
+
+
+@pytest.mark.parametrize("gain,dtype", [(1e-6, torch.float32), (3e4, torch.float32), (1e6, torch.float32),
+                                        (2e-6, torch.float16), (8e3, torch.float16)])
+@pytest.mark.parametrize("hd,hq,hkv", [(128, 8, 2), (64, 9, 3)])
+def test_chunks_and_prefixes_of_small_and_large_q(gain, dtype, hd, hq, hkv):
+    """What test_attention_of_small_and_large_q asks of one token holds for prefill
+    chunks and members of a shared prefix: they take another kernel."""
+    rng = np.random.default_rng(51)
+    t = Twin(hkv, hd, 16 * 120, hq, max_seqs=14)
+    t.fill(0, 100, rng)
+    for s in range(1, 12):
+        t.kv.share(0, s, 70)
+        t.rows[(0, s)] = list(t.rows[(0, 0)][:70])
+        t.fill(s, 71 + 5 * (s % 4), rng)
+    scale = float(np.float32(t.kv.default_scale / gain))
+    slopes = np.exp2(-np.arange(1, hq + 1)).astype(np.float32)
+    chunk = np.zeros(60, int), np.arange(40, 100)
+    members = np.arange(1, 12), np.array([t.kv.len(s) - 1 for s in range(1, 12)])
+    for (seqs, pos), shape in ((chunk, {}), (members, {}), (chunk, dict(softcap=5.0, window=40)),
+                               (chunk, dict(slopes=slopes))):
+        q = torch.from_numpy((rng.standard_normal((seqs.size, hq * hd)) * gain).astype(np.float32)).cuda().to(dtype)
+        dev = {k: (torch.from_numpy(v).cuda() if k == "slopes" else v) for k, v in shape.items()}
+        c0 = t.kv.cascade_launches()
+        if shape:
+            out = t.kv.attend_shaped(0, q, seqs, pos, scale=scale, **dev)
+        else:
+            out = t.kv.attend(0, q, seqs, pos, scale=scale)
+        assert t.kv.cascade_launches() == c0 + 1
+        ref = np.zeros((seqs.size, hq * hd))
+        for i, (s, p) in enumerate(zip(seqs, pos)):
+            ref[i] = A.attend(q[i].float().cpu().numpy().reshape(hq, hd), *t.values(0, int(s)), int(p), hq // hkv,
+                              scale, **shape).reshape(-1)
+        close(out, ref)
+    t.kv.check()
