@@ -976,6 +976,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         pp.q = q;
         pp.q_f32 = q_f32;
         pp.scale_q = kv->fmt == LT_KV_Q4_0;
+        pp.skip_rows = kv->fmt == LT_KV_F16;
         pp.scale_log2 = p.scale_log2;
         pp.pre_o = kv->d_pre_o;
         pp.pre_ml = kv->d_pre_ml;

@@ -164,6 +164,7 @@ struct PrefixParams {
     const void* q;
     int32_t q_f32;
     int32_t scale_q;     // LT_KV_Q4_0: rows of q go to the tensor core times a power of two
+    int32_t skip_rows;   // LT_KV_F16: V may hold Inf or NaN; a block's products leave out the rows it is masked for
     float scale_log2;
     float* pre_o;
     float* pre_ml;

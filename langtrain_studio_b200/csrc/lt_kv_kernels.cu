@@ -1036,6 +1036,18 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64
         : "memory");
 }
 
+// The same, leaving the rows of D whose bit in `skip` is set as they are.
+__device__ __forceinline__ void umma_f16_skip(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate, const uint32_t (&skip)[4]) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(skip[0]), "r"(skip[1]), "r"(skip[2]), "r"(skip[3])
+        : "memory");
+}
+
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile(
         "{\n\t.reg .pred e;\n\t"
@@ -1267,6 +1279,17 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             *reinterpret_cast<uint4*>(sbase + L.q_lo + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
+    // MMA warp: where rows lane, lane + 32, ... end, and the first of all rows' ends
+    int ends[4] = {}, first_end = 0x7fffffff;
+    if (p.skip_rows && warp == kPreMmaWarp) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int ti = (lane + 32 * w) / G;
+            ends[w] = ti < item.n_tok && ti < kPreRows / G ? p.tok_lim[item.tok_off + ti] : 0x7fffffff;
+            first_end = min(first_end, ends[w]);
+        }
+        first_end = __reduce_min_sync(0xffffffffu, first_end);
+    }
     fence_proxy_async_smem();  // Q -> visible to the tensor core
     tc_fence_before();
     __syncthreads();
@@ -1305,6 +1328,26 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             const int nblk = step_blocks(j);
             const uint64_t dv = sw128_desc(base + L.stage0 + st * STAGE + KPART, HALF_ROWS_BYTES, 1024);
             const uint64_t dp = dp0 + ((uint64_t)(bb * PBUF) >> 4);
+            // A prefill chunk's rows end at different blocks, and P = 0 does not keep an Inf
+            // or NaN of a V row that an earlier token must not see out of its O: there the
+            // products of a block leave the rows that end before it alone.  (An f16 cache;
+            // 4-bit values are finite.)
+            const int at = (item.blk0 + j * kPreStepBlocks) * kBlock;
+            if (at + nblk * kBlock > first_end) {
+#pragma unroll 1
+                for (int ks = 0; ks < nblk; ++ks) {
+                    uint32_t skip[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) skip[w] = __ballot_sync(0xffffffffu, ends[w] <= at + ks * kBlock);
+                    const uint64_t bdesc = dv + ((uint64_t)(ks * (kBlock * 128)) >> 4);
+                    umma_f16_skip(tmem_o, dp + (uint64_t)(ks * 2), bdesc, idesc_pv, (j > 0 || ks > 0) ? 1u : 0u, skip);
+                    umma_f16_skip(tmem_o + kPreResidualO, dp + ((uint64_t)(kPreRows * 128 + ks * 32) >> 4), bdesc,
+                                  idesc_pv, (j > 0 || ks > 0) ? 1u : 0u, skip);
+                }
+                umma_commit(kv_empty + 8u * st);
+                umma_commit(p_free + 8u * bb);
+                return;
+            }
 #pragma unroll
             for (int ks = 0; ks < kPreStepBlocks; ++ks) {
                 if (ks >= nblk) break;
@@ -1507,8 +1550,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                 float o[32], o2[32];
                 tmem_ld32(tmem_o + lane_off + c0, o);
                 tmem_ld32(tmem_o + kPreResidualO + lane_off + c0, o2);
+                // (a row without a position in this part of the blocks has an O of nothing)
+                const bool none = p.skip_rows && m_use == -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] += o2[i];
+                for (int i = 0; i < 32; ++i) o[i] = none ? 0.f : o[i] + o2[i];
                 if (live) {
                     if (half_out) {
                         uint4* hdst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * D + c0);

@@ -469,3 +469,34 @@ def test_cascade_groups_mixed_with_private_sequences(oracle_mod):
     assert t.kv.cascade_launches() == c0 + 1
     np.testing.assert_allclose(out2, ref, rtol=1e-4, atol=2e-5)
     t.kv.check()
+
+
+@pytest.mark.parametrize("hd,hq,hkv,length,chunk", [(64, 8, 2, 300, 200), (128, 8, 2, 330, 128), (128, 4, 1, 2100, 150)])
+def test_prefill_chunk_behind_cells_that_hold_inf_and_nan(hd, hq, hkv, length, chunk):
+    """A chunk's earlier tokens do not see its later ones' cells, whatever these
+    hold: not in the prefix pass either, where one V tile serves all rows.  Against
+    softmax attention in 64 bits; tolerances as for any prefill chunk."""
+    import _attn64 as A
+    from langtrain_studio_b200.kv import KvCache
+
+    rng = np.random.default_rng(length)
+    kv = KvCache(1, hkv, hd, length, n_heads=hq, max_seqs=1, max_batch=length)
+    x = rng.standard_normal((2, length, hkv * hd)).astype(np.float16)
+    bad = [length - chunk // 2, length - chunk // 3, length - 5]
+    for p, (k, v) in zip(bad, ((0.0, np.inf), (np.inf, np.nan), (np.nan, -np.inf))):
+        x[0, p] += k
+        x[1, p] += v
+    cells = kv.append_batch(np.zeros(length), np.arange(length))
+    kv.write(0, *cells, *(torch.from_numpy(a).cuda() for a in x))
+    pos = np.arange(length - chunk, length)
+    q = rng.standard_normal((chunk, hq * hd)).astype(np.float32)
+    c0 = kv.cascade_launches()
+    out = kv.attend(0, torch.from_numpy(q).cuda(), np.zeros(chunk), pos).cpu().numpy()
+    kv.check()
+    assert kv.cascade_launches() == c0 + 1
+    K, V = x.astype(np.float64).reshape(2, length, hkv, hd)
+    clean = int(np.argmax(pos == bad[0]))
+    for i in range(clean):
+        ref = A.attend(q[i].reshape(hq, hd), K, V, int(pos[i]), hq // hkv, kv.default_scale)
+        np.testing.assert_allclose(out[i], ref.reshape(-1), rtol=1e-4, atol=2e-5)
+    assert not np.isfinite(out[clean:]).any()  # these see the Inf row themselves
