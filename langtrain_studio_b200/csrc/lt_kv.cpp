@@ -755,10 +755,10 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
             return fail(kv, LT_E_ARG, "attend_gather of %u tokens exceeds the exported max_tokens %u", n,
                         kv->peer.max_tokens);
     }
-    if (n == 0) return flush(kv, st);
     if (score || kv->fmt == LT_KV_Q4_0)
         if (lt_status crc = refuse_capture(kv, st, score ? "lt_kv_attend_shaped" : "attention over a 4-bit cache"))
             return crc;
+    if (n == 0) return flush(kv, st);
     SlotHold hold(kv);
     // Per-token descriptors; the kernel derives its stream-K partition from them.
     const int q_f32 = q_dtype == LT_F32;

@@ -167,12 +167,28 @@ void staging(uint32_t fmt) {
     NEED(n_attend == 40, "%d launches", n_attend);
 }
 
+// A call that is refused in a capture leaves everything as it was, one of no
+// tokens too: a plan put into a graph would reach the tables only as it replays.
+void capture(uint32_t fmt, bool shaped) {
+    Cache c(fmt, 2, 2, 16 * 16, 2, 64);
+    c.fill(0, 20);
+    lt_kv_score score{};
+    g_capturing = true;
+    NEED(c.attend(shaped ? &score : nullptr) == LT_E_ARG && n_plan == 0, "no tokens: %d plans", n_plan);
+    c.tokens(0, 19, 20);
+    NEED(c.attend(shaped ? &score : nullptr) == LT_E_ARG && n_plan == 0, "one token: %d plans", n_plan);
+    g_capturing = false;
+    NEED(c.attend(shaped ? &score : nullptr) == LT_OK && n_attend == 1, "%s", lt_kv_last_error(c.kv));
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     if (what == "staging-f16") staging(LT_KV_F16);
     else if (what == "staging-q8_0") staging(LT_KV_Q8_0);
+    else if (what == "capture-q4_0") capture(LT_KV_Q4_0, false);
+    else if (what == "capture-shaped") capture(LT_KV_F16, true);
     else return std::printf("no scenario '%s'\n", what.c_str()), 2;
     std::printf("ok\n");
     return 0;

@@ -34,3 +34,10 @@ def test_a_call_keeps_its_staging(host_launch, fmt):
     """Calls of more than 512 tokens with shaped scores: the tokens' descriptors
     stay where the launch reads them while the call stages its intervals."""
     host_launch(f"staging-{fmt}")
+
+
+@pytest.mark.parametrize("what", ["q4_0", "shaped"])
+def test_a_refused_capture_leaves_no_trace(host_launch, what):
+    """Attention over a 4-bit cache and with shaped scores is refused inside a
+    capture before anything is queued on the stream, whatever the call holds."""
+    host_launch(f"capture-{what}")
