@@ -712,3 +712,69 @@ def test_chunks_and_prefixes_of_small_and_large_q(gain, dtype, hd, hq, hkv):
                               scale, **shape).reshape(-1)
         close(out, ref)
     t.kv.check()
+
+
+def test_scheduler_outputs_over_a_4_bit_cache(oracle_mod):
+    """Every step's outputs of the scheduler test above are attention over the rows
+    that the policy has cached: the oracle, driven by the restated policy, holds the
+    same rows after quantisation (its f16 values are the 4-bit ones exactly), and
+    eviction, preemption and compaction leave every cell where it says."""
+    import bench
+    from langtrain_studio_b200.sched import Scheduler
+    from oracle import churn
+
+    hkv, hq, d, n_slots, pool = 2, 8, 64, 24, 96
+
+    class Quantised:  # the driver's view of a cache, over the oracle
+        def __init__(self):
+            self.ok = oracle_mod.OracleKv(1, hkv * d, pool * 16, max_seqs=n_slots)
+            for name in ("free_blocks", "truncate", "share", "seq_blocks", "refs"):
+                setattr(self, name, getattr(self.ok, name))
+
+        def append_batch(self, seqs, pos):
+            rc, _, b, s = self.ok.append_batch(seqs, pos)
+            assert rc == 0
+            return b, s
+
+        def write(self, layer, b, s, k, v):
+            k, v = (A.value4(*A.quant4(x.reshape(-1, hkv, d))).astype(np.float16).reshape(-1, hkv * d) for x in (k, v))
+            self.ok.write_batch(layer, b, s, k, v)
+
+        def write_attend(self, layer, b, s, k, v, q, seqs, pos, out):
+            self.write(layer, b, s, k, v)
+            self.attended = np.zeros((len(seqs), hq * d))
+            for i, (seq, p) in enumerate(zip(seqs, pos)):
+                K, V = (r.view(np.float16).reshape(-1, hkv, d) for r in self.ok.rows(layer, int(seq), int(p) + 1))
+                self.attended[i] = A.attend(q[i].reshape(hq, d), K, V, int(p), hq // hkv, kv.default_scale).reshape(-1)
+
+        def compact(self):
+            return len(self.ok.compact())
+
+    kv = KvCache(1, hkv, d, 16 * pool, n_heads=hq, max_seqs=n_slots, max_batch=4096, max_blocks_per_seq=64,
+                 kv_format="q4_0")
+    sched, want = Scheduler(kv, n_slots), Quantised()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    kv_src = torch.randn((4096, hkv * d), generator=g, device="cuda", dtype=torch.float16)
+    q_src = torch.randn((n_slots, hq * d), generator=g, device="cuda", dtype=torch.float16)
+    drv = churn.ChurnDriver(want, n_slots, kv_src.cpu().numpy(), q_src.cpu().numpy())
+    arr = bench.Arrivals(1.5, 7, lo=8, hi=300, olo=4, ohi=40)
+    for step in range(60):
+        for p, o in arr.step():
+            sched.submit(p, o)
+            drv.submit(p, o)
+        out = torch.full((n_slots, hq * d), float("nan"), device="cuda", dtype=torch.float16)
+        nd = sched.step(kv_src, q_src, out)
+        drv.step(np.zeros((n_slots, hq * d), np.float16))
+        for s in range(n_slots):
+            assert np.array_equal(kv.seq_blocks(s), want.seq_blocks(s)), (step, s)
+        if nd:
+            assert len(want.attended) == nd
+            close(out[:nd], want.attended, torch.float16)
+        assert out[nd:].isnan().all()  # rows behind the last token stay as they were
+    st = sched.stats
+    assert st["evicted"] > 0 and st["moved_blocks"] > 0 and st["decode_tokens"] > 60 and st["prefill_tokens"] > 0, st
+    kc, vc, kd, vd = kv.pool_reference_layout(0)
+    for codes, scales, ref in ((kc, kd, want.ok.pool()[0][0]), (vc, vd, want.ok.pool()[1][0])):
+        got = A.value4(codes, scales.view(np.float16).astype(np.float64))
+        assert np.array_equal(got.reshape(ref.shape), ref.view(np.float16).astype(np.float64))
+    kv.check()
