@@ -650,10 +650,13 @@ int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n
     for (const Group& g : groups)
         for (int32_t c0 = 0; c0 < g.cnt; c0 += tpc) {
             const int32_t L = chunk_blocks(g, c0);
+            int32_t full = L;  // the tokens' smallest skip
+            for (int32_t k = c0; k < std::min(g.cnt, c0 + tpc); ++k)
+                full = std::min(full, kv->toks_tmp[toks[g.off + k]].skip);
             for (uint32_t h = 0; h < hkv; ++h)
                 for (int sp = 0; sp < S; ++sp) {
                     const int32_t b0 = (int32_t)((long long)L * sp / S), b1 = (int32_t)((long long)L * (sp + 1) / S);
-                    items.push_back({g.root, b0, b1, sp, (int32_t)h, g.off + c0, std::min(tpc, g.cnt - c0)});
+                    items.push_back({g.root, b0, b1, full, sp, (int32_t)h, g.off + c0, std::min(tpc, g.cnt - c0)});
                 }
         }
     const size_t item_words = items.size() * (sizeof(ltkv::PrefixItem) / 4);
@@ -719,7 +722,7 @@ int plan_whole(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, const ltkv::
             blk0 = std::max(blk0, first);  // (a chunk of empty intervals alone may lie before the group's first)
             longest = std::max(longest, blk1 - blk0);
             for (uint32_t h = 0; h < hkv; ++h)
-                items.push_back({(int32_t)used - first, blk0, std::max(blk1, blk0 + 1), 0, (int32_t)h, (int32_t)c0,
+                items.push_back({(int32_t)used - first, blk0, std::max(blk1, blk0 + 1), blk0, 0, (int32_t)h, (int32_t)c0,
                                  (int32_t)(c1 - c0)});
         }
         used += count;
@@ -975,8 +978,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
         pp.group = (int32_t)kv->group;
         pp.q = q;
         pp.q_f32 = q_f32;
-        pp.scale_q = kv->fmt == LT_KV_Q4_0;
-        pp.skip_rows = kv->fmt == LT_KV_F16;
+        pp.scale_q = kv->fmt == LT_KV_Q4_0 && q_f32;
         pp.scale_log2 = p.scale_log2;
         pp.pre_o = kv->d_pre_o;
         pp.pre_ml = kv->d_pre_ml;
@@ -1006,7 +1008,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
             pp.max_blocks = 1;
             pp.n_blocks = (int32_t)kv->exp_cap;
         }
-        const cudaError_t pe = ltkv::launch_prefix(pp, n_items, (int)kv->cfg.head_dim, score != nullptr, st);
+        const cudaError_t pe = ltkv::launch_prefix(pp, n_items, (int)kv->cfg.head_dim, kv->fmt == LT_KV_Q4_0, score != nullptr, st);
         if (pe != cudaSuccess) {
             rollback();
             return fail(kv, LT_E_CUDA, "prefix launch: %s", cudaGetErrorString(pe));

@@ -146,6 +146,7 @@ struct PrefixItem {
                        // lie in the workspace)
     int32_t blk0;      // this item's part of the shared blocks: [blk0, blk1)
     int32_t blk1;
+    int32_t full;      // blocks before this one count for every token of the item
     int32_t split;     // which partial slab it writes
     int32_t head;      // KV head
     int32_t tok_off;   // first of the item's tokens in the token list
@@ -163,8 +164,7 @@ struct PrefixParams {
     int32_t n_kv_heads, group;
     const void* q;
     int32_t q_f32;
-    int32_t scale_q;     // LT_KV_Q4_0: rows of q go to the tensor core times a power of two
-    int32_t skip_rows;   // LT_KV_F16: V may hold Inf or NaN; a block's products leave out the rows it is masked for
+    int32_t scale_q;     // q4: rows of q go to the tensor core times a power of two
     float scale_log2;
     float* pre_o;
     float* pre_ml;
@@ -180,7 +180,8 @@ struct PrefixParams {
 };
 // Tokens one prefix CTA covers: 128 query rows / group.
 inline int prefix_tokens_per_cta(int group) { return 128 / group; }
-cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, bool shaped, cudaStream_t s);
+// q4: the tiles are an expanded 4-bit cache's; only those have shaped scores.
+cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, bool q4, bool shaped, cudaStream_t s);
 
 // Warps of one attention launch on `device` (all resident at once), or 0.
 // fmt: lt_kv_format of the pool; shaped: the launch is launch_attend_shaped.

@@ -1132,7 +1132,8 @@ __device__ __forceinline__ void mbar_arrive1(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-template <int D, bool SH>
+// Q4: the tiles are an expanded 4-bit cache's.
+template <int D, bool SH, bool Q4>
 __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
     // The decode launch that folds these partials in may start on the SMs
     // this launch leaves free; it waits for this grid before the fold.
@@ -1239,36 +1240,37 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
     const size_t q_at = (((size_t)tok * Hkv + item.head) * G + hg) * D;
     float* maxima = reinterpret_cast<float*>(sbase + L.maxima);
     // p.scale_q: rows times a power of two as in the stream-K launch over the same
-    // cache, so that q far from 1 keeps its bits here too; q_inv takes it off S
+    // cache, so that q far from 1 keeps its bits here too; q_inv takes it off S.
+    // The half row is loaded at once: chunk by chunk, twice, took 13 us more a call
+    // (4 x 256 tokens over 2048, f32 q).
     float q_mul = 1.f, q_inv = 1.f;
-    if (p.scale_q) {
-        if (half < 2) {
-            float mx = 0.f;
-            if (live) {
-#pragma unroll 2
-                for (int c = half * (D / 16); c < (half + 1) * (D / 16); ++c) {
-                    float x[8];
-                    load8_f32(p.q, q_at + 8 * c, p.q_f32, x);
+    float x[D / 16][8];
+    if (half < 2) {
+        float mx = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
-                }
-            }
-            maxima[half * kPreRows + r] = mx;
+        for (int i = 0; i < D / 16; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+            if (live) load8_f32(p.q, q_at + (size_t)8 * (half * (D / 16) + i), p.q_f32, x[i]);
         }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[i][e]));
+        if (Q4 && p.scale_q) maxima[half * kPreRows + r] = mx;
+    }
+    if (Q4 && p.scale_q) {
         __syncthreads();
         if (half < 2) q_row_scale(fmaxf(maxima[r], maxima[kPreRows + r]), q_mul, q_inv);
     }
     if (half < 2) {
-#pragma unroll 1
-        for (int c = half * (D / 16); c < (half + 1) * (D / 16); ++c) {
-            float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
-            if (live) load8_f32(p.q, q_at + 8 * c, p.q_f32, x);
+        for (int i = 0; i < D / 16; ++i) {
+            const int c = half * (D / 16) + i;
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x0 = x[2 * e] * q_mul, x1 = x[2 * e + 1] * q_mul;
+                const float x0 = x[i][2 * e] * q_mul, x1 = x[i][2 * e + 1] * q_mul;
                 const __half2 h = __floats2half2_rn(x0, x1);
                 const float2 hf = __half22float2(h);
                 hi[e] = h2_bits(h);
@@ -1279,16 +1281,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             *reinterpret_cast<uint4*>(sbase + L.q_lo + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
-    // MMA warp: where rows lane, lane + 32, ... end, and the first of all rows' ends
-    int ends[4] = {}, first_end = 0x7fffffff;
-    if (p.skip_rows && warp == kPreMmaWarp) {
+    int ends[4] = {};  // MMA warp: where rows lane, lane + 32, ... end
+    if (!Q4 && warp == kPreMmaWarp) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const int ti = (lane + 32 * w) / G;
             ends[w] = ti < item.n_tok && ti < kPreRows / G ? p.tok_lim[item.tok_off + ti] : 0x7fffffff;
-            first_end = min(first_end, ends[w]);
         }
-        first_end = __reduce_min_sync(0xffffffffu, first_end);
     }
     fence_proxy_async_smem();  // Q -> visible to the tensor core
     tc_fence_before();
@@ -1332,13 +1331,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
             // or NaN of a V row that an earlier token must not see out of its O: there the
             // products of a block leave the rows that end before it alone.  (An f16 cache;
             // 4-bit values are finite.)
-            const int at = (item.blk0 + j * kPreStepBlocks) * kBlock;
-            if (at + nblk * kBlock > first_end) {
+            const int blk = item.blk0 + j * kPreStepBlocks;
+            if (!Q4 && blk + nblk > item.full) {
 #pragma unroll 1
                 for (int ks = 0; ks < nblk; ++ks) {
                     uint32_t skip[4];
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) skip[w] = __ballot_sync(0xffffffffu, ends[w] <= at + ks * kBlock);
+                    for (int w = 0; w < 4; ++w) skip[w] = __ballot_sync(0xffffffffu, ends[w] <= (blk + ks) * kBlock);
                     const uint64_t bdesc = dv + ((uint64_t)(ks * (kBlock * 128)) >> 4);
                     umma_f16_skip(tmem_o, dp + (uint64_t)(ks * 2), bdesc, idesc_pv, (j > 0 || ks > 0) ? 1u : 0u, skip);
                     umma_f16_skip(tmem_o + kPreResidualO, dp + ((uint64_t)(kPreRows * 128 + ks * 32) >> 4), bdesc,
@@ -1551,7 +1550,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
                 tmem_ld32(tmem_o + lane_off + c0, o);
                 tmem_ld32(tmem_o + kPreResidualO + lane_off + c0, o2);
                 // (a row without a position in this part of the blocks has an O of nothing)
-                const bool none = p.skip_rows && m_use == -INFINITY;
+                const bool none = !Q4 && m_use == -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = none ? 0.f : o[i] + o2[i];
                 if (live) {
@@ -1883,7 +1882,7 @@ cudaError_t launch_attend_shaped(const AttnShapedParams& p, int head_dim, cudaSt
 
 int attend_launches(const AttnParams& p) { return p.n_warps == 0 ? 0 : 1; }
 
-template <int D, bool SH>
+template <int D, bool SH, bool Q4>
 cudaError_t launch_prefix_d(const PrefixParams& p, int n_items, cudaStream_t s) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -1892,18 +1891,24 @@ cudaError_t launch_prefix_d(const PrefixParams& p, int n_items, cudaStream_t s) 
     static bool attr[64] = {};
     const size_t smem = PreSmem(D).alloc();
     if (!attr[dev]) {
-        e = cudaFuncSetAttribute(prefix_attn_kernel<D, SH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        e = cudaFuncSetAttribute(prefix_attn_kernel<D, SH, Q4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
         attr[dev] = true;
     }
-    prefix_attn_kernel<D, SH><<<n_items, kPreThreads, smem, s>>>(p);
+    prefix_attn_kernel<D, SH, Q4><<<n_items, kPreThreads, smem, s>>>(p);
     return cudaGetLastError();
 }
 
-cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, bool shaped, cudaStream_t s) {
+cudaError_t launch_prefix(const PrefixParams& p, int n_items, int head_dim, bool q4, bool shaped, cudaStream_t s) {
     if (n_items <= 0) return cudaSuccess;
-    if (shaped) return head_dim == 64 ? launch_prefix_d<64, true>(p, n_items, s) : launch_prefix_d<128, true>(p, n_items, s);
-    return head_dim == 64 ? launch_prefix_d<64, false>(p, n_items, s) : launch_prefix_d<128, false>(p, n_items, s);
+    if (shaped)
+        return head_dim == 64 ? launch_prefix_d<64, true, true>(p, n_items, s)
+                              : launch_prefix_d<128, true, true>(p, n_items, s);
+    if (q4)
+        return head_dim == 64 ? launch_prefix_d<64, false, true>(p, n_items, s)
+                              : launch_prefix_d<128, false, true>(p, n_items, s);
+    return head_dim == 64 ? launch_prefix_d<64, false, false>(p, n_items, s)
+                          : launch_prefix_d<128, false, false>(p, n_items, s);
 }
 
 cudaError_t launch_gather_permute(const void* gathered, void* out, int nranks, uint32_t n, size_t row_bytes,

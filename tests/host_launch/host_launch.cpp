@@ -66,7 +66,7 @@ cudaError_t launch_attend_shaped(const AttnShapedParams& p, int, cudaStream_t) {
     if (on_attend) on_attend(p, &p);
     return cudaSuccess;
 }
-cudaError_t launch_prefix(const PrefixParams& p, int n_items, int, bool, cudaStream_t) {
+cudaError_t launch_prefix(const PrefixParams& p, int n_items, int, bool, bool, cudaStream_t) {
     ++n_prefix;
     if (on_prefix) on_prefix(p, n_items);
     return cudaSuccess;
