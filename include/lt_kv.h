@@ -24,8 +24,10 @@
  * the next kernel-launching call.
  *
  * Pointers.  Arguments named *_host are host memory; `k`, `v`, `q`, `out`
- * and the pointers of lt_kv_rows are device memory.  seq / pos / block /
- * slot arrays are host memory (they are the reference's Vec arguments).
+ * and the pointers of lt_kv_rows and lt_kv_read are device memory, 16-byte
+ * aligned (other pointers, and null ones of a call of some rows, are refused
+ * with LT_E_ARG).  seq / pos / block / slot arrays are host memory (they are
+ * the reference's Vec arguments).
  *
  * Errors.  Every fallible call returns an lt_status; the message of the last
  * error is kept per handle (lt_kv_last_error).

@@ -466,6 +466,15 @@ lt_status require_device(lt_kv* kv) {
     return LT_OK;
 }
 
+// Device arrays of a call of n rows: the kernels read and write 16 bytes at a
+// time, and a fault would cost the context.
+lt_status check_arrays(lt_kv* kv, uint32_t n, std::initializer_list<const void*> arrays, const char* names) {
+    for (const void* a : arrays)
+        if (n > 0 && (!a || (reinterpret_cast<uintptr_t>(a) & 15)))
+            return fail(kv, LT_E_ARG, "%s must be 16-byte aligned device pointers", names);
+    return LT_OK;
+}
+
 lt_status check_tokens(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n) {
     if (n > kv->cfg.max_batch) return fail(kv, LT_E_ARG, "batch of %u tokens exceeds max_batch %u", n, kv->cfg.max_batch);
     for (uint32_t i = 0; i < n; ++i) {
@@ -749,9 +758,7 @@ lt_status attend_impl(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtype
                       const uint32_t* pos, uint32_t n, void* out, lt_dtype out_dtype, float scale, const void* k,
                       const void* v, lt_dtype kv_dtype, bool fused, cudaStream_t st, bool gather = false,
                       const lt_kv_score* score = nullptr) {
-    if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) ||
-        (k && (reinterpret_cast<uintptr_t>(k) & 15)) || (v && (reinterpret_cast<uintptr_t>(v) & 15)))
-        return fail(kv, LT_E_ARG, "q, out, k and v must be 16-byte aligned device pointers");
+    if (lt_status arc = check_arrays(kv, n, {q, out, fused ? k : q, fused ? v : q}, "q, out, k and v")) return arc;
     if (gather) {
         if (!kv->peer.ready) return fail(kv, LT_E_ARG, "attend_gather before lt_kv_peer_import");
         if (n > kv->peer.max_tokens)
@@ -1215,11 +1222,8 @@ lt_status lt_kv_write(lt_kv* kv, uint32_t layer, const int32_t* block, const int
     if ((rc = take_cells(kv, block, slot, n, kv->fmt == LT_KV_Q4_0))) return rc;
     DeviceGuard g(kv->cfg.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (kv->fmt == LT_KV_Q4_0) {
-        if ((reinterpret_cast<uintptr_t>(k) & 15) || (reinterpret_cast<uintptr_t>(v) & 15))
-            return fail(kv, LT_E_ARG, "k and v must be 16-byte aligned device pointers");
-        if ((rc = refuse_capture(kv, st, "lt_kv_write to a 4-bit cache"))) return rc;
-    }
+    if ((rc = check_arrays(kv, n, {k, v}, "k and v"))) return rc;
+    if (kv->fmt == LT_KV_Q4_0 && (rc = refuse_capture(kv, st, "lt_kv_write to a 4-bit cache"))) return rc;
     if ((rc = flush(kv, st))) return rc;
     if (n == 0) return LT_OK;
     SlotHold hold(kv);
@@ -1547,6 +1551,7 @@ lt_status lt_kv_rows(lt_kv* kv, uint32_t layer, uint32_t seq, uint32_t n, void* 
     if (rc) return rc;
     if (layer >= kv->cfg.n_layers || seq >= kv->cfg.max_seqs || n > kv->lens[seq])
         return fail(kv, LT_E_ARG, "rows(layer %u, seq %u, n %u) out of range", layer, seq, n);
+    if ((rc = check_arrays(kv, n, {k_out, v_out}, "k_out and v_out"))) return rc;
     DeviceGuard g(kv->cfg.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (kv->fmt == LT_KV_Q4_0 && (rc = refuse_capture(kv, st, "lt_kv_rows of a 4-bit cache"))) return rc;
@@ -1567,8 +1572,7 @@ lt_status lt_kv_read(lt_kv* kv, uint32_t layer, const int32_t* block, const int3
     if (rc || (rc = require_device(kv))) return rc;
     if (layer >= kv->cfg.n_layers) return fail(kv, LT_E_ARG, "layer %u out of range", layer);
     if ((rc = take_cells(kv, block, slot, n, false))) return rc;
-    if ((reinterpret_cast<uintptr_t>(k_out) & 15) || (reinterpret_cast<uintptr_t>(v_out) & 15))
-        return fail(kv, LT_E_ARG, "k_out and v_out must be 16-byte aligned device pointers");
+    if ((rc = check_arrays(kv, n, {k_out, v_out}, "k_out and v_out"))) return rc;
     DeviceGuard g(kv->cfg.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if ((rc = refuse_capture(kv, st, "lt_kv_read"))) return rc;

@@ -50,7 +50,7 @@ cudaError_t CUDARTAPI cudaStreamIsCapturing(cudaStream_t, cudaStreamCaptureStatu
 namespace {
 std::function<void(const ltkv::AttnParams&, const ltkv::AttnShapedParams*)> on_attend;
 std::function<void(const ltkv::PrefixParams&, int)> on_prefix;
-int n_attend = 0, n_prefix = 0, n_plan = 0;
+int n_attend = 0, n_prefix = 0, n_plan = 0, n_write = 0, n_rows = 0;
 }  // namespace
 namespace ltkv {
 int attend_warps(int, int, int, int, int, bool) { return 1184; }
@@ -76,13 +76,16 @@ cudaError_t launch_expand_q4(const uint8_t*, const int32_t*, int, const ExpandGr
     return cudaSuccess;
 }
 cudaError_t launch_write(uint16_t*, const int2*, int, int, int, int, const void*, const void*, int, int, cudaStream_t) {
+    ++n_write;
     return cudaSuccess;
 }
 cudaError_t launch_read(const uint16_t*, const int2*, int, int, int, int, void*, void*, int, int, cudaStream_t) {
+    ++n_rows;
     return cudaSuccess;
 }
 cudaError_t launch_rows(const uint16_t*, const int32_t*, int, int, int, uint16_t*, uint16_t*, int, int, int32_t*,
                         cudaStream_t) {
+    ++n_rows;
     return cudaSuccess;
 }
 cudaError_t launch_apply_plan(uint16_t*, size_t, size_t, int, const int2*, int, int32_t* tables, const int2* tw, int n_tw,
@@ -181,6 +184,38 @@ void capture(uint32_t fmt, bool shaped) {
     NEED(c.attend(shaped ? &score : nullptr) == LT_OK && n_attend == 1, "%s", lt_kv_last_error(c.kv));
 }
 
+// Device pointers that the kernels' 16-byte accesses cannot take, or that are
+// none, are refused before anything is queued; with no tokens none is looked at.
+void pointers(uint32_t fmt) {
+    Cache c(fmt, 2, 2, 16 * 16, 2, 64);
+    c.fill(0, 20);
+    alignas(16) static char buf[64];
+    void *ok = buf, *odd = buf + 2;
+    const int32_t block = 0, slot = 3;
+    const uint32_t seq = 0, pos = 19;
+    int32_t last[2];
+    NEED(lt_kv_seq_blocks(c.kv, 0, last, 2) == 2, "blocks");
+    auto refused = [&](lt_status rc, const char* what) {
+        NEED(rc == LT_E_ARG && n_plan == 0 && n_attend == 0 && n_write == 0 && n_rows == 0, "%s: status %d", what, rc);
+    };
+    for (void* bad : {odd, (void*)nullptr})
+        for (int which = 0; which < 2; ++which) {
+            void *a = which ? ok : bad, *b = which ? bad : ok;
+            refused(lt_kv_write(c.kv, 0, &block, &slot, 1, a, b, LT_F16, nullptr), "write");
+            refused(lt_kv_rows(c.kv, 0, 0, 20, a, b, nullptr), "rows");
+            refused(lt_kv_read(c.kv, 0, &block, &slot, 1, a, b, LT_F16, nullptr), "read");
+            refused(lt_kv_attend(c.kv, 0, a, LT_F32, &seq, &pos, 1, b, LT_F32, 1.f, nullptr), "attend");
+            const int32_t own = 3;
+            refused(lt_kv_write_attend(c.kv, 0, &last[1], &own, a, b, LT_F32, ok, LT_F32, &seq, &pos, 1, ok, LT_F32, 1.f,
+                                       nullptr), "write_attend");
+        }
+    NEED(lt_kv_write(c.kv, 0, nullptr, nullptr, 0, nullptr, nullptr, LT_F16, nullptr) == LT_OK, "no tokens");
+    NEED(lt_kv_read(c.kv, 0, nullptr, nullptr, 0, nullptr, nullptr, LT_F16, nullptr) == LT_OK, "no tokens");
+    NEED(lt_kv_rows(c.kv, 0, 0, 0, nullptr, nullptr, nullptr) == LT_OK, "no rows");
+    NEED(lt_kv_attend(c.kv, 0, nullptr, LT_F32, nullptr, nullptr, 0, nullptr, LT_F32, 1.f, nullptr) == LT_OK, "no tokens");
+    NEED(lt_kv_write(c.kv, 0, &block, &slot, 1, ok, ok, LT_F16, nullptr) == LT_OK && n_write == 1, "write");
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -189,6 +224,9 @@ int main(int argc, char** argv) {
     else if (what == "staging-q8_0") staging(LT_KV_Q8_0);
     else if (what == "capture-q4_0") capture(LT_KV_Q4_0, false);
     else if (what == "capture-shaped") capture(LT_KV_F16, true);
+    else if (what == "pointers-f16") pointers(LT_KV_F16);
+    else if (what == "pointers-q8_0") pointers(LT_KV_Q8_0);
+    else if (what == "pointers-q4_0") pointers(LT_KV_Q4_0);
     else return std::printf("no scenario '%s'\n", what.c_str()), 2;
     std::printf("ok\n");
     return 0;

@@ -41,3 +41,10 @@ def test_a_refused_capture_leaves_no_trace(host_launch, what):
     """Attention over a 4-bit cache and with shaped scores is refused inside a
     capture before anything is queued on the stream, whatever the call holds."""
     host_launch(f"capture-{what}")
+
+
+@pytest.mark.parametrize("fmt", ["f16", "q8_0", "q4_0"])
+def test_pointers_are_checked_before_the_launch(host_launch, fmt):
+    """Null or misaligned device arrays, of which a kernel's 16-byte accesses would
+    fault, are refused by every call that takes them, for every cache format."""
+    host_launch(f"pointers-{fmt}")
