@@ -23,6 +23,14 @@
  * stream; their device-side effect is applied, in call order, right before
  * the next kernel-launching call.
  *
+ * Captures.  A call stages its cells and descriptors in buffers that later
+ * calls reuse, and its kernels hand split results over by flags that hold the
+ * call's number; a replay would find another call's staging and its own flags
+ * already up.  Calls on a 4-bit cache, shaped attention and lt_kv_read refuse
+ * a capturing stream.  The other calls do not look, and the same holds for
+ * them: a replay of attention that splits a sequence over warps may merge
+ * before this replay's parts are written.
+ *
  * Pointers.  Arguments named *_host are host memory; `k`, `v`, `q`, `out`
  * and the pointers of lt_kv_rows and lt_kv_read are device memory, 16-byte
  * aligned (other pointers, and null ones of a call of some rows, are refused
@@ -177,8 +185,9 @@ lt_status lt_kv_attend(lt_kv* kv, uint32_t layer, const void* q, lt_dtype q_dtyp
  * first_host NULL counts as 0, end_host NULL as p + 1 (causal), window 0 as no
  * window.  end[i] may lie past p + 1 (a bidirectional prefix) but not past the
  * sequence; a token whose interval is empty answers zero.  Blocks outside the
- * interval are not read, and nothing that a masked cell holds (Inf, NaN)
- * reaches an output. */
+ * interval are not read (a 4-bit cache's prefill chunks: blocks outside the
+ * intervals of a sequence's tokens taken together), and nothing that a masked
+ * cell holds (Inf, NaN) reaches an output. */
 typedef struct lt_kv_score {
     float softcap;              /* 0 .. 1e30; 0: no cap                         */
     uint32_t window;            /* positions before and with the token's own;    0: all */

@@ -28,9 +28,9 @@ using ltkv::kBlock;
 namespace {
 
 constexpr int kSlots = 8;  // staging ring depth (pinned host + device pairs)
-constexpr uint32_t kCascadeMaxTokens = 1024;  // tokens of one call the prefix pass serves
+constexpr uint32_t kCascadeMaxTokens = 1024;  // tokens of one call the prefix pass serves (what its partials' memory holds)
 constexpr int kCascadeMinBlocks = 4;          // shortest shared prefix worth a pass (64 positions)
-constexpr size_t kExpandBytes = 128u << 20;   // f16 workspace of a 4-bit cache's prefix pass
+constexpr size_t kExpandBytes = 128u << 20;   // f16 workspace of a 4-bit cache's prefix pass, at most
 constexpr uint32_t kWholeMinTokens = 8;       // tokens of a sequence in a call that the prefix pass attends whole
 constexpr long long kSmallTiles = 1184;       // tiles of an attention call that counts as small
 constexpr uint32_t kClean = 0xFFFFFFFFu;
@@ -530,7 +530,8 @@ lt_status take_cells(lt_kv* kv, const int32_t* block, const int32_t* slot, uint3
 }
 
 // The launches of a call read staging slots and flags tagged for that call,
-// which a replayed graph would not refresh.
+// which a replayed graph would not refresh (the f16 and Q8_0 calls' too, which
+// have never been refused).
 lt_status refuse_capture(lt_kv* kv, cudaStream_t st, const char* what) {
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
     LT_CUDA(kv, cudaStreamIsCapturing(st, &cs));
@@ -682,8 +683,10 @@ int plan_cascade(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, uint32_t n
 // A call of prefill chunks alone over a 4-bit cache: every sequence has at least
 // cascade_min_tokens tokens in it (and kWholeMinTokens: fewer would leave the
 // pass's 128 rows empty), one after the other, the workspace holds all their
-// blocks, and the items (KV head x 128 / group tokens) leave no SMs to split long
-// ones over.  Then the pass attends every token's positions, its own block's too,
+// blocks, and the items (KV head x 128 / group tokens) fill more than half the SMs
+// or are short: plan_cascade splits long ones over idle SMs, which this cannot, as
+// a split's rows are partials (a shaped call, which plan_cascade does not take, then
+// goes through the stream-K launch a token at a time).  Then the pass attends every token's positions, its own block's too,
 // and writes the outputs; nothing is left for the stream-K launch.  (Of 160 us for
 // 4 x 256 tokens over 2048, 8 x 128, the launch for the tokens' own blocks took 30.)
 // Fills casc_buf and exp_groups as plan_cascade does, items for no split; returns
@@ -736,7 +739,7 @@ int plan_whole(lt_kv* kv, const uint32_t* seq, const uint32_t* pos, const ltkv::
         }
         used += count;
     }
-    if (items.size() * 2 <= (size_t)kv->sm_count && longest >= 2 * 4) return 0;  // plan_cascade would split these
+    if (items.size() * 2 <= (size_t)kv->sm_count && longest >= 2 * 4) return 0;  // few and long
     const size_t item_words = items.size() * (sizeof(ltkv::PrefixItem) / 4);
     kv->casc_buf.resize(item_words + (shapes ? 4 : 2) * (size_t)n);
     std::memcpy(kv->casc_buf.data(), items.data(), items.size() * sizeof(ltkv::PrefixItem));

@@ -84,7 +84,7 @@ struct AttnParams {
     const float* pre_ml;         // [pre_splits][rows][2]: its (m, l); row = (token*n_kv_heads + h)*group + g
     int32_t pre_splits;          // partials per row (the prefix blocks split over that many CTAs)
     int64_t pre_split_rows;      // rows between split slabs
-    int32_t fmt;                 // lt_kv_format of the pool's tiles; prefix partials only for LT_KV_F16
+    int32_t fmt;                 // lt_kv_format of the pool's tiles; LT_KV_Q8_0 has no prefix partials
     // Head-sharded gather over NVLink (lt_kv_attend_gather).  With n_peers > 0
     // every output row goes, instead of to `out`, to this rank's gather half
     // gather_out at row tok*(n_peers*n_heads) + peer_rank*n_heads + head, and

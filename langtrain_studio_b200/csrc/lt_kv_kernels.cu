@@ -995,12 +995,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attn_kernel(const __grid
 //                  (each accumulation of the tensor core rounds O towards zero).
 // The pool's 16 x 64 sub-tiles are already the 128-byte-swizzled K-major (K)
 // and MN-major (V) operand layouts, so the tiles go from the bulk copy
-// straight to the tensor cores.  SH: scores of lt_kv_score, of 4-bit caches alone,
-// whose masked cells hold no Inf or NaN that 0 * V could spread.  At the end each
-// row writes (m, l, O), or, of a call whose every token is attended here whole
+// straight to the tensor cores.  An f16 V may hold Inf or NaN in a row that some of the
+// 128 rows are masked for, and 0 * Inf is NaN: there the products of a block leave those
+// rows of O alone (2 % of a chunked prefill call).  Blocks are masked whole there; SH,
+// scores of lt_kv_score, masks inside a block and is for 4-bit tiles alone, whose values
+// are finite.  At the end each row writes (m, l, O), or, of a call whose every token is attended here whole
 // (p.out), O / l as its output.
 // What bounds it: the chain P(j) -> P V and S two steps on -> softmax, ~1.25 us a
-// step of 64 positions where the MMAs alone need ~0.45.  Half the columns a
+// step of 64 positions where the MMAs alone need ~0.45 (4 x 256 tokens over 2048,
+// f16 q: 101 us with the 4-bit tiles' expansion).  Half the columns a
 // thread gave 1 % (the exponentials are not the bound: without them the time is the
 // same), a fourth stage for f16 q 4 % (it has no place beside an f32 q's residual).
 // Every wait is bounded; on a timeout the CTA sets the error flag, drains
@@ -1020,11 +1023,9 @@ __device__ __forceinline__ uint32_t f16_idesc(int n, bool b_mn_major) {
     return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-// Called by a whole converged warp, one elected lane of which issues.  (In a
-// branch that one lane alone takes the compiler cannot hold the operands in
-// uniform registers and moves all of them there for every instruction: the
-// issue, not the tensor cores, then bounds the pass; 4 x 256 tokens over 2048,
-// f16 q: 123 us against 106.)
+// Called by a whole converged warp, one elected lane of which issues: a loop that
+// one lane runs alone takes 123 us where this takes 106 (4 x 256 tokens over
+// 2048 of a 4-bit cache, f16 q).
 __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t accumulate) {
     asm volatile(
@@ -1193,7 +1194,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefix_attn_kernel(const __gri
     const int32_t* trow = p.tables + (int64_t)item.root_seq * p.max_blocks + item.blk0;
     const size_t tile_elems = 2 * kBlock * D;
     auto step_blocks = [&](int j) { return min(kPreStepBlocks, nbk - j * kPreStepBlocks); };
-    int issued = 0;  // warp 5 lane 0: steps whose copies were issued
+    int issued = 0;  // copy warp, lane 0: steps whose copies were issued
     // The step's block ids, loaded together (independent loads) a step ahead
     // of the copies that use them.
     auto load_ids = [&](int j, int (&ids)[kPreStepBlocks]) {
