@@ -27,9 +27,10 @@
  * calls reuse, and its kernels hand split results over by flags that hold the
  * call's number; a replay would find another call's staging and its own flags
  * already up.  Calls on a 4-bit cache, shaped attention and lt_kv_read refuse
- * a capturing stream.  The other calls do not look, and the same holds for
- * them: a replay of attention that splits a sequence over warps may merge
- * before this replay's parts are written.
+ * a capturing stream.  The other calls of a handle do not look, and the same
+ * holds for them: a replay of attention that splits a sequence over warps may
+ * merge before this replay's parts are written.  lt_paged_attend_noalloc has
+ * no handle and can be captured.
  *
  * Pointers.  Arguments named *_host are host memory; `k`, `v`, `q`, `out`
  * and the pointers of lt_kv_rows and lt_kv_read are device memory, 16-byte
@@ -465,7 +466,9 @@ lt_status lt_kv_write_attend_gather(lt_kv* kv, uint32_t layer, const int32_t* bl
  *     LT_E_SCRATCH before any work.  Calls of more than 512 tokens run as
  *     consecutive launches on `stream`.
  *   - The first call on a device looks up the array's address with that
- *     device current; make that first call before any stream capture.
+ *     device current; make that first call before any stream capture.  A
+ *     captured call clears the flags first, so that its replays merge nothing
+ *     stale.
  *   - All calls share the array and it keeps the last call's contents; each
  *     launch tags its flags with a fresh epoch and rewrites the partials it
  *     reads.  Calls that overlap on the GPU race: issue them in order on

@@ -129,6 +129,9 @@ extern "C" lt_status lt_paged_attend_noalloc(const void* pool_layer, uint32_t kv
     if (scratch_ptr(&dev, &base) != cudaSuccess) return LT_E_CUDA;
     unsigned char* b = static_cast<unsigned char*>(base);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) return LT_E_CUDA;
+    const bool captured = capture != cudaStreamCaptureStatusNone;
     const int q_f32 = q_dtype == LT_F32;
     const int max_warps = ltkv::attend_warps(dev, (int)group, (int)head_dim, q_f32, 0);
     if (max_warps <= 0) return LT_E_CUDA;
@@ -177,12 +180,13 @@ extern "C" lt_status lt_paged_attend_noalloc(const void* pool_layer, uint32_t kv
         // The flags keep earlier launches' epochs: a fresh epoch per launch on
         // this device (the array starts zeroed, and 0 is never used).  When the
         // count wraps, any earlier epoch may still be there, so the flags are
-        // cleared.
+        // cleared.  So they are in a captured call, each replay of which has the
+        // same epoch: a merge must not take the flags of the replay before.
         p.flags = reinterpret_cast<uint32_t*>(b + kFlagsOffset);
         uint32_t epoch = g_epoch[dev] + 1;
-        if (epoch == 0) {
+        if (epoch == 0 || captured) {
             if (cudaMemsetAsync(b + kFlagsOffset, 0, kFlagsBytes, st) != cudaSuccess) return LT_E_CUDA;
-            epoch = 1;
+            epoch = std::max(epoch, 1u);
         }
         g_epoch[dev] = epoch;
         p.epoch = epoch;

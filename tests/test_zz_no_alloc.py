@@ -170,3 +170,50 @@ def test_noalloc_rejects_oversized_requests_and_q8_pools():
     assert _noalloc(lib, kv, 0, q[:1], out[:1], [0], [0], 0.125, kv_format=N.LT_KV_Q8_0) == N.LT_E_UNSUPPORTED
     assert lib.lt_paged_attend_noalloc_check(_stream()) == N.LT_OK
     kv.close()
+
+
+def test_captured_call_replays(oracle_mod):
+    """A captured call gives the eager call's bits at every replay, with q changed in
+    between and with other calls in between: the flags over which a sequence's parts
+    are merged do not stand from the replay before."""
+    from langtrain_studio_b200 import _native as N
+
+    lib = N.lib()
+    hq, hkv, d = 8, 1, 128
+    lens = [4000, 40]
+    kv, _, _ = _twin(oracle_mod, 1, hq, hkv, d, lens, 31)
+    scale = float(1 / np.sqrt(d))
+    g = torch.Generator(device="cuda").manual_seed(2)
+    seqs, pos = np.arange(2), np.array(lens) - 1
+    q = torch.empty((2, hq * d), device="cuda")
+    out, eager = torch.empty_like(q), torch.empty_like(q)
+    assert _noalloc(lib, kv, 0, q.zero_(), out, seqs, pos, scale) == N.LT_OK  # before any capture
+    torch.cuda.synchronize()
+    graph, st = torch.cuda.CUDAGraph(keep_graph=True), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=st):
+        assert _noalloc(lib, kv, 0, q, out, seqs, pos, scale) == N.LT_OK
+    # one launch, and before it a node that takes the flags down
+    runtime = pytest.importorskip("cuda.bindings.runtime")
+    handle = runtime.cudaGraph_t(graph.raw_cuda_graph())
+    _, _, n_nodes = runtime.cudaGraphGetNodes(handle)
+    _, nodes, _ = runtime.cudaGraphGetNodes(handle, n_nodes)
+    kinds = [runtime.cudaGraphNodeGetType(node)[1] for node in nodes[:n_nodes]]
+    kind = runtime.cudaGraphNodeType
+    assert sorted(kinds) == sorted([kind.cudaGraphNodeTypeMemset, kind.cudaGraphNodeTypeKernel])
+    graph.instantiate()
+    qs = [torch.randn(q.shape, generator=g, device="cuda") for _ in range(30)]
+    want = []
+    for x in qs:
+        assert _noalloc(lib, kv, 0, x, eager, seqs, pos, scale) == N.LT_OK
+        want.append(eager.clone())
+    for i, x in enumerate(qs):
+        q.copy_(x)
+        if i % 5 == 4:  # another call's flags and partials in the shared array
+            assert _noalloc(lib, kv, 0, x, eager, seqs[:1], pos[:1] // 2, scale) == N.LT_OK
+        out.zero_()
+        graph.replay()
+        got = out.clone()
+        assert lib.lt_paged_attend_noalloc_check(_stream()) == N.LT_OK
+        assert torch.equal(got, want[i]), i
+    del graph
+    kv.close()
